@@ -1,0 +1,95 @@
+// ccb_nn_dropout: out = residual + keep(e) * x / (1 - p), the mask a pure
+// function of (seed, offset, element index) that is never stored; the
+// gradient is the same call on dy without the residual.
+//
+// Bytes: x and the residual read once, out written once.
+#include "nn_common.cuh"
+
+namespace ccb_nn {
+namespace {
+
+struct DropoutP {
+  const void* x;
+  const void* res;
+  void* out;
+  i64 rows, cols, xs, rs, os;
+  Drop d;
+};
+
+// Any alignment, stride and base: a thread takes one block of the generator,
+// the up to four elements of the tensor that lie in it.
+template <class T>
+__global__ void __launch_bounds__(256) dropout_any(const __grid_constant__ DropoutP p) {
+  const u64 n = (u64)p.rows * (u64)p.cols;
+  const u64 q0 = p.d.base >> 2, q1 = (p.d.base + n - 1) >> 2;
+  const T* x = static_cast<const T*>(p.x);
+  const T* res = static_cast<const T*>(p.res);
+  T* out = static_cast<T*>(p.out);
+  const u64 step = (u64)gridDim.x * blockDim.x;
+  for (u64 q = q0 + (u64)blockIdx.x * blockDim.x + threadIdx.x; q <= q1; q += step) {
+    unsigned w[4] = {};
+    if (p.d.on) philox4(p.d, q, w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const u64 e = 4 * q + j;
+      if (e < p.d.base || e - p.d.base >= n) continue;
+      const i64 i = (i64)(e - p.d.base);
+      const i64 r = p.rows == 1 ? 0 : i / p.cols, c = i - r * p.cols;
+      const float v = to_f<T>(x[r * p.xs + c]);
+      float y = p.d.on ? dropped(p.d, w[j], v) : v * p.d.factor;
+      if (res) y += to_f<T>(res[r * p.rs + c]);
+      out[r * p.os + c] = from_f<T>(y);
+    }
+  }
+}
+
+template <class T>
+void go(const DropoutP& p, int sms, cudaStream_t st) {
+  const u64 n = (u64)p.rows * (u64)p.cols;
+  const u64 blocks = n / 4 + 2;
+  const u64 want = (blocks + 255) / 256, most = (u64)sms * 32;
+  dropout_any<T><<<(unsigned)(want < most ? want : most), 256, 0, st>>>(p);
+}
+
+}  // namespace
+}  // namespace ccb_nn
+
+using namespace ccb_nn;
+
+extern "C" int ccb_nn_dropout(const ccb_nn_dropout_t* a, void* stream) {
+  static const char* const me = "ccb_nn_dropout";
+  CCB_NN_GUARD(me, {
+    if (!a) return fail(CCB_ERR_INVALID, me, "null argument block");
+    if (!float_type(a->dtype)) return fail(CCB_ERR_INVALID, me, "dtype code " + std::to_string(a->dtype) + " (0 f32, 4 bf16, 5 f16)");
+    if (!(a->p >= 0.0 && a->p <= 1.0)) return fail(CCB_ERR_INVALID, me, "p = " + std::to_string(a->p) + " is outside [0, 1]");
+    if (!sane(a->rows, a->cols, a->x_stride) || !sane(a->rows, a->cols, a->out_stride) ||
+        (a->residual && !sane(a->rows, a->cols, a->residual_stride)) || (a->cols > 0 && a->rows > (1ll << 60) / a->cols))
+      return fail(CCB_ERR_INVALID, me, "rows, cols or a stride is out of range");
+    if (a->rows > 1 && (a->x_stride < a->cols || a->out_stride < a->cols || (a->residual && a->residual_stride < a->cols)))
+      return fail(CCB_ERR_INVALID, me, "a row stride is shorter than a row");
+    const i64 n = a->rows * a->cols;
+    if (n == 0) return CCB_OK;
+    if (a->base > ~0ull - (u64)n) return fail(CCB_ERR_INVALID, me, "base + rows * cols passes 2^64");
+    if (!a->x || !a->out) return fail(CCB_ERR_INVALID, me, "null pointer");
+    const int b = type_bytes(a->dtype);
+    if (!aligned(a->x, b) || !aligned(a->out, b) || !aligned(a->residual, b))
+      return fail(CCB_ERR_INVALID, me, "a pointer is not aligned to its element type");
+    int sms = 0;
+    if (const int rc = sm_count(me, &sms)) return rc;
+    DropoutP p = {a->x, a->residual, a->out, a->rows, a->cols, a->x_stride, a->residual_stride, a->out_stride,
+                  make_drop(a->p, a->seed, a->offset, a->base)};
+    // dense rows are one long row
+    if (p.rows > 1 && p.xs == p.cols && p.os == p.cols && (!p.res || p.rs == p.cols)) {
+      p.cols = n;
+      p.rows = 1;
+    }
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->dtype == CCB_F32)
+      go<float>(p, sms, st);
+    else if (a->dtype == CCB_BF16)
+      go<__nv_bfloat16>(p, sms, st);
+    else
+      go<__half>(p, sms, st);
+    return launched(me);
+  })
+}

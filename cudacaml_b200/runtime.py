@@ -114,6 +114,14 @@ def _declare(L):
         "ccb_comm_destroy": (I, [P]),
         "ccb_allreduce": (I, [P, P, P, SZ, I, I, P]),
         "ccb_sum_f32_noalloc": (I, [P, c.c_longlong, P, P]),
+        "ccb_nn_dropout": (I, [P, P]),
+        "ccb_nn_block_norm": (I, [P, P]),
+        "ccb_nn_block_norm_backward": (I, [P, P]),
+        "ccb_nn_block_norm_backward_workspace": (I, [c.c_longlong, c.c_longlong, c.POINTER(SZ)]),
+        "ccb_nn_grouped_matmul": (I, [P, P]),
+        "ccb_nn_grouped_matmul_workspace": (I, [P, c.POINTER(SZ)]),
+        "ccb_nn_grouped_matmul_dw": (I, [P, P]),
+        "ccb_nn_grouped_matmul_dw_workspace": (I, [P, c.POINTER(SZ)]),
         "ccb_ipc_mem_handle": (I, [P, c.POINTER(c.c_ubyte)]),
         "ccb_ipc_mem_open": (I, [c.POINTER(c.c_ubyte), c.POINTER(P)]),
         "ccb_ipc_mem_close": (I, [P]),

@@ -237,6 +237,119 @@ int ccb_graph_destroy(ccb_graph_t graph);
  * CCB_ERR_DRIVER, with the message in ccb_last_error(). */
 int ccb_sum_f32_noalloc(const float* x, long long n, float* out, void* stream);
 
+/* ---------------------------------------------------------------- residual blocks with experts
+ * No counterpart in the reference. Operators on caller-owned device memory,
+ * for training and serving a network whose residual blocks hold experts:
+ * dropout, the norms around a block fused with its gate and residual scale,
+ * and products grouped by expert. Each is issued on `stream` (NULL = legacy
+ * default) on the current device and does not synchronise; none allocates or
+ * keeps anything between calls, and each may be captured in a CUDA graph.
+ * Matrices are rows x cols with unit stride along a row and `*_stride`
+ * elements from one row to the next (at least cols). Element types are f32
+ * and, for these entry points alone, the two 16-bit codes below; arithmetic
+ * is in 32 bits and a result is rounded to its type once. Pointers are
+ * aligned to their element type. Outputs overlap no input unless an entry
+ * says so. An empty tensor is CCB_OK without a launch. */
+enum { CCB_F32 = 0, CCB_BF16 = 4, CCB_F16 = 5 };
+
+/* out = residual + keep(e) * x / (1 - p) (residual may be NULL). Element
+ * e = base + row * cols + col is dropped when word e % 4 of Philox-4x32-10 at
+ * the counter (e / 4 in 64 bits, offset in 64 bits) under the key `seed` is
+ * below round(p * 2^32); a dropped element gives residual + 0 whatever x
+ * holds. The mask is a function of (seed, offset, e) alone and is never
+ * stored: the gradient is the same call on dy with no residual. `base` is
+ * the index of the first element, so that ranks holding slices of one tensor
+ * draw that tensor's mask. out may be x or residual. */
+typedef struct {
+  const void* x;
+  const void* residual;
+  void* out;
+  long long rows, cols, x_stride, residual_stride, out_stride;
+  unsigned long long seed, offset, base;
+  double p;
+  int dtype;
+} ccb_nn_dropout_t;
+int ccb_nn_dropout(const ccb_nn_dropout_t* a, void* stream);
+
+/* The join of a residual block and the next block's norm, one pass:
+ *   u = norm(branch) * post_weight + post_bias      (u = branch if !post_norm)
+ *   y = x + scale * drop(act(gate) * u)
+ *   h = norm(y) * pre_weight + pre_bias             (from y before its rounding)
+ * norm(v) = v / sqrt(mean(v^2) + eps) for kind 0, (v - mean(v)) /
+ * sqrt(var(v) + eps) for kind 1, along a row. branch NULL: y = x (y must be
+ * NULL), h = norm(x). y or h may be NULL. Weights and biases are vectors of
+ * `cols` (NULL: 1 and 0) of type weight_dtype. gate NULL: 1; gate_stride 0:
+ * one row for all (a gate for each channel). act: 0 none, 1 sigmoid, 2 tanh.
+ * drop is ccb_nn_dropout's with p, seed, offset and base. x and y have type
+ * x_dtype (dtype, or f32), branch and h have dtype, the gate dtype or f32.
+ * y may be x. */
+typedef struct {
+  const void *x, *branch, *gate, *pre_weight, *pre_bias, *post_weight, *post_bias;
+  void *y, *h;
+  long long rows, cols, x_stride, branch_stride, gate_stride, y_stride, h_stride;
+  unsigned long long seed, offset, base;
+  double p, eps, scale;
+  int dtype, x_dtype, gate_dtype, weight_dtype, kind, act, post_norm;
+} ccb_nn_block_norm_t;
+int ccb_nn_block_norm(const ccb_nn_block_norm_t* a, void* stream);
+
+/* Its gradient, from the stored y and the forward pass's other inputs; the
+ * statistics are computed again. dy (of y) or dh (of h) may be NULL (zero),
+ * not both. dx has x_dtype and is the whole gradient of x (through y and h);
+ * dbranch has dtype, dgate the gate's type, or f32 summed over rows for
+ * gate_stride 0; dpre_weight, dpre_bias, dpost_weight, dpost_bias are f32
+ * vectors summed over rows in a fixed order. Any output may be NULL. dx may
+ * be dy, dbranch may be dh. workspace: at least
+ * ccb_nn_block_norm_backward_workspace bytes, 16-byte aligned, uninitialised. */
+typedef struct {
+  const void *y, *dy, *dh, *branch, *gate, *pre_weight, *post_weight, *post_bias;
+  void *dx, *dbranch, *dgate, *dpre_weight, *dpre_bias, *dpost_weight, *dpost_bias, *workspace;
+  long long rows, cols, y_stride, dy_stride, dh_stride, branch_stride, gate_stride, dx_stride, dbranch_stride, dgate_stride;
+  unsigned long long workspace_bytes, seed, offset, base;
+  double p, eps, scale;
+  int dtype, x_dtype, gate_dtype, weight_dtype, kind, act, post_norm;
+} ccb_nn_block_norm_backward_t;
+int ccb_nn_block_norm_backward(const ccb_nn_block_norm_backward_t* a, void* stream);
+int ccb_nn_block_norm_backward_workspace(long long rows, long long cols, size_t* bytes);
+
+/* Rows offsets[e] .. offsets[e+1] - 1 of x (rows x k) times matrix e of w
+ * (k x n, or n x k with transpose_w), for e in [0, experts): out is rows x n.
+ * Rows before offsets[0] and from offsets[experts] on give 0. `offsets` is
+ * experts + 1 i32 words in device memory, ascending, in [0, rows]: the host
+ * never learns them. Words out of order or range are clamped and raise bit 64
+ * of *err; a wait that ran out raises bit 16 (err may be NULL). Matrix e of w
+ * starts w_stride * e elements in, its rows w_row_stride apart. The gradient
+ * of x is the same call on dy with transpose_w flipped. Sums are in 32 bits,
+ * the same bits in every run. workspace: at least
+ * ccb_nn_grouped_matmul_workspace bytes, 16-byte aligned, uninitialised. */
+typedef struct {
+  const void *x, *w;
+  const int* offsets;
+  void *out, *workspace;
+  unsigned* err;
+  long long rows, experts, k, n, x_stride, w_stride, w_row_stride, out_stride;
+  unsigned long long workspace_bytes;
+  int dtype, transpose_w;
+} ccb_nn_grouped_matmul_t;
+int ccb_nn_grouped_matmul(const ccb_nn_grouped_matmul_t* a, void* stream);
+/* Bytes that a call with these sizes, strides and pointers needs (0: none;
+ * workspace, workspace_bytes, offsets and err are not read). */
+int ccb_nn_grouped_matmul_workspace(const ccb_nn_grouped_matmul_t* a, size_t* bytes);
+
+/* The gradient of w: matrix e of out (k x n) = (x rows of e)^T (dy rows of e),
+ * 0 for an expert without rows. out has dtype or f32 (out_dtype). */
+typedef struct {
+  const void *x, *dy;
+  const int* offsets;
+  void *out, *workspace;
+  unsigned* err;
+  long long rows, experts, k, n, x_stride, dy_stride, out_stride, out_row_stride;
+  unsigned long long workspace_bytes;
+  int dtype, out_dtype;
+} ccb_nn_grouped_matmul_dw_t;
+int ccb_nn_grouped_matmul_dw(const ccb_nn_grouped_matmul_dw_t* a, void* stream);
+int ccb_nn_grouped_matmul_dw_workspace(const ccb_nn_grouped_matmul_dw_t* a, size_t* bytes);
+
 /* ---------------------------------------------------------------- peer memory and the cross-rank sum
  * New: the reference has no collective (lib/backend_cuda/multi.ml:51-109
  * combines per-device results on the host). A rank exports a device

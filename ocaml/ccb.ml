@@ -162,6 +162,170 @@ let graph_destroy = fn "ccb_graph_destroy" (handle @-> returning int)
 (* ---------------------------------------------------------------- allocation-free sum (no reference counterpart) *)
 let sum_f32_noalloc = fn "ccb_sum_f32_noalloc" (ptr float @-> llong @-> ptr float @-> handle @-> returning int)
 
+(* ---------------------------------------------------------------- residual blocks with experts
+   (no reference counterpart). Each call reads its argument block and takes a
+   stream; element types are dtype codes 0 f32, 4 bf16, 5 f16. *)
+let bf16_code = 4
+let f16_code = 5
+
+type nn_dropout_t
+
+let nn_dropout_t : nn_dropout_t structure typ = structure "ccb_nn_dropout_t"
+let nd_x = field nn_dropout_t "x" (ptr void)
+let nd_residual = field nn_dropout_t "residual" (ptr void)
+let nd_out = field nn_dropout_t "out" (ptr void)
+let nd_rows = field nn_dropout_t "rows" llong
+let nd_cols = field nn_dropout_t "cols" llong
+let nd_x_stride = field nn_dropout_t "x_stride" llong
+let nd_residual_stride = field nn_dropout_t "residual_stride" llong
+let nd_out_stride = field nn_dropout_t "out_stride" llong
+let nd_seed = field nn_dropout_t "seed" ullong
+let nd_offset = field nn_dropout_t "offset" ullong
+let nd_base = field nn_dropout_t "base" ullong
+let nd_p = field nn_dropout_t "p" double
+let nd_dtype = field nn_dropout_t "dtype" int
+let () = seal nn_dropout_t
+
+type nn_block_norm_t
+
+let nn_block_norm_t : nn_block_norm_t structure typ = structure "ccb_nn_block_norm_t"
+let nb_x = field nn_block_norm_t "x" (ptr void)
+let nb_branch = field nn_block_norm_t "branch" (ptr void)
+let nb_gate = field nn_block_norm_t "gate" (ptr void)
+let nb_pre_weight = field nn_block_norm_t "pre_weight" (ptr void)
+let nb_pre_bias = field nn_block_norm_t "pre_bias" (ptr void)
+let nb_post_weight = field nn_block_norm_t "post_weight" (ptr void)
+let nb_post_bias = field nn_block_norm_t "post_bias" (ptr void)
+let nb_y = field nn_block_norm_t "y" (ptr void)
+let nb_h = field nn_block_norm_t "h" (ptr void)
+let nb_rows = field nn_block_norm_t "rows" llong
+let nb_cols = field nn_block_norm_t "cols" llong
+let nb_x_stride = field nn_block_norm_t "x_stride" llong
+let nb_branch_stride = field nn_block_norm_t "branch_stride" llong
+let nb_gate_stride = field nn_block_norm_t "gate_stride" llong
+let nb_y_stride = field nn_block_norm_t "y_stride" llong
+let nb_h_stride = field nn_block_norm_t "h_stride" llong
+let nb_seed = field nn_block_norm_t "seed" ullong
+let nb_offset = field nn_block_norm_t "offset" ullong
+let nb_base = field nn_block_norm_t "base" ullong
+let nb_p = field nn_block_norm_t "p" double
+let nb_eps = field nn_block_norm_t "eps" double
+let nb_scale = field nn_block_norm_t "scale" double
+let nb_dtype = field nn_block_norm_t "dtype" int
+let nb_x_dtype = field nn_block_norm_t "x_dtype" int
+let nb_gate_dtype = field nn_block_norm_t "gate_dtype" int
+let nb_weight_dtype = field nn_block_norm_t "weight_dtype" int
+let nb_kind = field nn_block_norm_t "kind" int
+let nb_act = field nn_block_norm_t "act" int
+let nb_post_norm = field nn_block_norm_t "post_norm" int
+let () = seal nn_block_norm_t
+
+type nn_block_norm_backward_t
+
+let nn_block_norm_backward_t : nn_block_norm_backward_t structure typ = structure "ccb_nn_block_norm_backward_t"
+let nbb_y = field nn_block_norm_backward_t "y" (ptr void)
+let nbb_dy = field nn_block_norm_backward_t "dy" (ptr void)
+let nbb_dh = field nn_block_norm_backward_t "dh" (ptr void)
+let nbb_branch = field nn_block_norm_backward_t "branch" (ptr void)
+let nbb_gate = field nn_block_norm_backward_t "gate" (ptr void)
+let nbb_pre_weight = field nn_block_norm_backward_t "pre_weight" (ptr void)
+let nbb_post_weight = field nn_block_norm_backward_t "post_weight" (ptr void)
+let nbb_post_bias = field nn_block_norm_backward_t "post_bias" (ptr void)
+let nbb_dx = field nn_block_norm_backward_t "dx" (ptr void)
+let nbb_dbranch = field nn_block_norm_backward_t "dbranch" (ptr void)
+let nbb_dgate = field nn_block_norm_backward_t "dgate" (ptr void)
+let nbb_dpre_weight = field nn_block_norm_backward_t "dpre_weight" (ptr void)
+let nbb_dpre_bias = field nn_block_norm_backward_t "dpre_bias" (ptr void)
+let nbb_dpost_weight = field nn_block_norm_backward_t "dpost_weight" (ptr void)
+let nbb_dpost_bias = field nn_block_norm_backward_t "dpost_bias" (ptr void)
+let nbb_workspace = field nn_block_norm_backward_t "workspace" (ptr void)
+let nbb_rows = field nn_block_norm_backward_t "rows" llong
+let nbb_cols = field nn_block_norm_backward_t "cols" llong
+let nbb_y_stride = field nn_block_norm_backward_t "y_stride" llong
+let nbb_dy_stride = field nn_block_norm_backward_t "dy_stride" llong
+let nbb_dh_stride = field nn_block_norm_backward_t "dh_stride" llong
+let nbb_branch_stride = field nn_block_norm_backward_t "branch_stride" llong
+let nbb_gate_stride = field nn_block_norm_backward_t "gate_stride" llong
+let nbb_dx_stride = field nn_block_norm_backward_t "dx_stride" llong
+let nbb_dbranch_stride = field nn_block_norm_backward_t "dbranch_stride" llong
+let nbb_dgate_stride = field nn_block_norm_backward_t "dgate_stride" llong
+let nbb_workspace_bytes = field nn_block_norm_backward_t "workspace_bytes" ullong
+let nbb_seed = field nn_block_norm_backward_t "seed" ullong
+let nbb_offset = field nn_block_norm_backward_t "offset" ullong
+let nbb_base = field nn_block_norm_backward_t "base" ullong
+let nbb_p = field nn_block_norm_backward_t "p" double
+let nbb_eps = field nn_block_norm_backward_t "eps" double
+let nbb_scale = field nn_block_norm_backward_t "scale" double
+let nbb_dtype = field nn_block_norm_backward_t "dtype" int
+let nbb_x_dtype = field nn_block_norm_backward_t "x_dtype" int
+let nbb_gate_dtype = field nn_block_norm_backward_t "gate_dtype" int
+let nbb_weight_dtype = field nn_block_norm_backward_t "weight_dtype" int
+let nbb_kind = field nn_block_norm_backward_t "kind" int
+let nbb_act = field nn_block_norm_backward_t "act" int
+let nbb_post_norm = field nn_block_norm_backward_t "post_norm" int
+let () = seal nn_block_norm_backward_t
+
+type nn_grouped_matmul_t
+
+let nn_grouped_matmul_t : nn_grouped_matmul_t structure typ = structure "ccb_nn_grouped_matmul_t"
+let ng_x = field nn_grouped_matmul_t "x" (ptr void)
+let ng_w = field nn_grouped_matmul_t "w" (ptr void)
+let ng_offsets = field nn_grouped_matmul_t "offsets" (ptr void)
+let ng_out = field nn_grouped_matmul_t "out" (ptr void)
+let ng_workspace = field nn_grouped_matmul_t "workspace" (ptr void)
+let ng_err = field nn_grouped_matmul_t "err" (ptr void)
+let ng_rows = field nn_grouped_matmul_t "rows" llong
+let ng_experts = field nn_grouped_matmul_t "experts" llong
+let ng_k = field nn_grouped_matmul_t "k" llong
+let ng_n = field nn_grouped_matmul_t "n" llong
+let ng_x_stride = field nn_grouped_matmul_t "x_stride" llong
+let ng_w_stride = field nn_grouped_matmul_t "w_stride" llong
+let ng_w_row_stride = field nn_grouped_matmul_t "w_row_stride" llong
+let ng_out_stride = field nn_grouped_matmul_t "out_stride" llong
+let ng_workspace_bytes = field nn_grouped_matmul_t "workspace_bytes" ullong
+let ng_dtype = field nn_grouped_matmul_t "dtype" int
+let ng_transpose_w = field nn_grouped_matmul_t "transpose_w" int
+let () = seal nn_grouped_matmul_t
+
+type nn_grouped_matmul_dw_t
+
+let nn_grouped_matmul_dw_t : nn_grouped_matmul_dw_t structure typ = structure "ccb_nn_grouped_matmul_dw_t"
+let ngw_x = field nn_grouped_matmul_dw_t "x" (ptr void)
+let ngw_dy = field nn_grouped_matmul_dw_t "dy" (ptr void)
+let ngw_offsets = field nn_grouped_matmul_dw_t "offsets" (ptr void)
+let ngw_out = field nn_grouped_matmul_dw_t "out" (ptr void)
+let ngw_workspace = field nn_grouped_matmul_dw_t "workspace" (ptr void)
+let ngw_err = field nn_grouped_matmul_dw_t "err" (ptr void)
+let ngw_rows = field nn_grouped_matmul_dw_t "rows" llong
+let ngw_experts = field nn_grouped_matmul_dw_t "experts" llong
+let ngw_k = field nn_grouped_matmul_dw_t "k" llong
+let ngw_n = field nn_grouped_matmul_dw_t "n" llong
+let ngw_x_stride = field nn_grouped_matmul_dw_t "x_stride" llong
+let ngw_dy_stride = field nn_grouped_matmul_dw_t "dy_stride" llong
+let ngw_out_stride = field nn_grouped_matmul_dw_t "out_stride" llong
+let ngw_out_row_stride = field nn_grouped_matmul_dw_t "out_row_stride" llong
+let ngw_workspace_bytes = field nn_grouped_matmul_dw_t "workspace_bytes" ullong
+let ngw_dtype = field nn_grouped_matmul_dw_t "dtype" int
+let ngw_out_dtype = field nn_grouped_matmul_dw_t "out_dtype" int
+let () = seal nn_grouped_matmul_dw_t
+
+let nn_dropout = fn "ccb_nn_dropout" (ptr nn_dropout_t @-> handle @-> returning int)
+let nn_block_norm = fn "ccb_nn_block_norm" (ptr nn_block_norm_t @-> handle @-> returning int)
+let nn_block_norm_backward = fn "ccb_nn_block_norm_backward" (ptr nn_block_norm_backward_t @-> handle @-> returning int)
+
+let nn_block_norm_backward_workspace =
+  fn "ccb_nn_block_norm_backward_workspace" (llong @-> llong @-> ptr size_t @-> returning int)
+
+let nn_grouped_matmul = fn "ccb_nn_grouped_matmul" (ptr nn_grouped_matmul_t @-> handle @-> returning int)
+
+let nn_grouped_matmul_workspace =
+  fn "ccb_nn_grouped_matmul_workspace" (ptr nn_grouped_matmul_t @-> ptr size_t @-> returning int)
+
+let nn_grouped_matmul_dw = fn "ccb_nn_grouped_matmul_dw" (ptr nn_grouped_matmul_dw_t @-> handle @-> returning int)
+
+let nn_grouped_matmul_dw_workspace =
+  fn "ccb_nn_grouped_matmul_dw_workspace" (ptr nn_grouped_matmul_dw_t @-> ptr size_t @-> returning int)
+
 (* ---------------------------------------------------------------- peer memory and the cross-rank sum
    (no reference counterpart) *)
 let ipc_mem_handle = fn "ccb_ipc_mem_handle" (ptr void @-> ptr uchar @-> returning int)
