@@ -2,6 +2,8 @@
 // expert. The row ranges of the experts live in device memory, so every block
 // lays the tiles out for itself: it clamps the offsets, counts the row tiles
 // of each segment and scans the counts in shared memory.
+#include "ccb_skel.cuh"
+#include "dyn.hpp"
 #include "nn_common.cuh"
 
 namespace ccb_nn {
@@ -202,6 +204,374 @@ void any_dw(const GroupDwP& p, int sms, cudaStream_t st) {
   grouped_dw_any<T, TO><<<(unsigned)(tiles < most ? tiles : most), 256, 0, st>>>(p);
 }
 
+// ------------------------------------------------------------ tensor cores
+// One kernel for the three products, on pairs of SMs (cta_group::2). The MMA's
+// 256-high M side holds output features (a weight's columns, or dy's), its N
+// side the ragged dimension: the tokens of one expert, or x's columns for dw.
+// So a short range costs what it holds (N is any multiple of 32), the pair's
+// accumulators have consecutive features in consecutive TMEM lanes, and a
+// warp's stores of one token are contiguous without a transpose.
+//
+// Warps of each CTA: 0 TMA producer (a ring of 6 stages, 64 of the contraction
+// each: 128 features of the M side and half of the N side), 1 MMA issuer (of
+// the even CTA, for both), 2-5 drain one of two accumulators while the other
+// fills, 6 (dw) clears the rows past an expert's end: the contraction runs
+// over rows there, so what the next expert holds must not reach the sum. Both
+// CTAs' copies complete on the even CTA's barrier; copies whose rows have to
+// be cleared complete on the CTA's own, and warp 6 passes them on.
+//
+// Every tile is dealt out round-robin; a segment's rows are cut evenly, so
+// that no tile is a short remainder.
+namespace tcg {
+constexpr int kFeat = 256, kTok = 256, kBK = 64, kStages = 6;
+constexpr unsigned kABytes = 128 * kBK * 2, kBBytes = 128 * kBK * 2, kStageBytes = kABytes + kBBytes;
+constexpr unsigned kTmemCols = 512;
+constexpr int kThreads = 224;
+constexpr unsigned kErrWait = 16u;
+
+struct Tail {  // after the ring
+  ccb::u64 full[kStages], empty[kStages], part[kStages], accf[2], acce[2];
+  unsigned tmem;
+  Segments g;
+};
+constexpr unsigned kSmem = kStages * kStageBytes + sizeof(Tail) + 1024;
+
+struct P {
+  ccb::TmaDesc ta, tb;  // M side, N side
+  const int* off;
+  void* out;
+  unsigned* err;
+  i64 os, oe;           // strides of out: a row, an expert's matrix (dw)
+  i64 split_stride;     // elements from one part's result to the next
+  int rows, experts, n, k, splits, format;
+};
+
+// Acquires at cluster scope: what the pair's other CTA wrote before it arrived.
+__device__ __forceinline__ bool try_wait(ccb::u64* bar, unsigned parity) {
+  unsigned ok;
+  asm volatile(
+      "{\n .reg .pred q;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 q, [%1], %2;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(ok)
+      : "r"(ccb::smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded; once a wait has run out the thread's later ones hardly poll, so
+// that the kernel ends (with the error bit raised and `out` undefined).
+struct Waiter {
+  unsigned limit = ccb::MBAR_SPIN_LIMIT;
+  unsigned* err;
+  __device__ __forceinline__ explicit Waiter(unsigned* e) : err(e) {}
+  __device__ __forceinline__ void operator()(ccb::u64* bar, unsigned parity) {
+    for (unsigned it = 0; it < limit; ++it)
+      if (try_wait(bar, parity)) return;
+    if (err) atomicOr(err, kErrWait);
+    limit = 64;
+  }
+};
+
+__device__ __forceinline__ void load3(unsigned dst, const ccb::TmaDesc* map, int x, int y, int z, unsigned bar) {
+  ccb::tc2::tma_load_3d(dst, map, x, y, z, bar);
+}
+__device__ __forceinline__ void load4(unsigned dst, const ccb::TmaDesc* map, int x, int y, int z, int w, unsigned bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"((unsigned long long)map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma(unsigned d, ccb::u64 a, ccb::u64 b, unsigned idesc, unsigned accumulate) {
+  const unsigned z = 0;
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z));
+}
+// 16-bit operands, 128-byte swizzle. K-major: 128-byte rows of 64 along the
+// contraction, 8-row groups 1024 bytes apart, 16 of the contraction 32 bytes
+// further. MN-major: 64 along M or N are one 128-byte row, one row for each
+// step of the contraction, 8-row groups 1024 bytes apart, the next 64 along M
+// or N 8192 bytes on, 16 of the contraction 2048 bytes further.
+__device__ __forceinline__ ccb::u64 desc_k(unsigned tile, int kk) { return ccb::tc::desc_k(tile, kk); }
+__device__ __forceinline__ ccb::u64 desc_mn(unsigned tile, int kk) {
+  return ccb::tc::sdesc(tile + kk * 2048u, 8192u, 1024u, ccb::tc::LAYOUT_SW128);
+}
+
+struct Tile {
+  int expert;      // -1: rows of no expert
+  int r0, r1;      // rows: of the result (forward), of the contraction (dw)
+  int f0, c0;      // first feature; first column of x (dw)
+  int nn;          // N of the MMA
+  int b0, b1;      // steps of the contraction
+  int split;
+};
+enum { kForward = 0, kForwardT = 1, kDw = 2 };
+
+template <int MODE>
+__device__ __forceinline__ i64 tiles_of(const P& p, const Segments& g) {
+  const i64 nf = (p.n + kFeat - 1) / kFeat;
+  if (MODE == kDw) return nf * ((p.k + kTok - 1) / kTok) * p.experts * p.splits;
+  return nf * g.tile[p.experts + 2] * p.splits;
+}
+// Tile t: features innermost, then the parts of the contraction, then tokens:
+// the pairs work on one expert's matrix at a time, which stays in L2.
+template <int MODE>
+__device__ __forceinline__ Tile tile_at(const P& p, const Segments& g, i64 t) {
+  Tile o;
+  const int nf = (p.n + kFeat - 1) / kFeat;
+  o.f0 = (int)(t % nf) * kFeat;
+  t /= nf;
+  o.split = (int)(t % p.splits);
+  t /= p.splits;
+  int steps;
+  if (MODE == kDw) {
+    const int nc = (p.k + kTok - 1) / kTok;
+    o.c0 = (int)(t % nc) * kTok;
+    o.expert = (int)(t / nc);
+    o.r0 = g.row[o.expert + 1];
+    o.r1 = g.row[o.expert + 2];
+    o.nn = p.k - o.c0 > kTok / 2 ? kTok : kTok / 2;
+    steps = (o.r1 - o.r0 + kBK - 1) / kBK;
+  } else {
+    const int s = segment_of(g, p.experts + 2, (int)t);
+    const int first = g.row[s], rows = g.row[s + 1] - first, parts = g.tile[s + 1] - g.tile[s], i = (int)t - g.tile[s];
+    const int each = (rows + parts - 1) / parts;
+    o.expert = s >= 1 && s <= p.experts ? s - 1 : -1;
+    o.r0 = first + min(i * each, rows);
+    o.r1 = first + min((i + 1) * each, rows);
+    o.c0 = 0;
+    o.nn = max((o.r1 - o.r0 + 31) & ~31, 32);
+    steps = o.expert < 0 ? 0 : (p.k + kBK - 1) / kBK;
+  }
+  o.b0 = (int)((i64)steps * o.split / p.splits);
+  o.b1 = (int)((i64)steps * (o.split + 1) / p.splits);
+  return o;
+}
+// The last step of a dw tile that reaches past its expert's rows.
+template <int MODE>
+__device__ __forceinline__ bool clears(const Tile& o, int b) {
+  return MODE == kDw && (i64)(b + 1) * kBK > o.r1 - o.r0;
+}
+
+template <class TO, int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped_tc(const __grid_constant__ P p) {
+  using namespace ccb;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const unsigned raw = smem_u32(smem), pad = (1024u - (raw & 1023u)) & 1023u;
+  const unsigned ring = raw + pad;
+  Tail& s = *reinterpret_cast<Tail*>(smem + pad + kStages * kStageBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned rank = tc2::cta_rank();
+  const i64 pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  lay_out(s.g, p.off, p.experts, p.rows, kTok, p.err);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s.full[i], 2);  // each CTA's producer (or its clearing warp), and both CTAs' bytes
+      mbar_init(&s.empty[i], 1);
+      mbar_init(&s.part[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.accf[i], 1);
+      mbar_init(&s.acce[i], 8);  // four draining warps of each CTA
+    }
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc::fence_before();
+  tc2::cluster_sync();
+  tc::fence_after();
+  const unsigned tmem = s.tmem;
+  const i64 tiles = tiles_of<MODE>(p, s.g);
+  Waiter wait(p.err);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      unsigned stage = 0, phase = 0;
+      for (i64 t = pair; t < tiles; t += pairs) {
+        const Tile o = tile_at<MODE>(p, s.g, t);
+        const int half = o.nn >> 1;
+        const unsigned boxes = MODE == kDw ? half / 64 : (half + 31) / 32, bytes = kABytes + boxes * (MODE == kDw ? 8192u : 4096u);
+        const int f = o.f0 + (int)rank * 128;
+        for (int b = o.b0; b < o.b1; ++b) {
+          wait(&s.empty[stage], phase ^ 1u);
+          const unsigned sa = ring + stage * kStageBytes, sb = sa + kABytes;
+          unsigned bar;
+          if (clears<MODE>(o, b)) {
+            mbar_expect_tx(&s.part[stage], bytes);
+            bar = smem_u32(&s.part[stage]);
+          } else {
+            bar = tc2::peer_addr(&s.full[stage], 0);
+            if (rank == 0)
+              mbar_expect_tx(&s.full[stage], 2u * bytes);
+            else
+              tc2::arrive_leader(&s.full[stage]);
+          }
+          const int k0 = b * kBK;
+          if (MODE == kDw) {
+            load3(sa, &p.ta, f, o.r0 + k0, 0, bar);
+            load3(sa + 8192u, &p.ta, f + 64, o.r0 + k0, 0, bar);
+            for (unsigned i = 0; i < boxes; ++i) load3(sb + i * 8192u, &p.tb, o.c0 + (int)rank * half + 64 * i, o.r0 + k0, 0, bar);
+          } else {
+            if (MODE == kForward) {
+              load4(sa, &p.ta, f, k0, o.expert, 0, bar);
+              load4(sa + 8192u, &p.ta, f + 64, k0, o.expert, 0, bar);
+            } else {
+              load4(sa, &p.ta, k0, f, o.expert, 0, bar);
+            }
+            for (unsigned i = 0; i < boxes; ++i) load3(sb + i * 4096u, &p.tb, k0, o.r0 + (int)rank * half + 32 * i, 0, bar);
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const unsigned base = (1u << 4) | ((unsigned)p.format << 7) | ((unsigned)p.format << 10) | ((MODE != kForwardT ? 1u : 0u) << 15) |
+                            ((MODE == kDw ? 1u : 0u) << 16) | (16u << 24);
+      unsigned stage = 0, phase = 0, it = 0;
+      for (i64 t = pair; t < tiles; t += pairs, ++it) {
+        const Tile o = tile_at<MODE>(p, s.g, t);
+        const unsigned ab = it & 1u, aph = (it >> 1) & 1u, d = tmem + ab * kTok;
+        const unsigned idesc = base | ((unsigned)(o.nn >> 3) << 17);
+        wait(&s.acce[ab], aph ^ 1u);
+        tc::fence_after();
+        for (int b = o.b0; b < o.b1; ++b) {
+          wait(&s.full[stage], phase);
+          tc::fence_after();
+          const unsigned sa = ring + stage * kStageBytes, sb = sa + kABytes;
+          const int kks = clears<MODE>(o, b) ? (o.r1 - o.r0 - b * kBK + 15) / 16 : kBK / 16;
+          for (int kk = 0; kk < kks; ++kk)
+            mma(d, MODE == kForwardT ? desc_k(sa, kk) : desc_mn(sa, kk), MODE == kDw ? desc_mn(sb, kk) : desc_k(sb, kk), idesc,
+                b > o.b0 || kk > 0 ? 1u : 0u);
+          tc2::commit_both(&s.empty[stage]);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        tc2::commit_both(&s.accf[ab]);
+      }
+    }
+  } else if (warp < 6) {
+    const int q = warp & 3;
+    unsigned it = 0;
+    for (i64 t = pair; t < tiles; t += pairs, ++it) {
+      const Tile o = tile_at<MODE>(p, s.g, t);
+      const unsigned ab = it & 1u, aph = (it >> 1) & 1u;
+      const int f = o.f0 + (int)rank * 128 + q * 32 + lane;
+      const int count = MODE == kDw ? min(p.k - o.c0, o.nn) : o.r1 - o.r0;
+      TO* out = static_cast<TO*>(p.out) + o.split * p.split_stride + f + (MODE == kDw ? o.expert * p.oe + (i64)o.c0 * p.os : (i64)o.r0 * p.os);
+      wait(&s.accf[ab], aph);
+      __syncwarp();
+      tc::fence_after();
+      for (int c = 0; c < count; c += 32) {
+        float v[32];
+        __syncwarp();
+        tc::ld32(tmem + ((unsigned)(q * 32) << 16) + ab * kTok + c, v);
+        if (o.b0 >= o.b1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+        }
+        if (f < p.n) {
+          TO* dst = out + (i64)c * p.os;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (c + i < count) *dst = from_f<TO>(v[i]);
+            dst += p.os;
+          }
+        }
+      }
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) tc2::arrive_leader(&s.acce[ab]);
+    }
+  } else if (MODE == kDw) {
+    unsigned stage = 0, phases = 0;  // bit i: parity of part[i]
+    for (i64 t = pair; t < tiles; t += pairs) {
+      const Tile o = tile_at<MODE>(p, s.g, t);
+      for (int b = o.b0; b < o.b1; ++b) {
+        if (clears<MODE>(o, b)) {
+          wait(&s.part[stage], (phases >> stage) & 1u);
+          __syncwarp();
+          phases ^= 1u << stage;
+          const int left = o.r1 - o.r0 - b * kBK, to = (left + 15) & ~15;
+          unsigned char* at = smem + pad + stage * kStageBytes;
+          const int blocks = 2 + (o.nn >> 7);  // of 64 features: two of the M side, then the N side's
+          for (int i = lane; i < blocks * (to - left) * 8; i += 32) {
+            const int blk = i / ((to - left) * 8), j = i % ((to - left) * 8);
+            *reinterpret_cast<uint4*>(at + blk * 8192 + (left + j / 8) * 128 + (j % 8) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) tc2::arrive_leader(&s.full[stage]);
+        }
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+      }
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc2::cluster_sync();
+  tc::fence_after();
+  __syncwarp();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+// The sum of the parts of a divided contraction, in order.
+template <class TO>
+__global__ void __launch_bounds__(256) add_parts(const float* part, i64 stride, int parts, TO* out, i64 rows_, i64 cols, i64 os, i64 mats, i64 oe) {
+  const i64 each = rows_ * cols, total = mats * each;
+  for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < total; i += (i64)gridDim.x * 256) {
+    float v = 0.0f;
+    for (int s = 0; s < parts; ++s) v += part[s * stride + i];
+    const i64 m = i / each, r = (i - m * each) / cols, c = i - m * each - r * cols;
+    out[m * oe + r * os + c] = from_f<TO>(v);
+  }
+}
+
+// A tensor map over 16-bit elements; dimensions of extent 1 get a legal stride.
+bool encode(ccb::TmaDesc* out, int format, const void* base, int rank, const i64* dims, const i64* strides /* elements, rank - 1 */, const int* box) {
+  const ccb::Driver& d = ccb::driver();
+  if (!d.ok || !aligned(base, 16)) return false;
+  cuuint64_t gd[4], gs[3];
+  cuuint32_t bx[4], one[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    if (dims[i] < 1 || dims[i] >= (1ll << 32)) return false;
+    gd[i] = (cuuint64_t)dims[i];
+    bx[i] = (cuuint32_t)box[i];
+    if (i > 0) {
+      const i64 st = dims[i] == 1 ? 8 : strides[i - 1];
+      if (st % 8 != 0 || st < 8 || st >= (1ll << 38)) return false;
+      gs[i - 1] = (cuuint64_t)st * 2;
+    }
+  }
+  static_assert(sizeof(CUtensorMap) == sizeof(ccb::TmaDesc), "tensor map size");
+  return d.cuTensorMapEncodeTiled(reinterpret_cast<CUtensorMap*>(out), format ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                                  (cuuint32_t)rank, const_cast<void*>(base), gd, gs, bx, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class TO, int MODE>
+int go(const P& p, int sms, cudaStream_t st, const char* me) {
+  static bool ready[64];  // the kernel's shared-memory limit was raised on the device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !__atomic_load_n(&ready[dev], __ATOMIC_RELAXED)) {
+    const cudaError_t e = cudaFuncSetAttribute(grouped_tc<TO, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return fail(CCB_ERR_DRIVER, me, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) __atomic_store_n(&ready[dev], true, __ATOMIC_RELAXED);
+  }
+  grouped_tc<TO, MODE><<<(unsigned)(sms & ~1), kThreads, kSmem, st>>>(p);
+  return launched(me);
+}
+}  // namespace tcg
+
 std::string check_sizes(i64 rows, i64 experts, i64 k, i64 n, int dtype) {
   if (rows < 0 || rows > INT_MAX) return "rows must be in [0, 2^31)";
   if (experts < 1 || experts > kMaxExperts) return "experts must be in [1, " + std::to_string(kMaxExperts) + "]";
@@ -240,8 +610,66 @@ std::string check_dw(const ccb_nn_grouped_matmul_dw_t* a) {
   if (bad.empty()) bad = check_stack(a->out, a->experts, a->k, a->n, a->out_stride, a->out_row_stride, type_bytes(a->out_dtype), "out");
   return bad;
 }
+
+// Whether a matrix can be read by the copy engine: 16-byte aligned, rows too.
+bool tma_ok(const void* p, i64 rows, i64 stride) { return aligned(p, 16) && (rows <= 1 || (stride % 8 == 0 && stride < (1ll << 38))); }
+
+// The tensor cores take 16-bit operands that the copy engine can read.
+bool on_tensor_cores(const ccb_nn_grouped_matmul_t* a) {
+  const i64 wr = a->transpose_w ? a->n : a->k;
+  return a->dtype != CCB_F32 && a->k > 0 && tma_ok(a->x, a->rows, a->x_stride) && tma_ok(a->w, wr, a->w_row_stride) &&
+         tma_ok(a->w, a->experts, a->w_stride);
+}
+bool on_tensor_cores(const ccb_nn_grouped_matmul_dw_t* a) {
+  return a->dtype != CCB_F32 && a->rows > 0 && tma_ok(a->x, a->rows, a->x_stride) && tma_ok(a->dy, a->rows, a->dy_stride);
+}
 size_t workspace_of(const ccb_nn_grouped_matmul_t*) { return 0; }
 size_t workspace_of(const ccb_nn_grouped_matmul_dw_t*) { return 0; }
+
+int tensor_forward(const ccb_nn_grouped_matmul_t* a, int sms, cudaStream_t st, const char* me) {
+  tcg::P p = {};
+  const int fmt = a->dtype == CCB_BF16;
+  const i64 xd[3] = {a->k, a->rows, 1}, xs[2] = {a->x_stride, 8};
+  const int xb[3] = {64, 32, 1};
+  const i64 wd[4] = {a->transpose_w ? a->k : a->n, a->transpose_w ? a->n : a->k, a->experts, 1}, ws[3] = {a->w_row_stride, a->w_stride, 8};
+  const int wb[4] = {64, a->transpose_w ? 128 : 64, 1, 1};
+  if (!tcg::encode(&p.tb, fmt, a->x, 3, xd, xs, xb) || !tcg::encode(&p.ta, fmt, a->w, 4, wd, ws, wb))
+    return fail(CCB_ERR_DRIVER, me, "cuTensorMapEncodeTiled refused x or w");
+  p.off = a->offsets;
+  p.out = a->out;
+  p.err = a->err;
+  p.os = a->out_stride;
+  p.rows = (int)a->rows;
+  p.experts = (int)a->experts;
+  p.n = (int)a->n;
+  p.k = (int)a->k;
+  p.splits = 1;
+  p.format = fmt;
+  if (a->transpose_w) return fmt ? tcg::go<__nv_bfloat16, tcg::kForwardT>(p, sms, st, me) : tcg::go<__half, tcg::kForwardT>(p, sms, st, me);
+  return fmt ? tcg::go<__nv_bfloat16, tcg::kForward>(p, sms, st, me) : tcg::go<__half, tcg::kForward>(p, sms, st, me);
+}
+
+int tensor_dw(const ccb_nn_grouped_matmul_dw_t* a, int sms, cudaStream_t st, const char* me) {
+  tcg::P p = {};
+  const int fmt = a->dtype == CCB_BF16;
+  const i64 xd[3] = {a->k, a->rows, 1}, xs[2] = {a->x_stride, 8}, yd[3] = {a->n, a->rows, 1}, ys[2] = {a->dy_stride, 8};
+  const int box[3] = {64, 64, 1};
+  if (!tcg::encode(&p.tb, fmt, a->x, 3, xd, xs, box) || !tcg::encode(&p.ta, fmt, a->dy, 3, yd, ys, box))
+    return fail(CCB_ERR_DRIVER, me, "cuTensorMapEncodeTiled refused x or dy");
+  p.off = a->offsets;
+  p.out = a->out;
+  p.err = a->err;
+  p.os = a->out_row_stride;
+  p.oe = a->out_stride;
+  p.rows = (int)a->rows;
+  p.experts = (int)a->experts;
+  p.n = (int)a->n;
+  p.k = (int)a->k;
+  p.splits = 1;
+  p.format = fmt;
+  if (a->out_dtype == CCB_F32) return tcg::go<float, tcg::kDw>(p, sms, st, me);
+  return fmt ? tcg::go<__nv_bfloat16, tcg::kDw>(p, sms, st, me) : tcg::go<__half, tcg::kDw>(p, sms, st, me);
+}
 
 }  // namespace
 }  // namespace ccb_nn
@@ -282,6 +710,7 @@ extern "C" int ccb_nn_grouped_matmul(const ccb_nn_grouped_matmul_t* a, void* str
     int sms = 0;
     if (const int rc = sm_count(me, &sms)) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (on_tensor_cores(a)) return tensor_forward(a, sms, st, me);
     const GroupP p = {a->x, a->w, a->offsets, a->out, a->err, a->k, a->n, a->x_stride, a->w_stride, a->w_row_stride, a->out_stride, (int)a->rows, (int)a->experts};
     if (a->dtype == CCB_F32)
       any<float>(p, a->transpose_w, sms, st);
@@ -305,6 +734,7 @@ extern "C" int ccb_nn_grouped_matmul_dw(const ccb_nn_grouped_matmul_dw_t* a, voi
     int sms = 0;
     if (const int rc = sm_count(me, &sms)) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (on_tensor_cores(a)) return tensor_dw(a, sms, st, me);
     const GroupDwP p = {a->x, a->dy, a->offsets, a->out, a->err, a->k, a->n, a->x_stride, a->dy_stride, a->out_stride, a->out_row_stride, (int)a->rows, (int)a->experts};
     if (a->dtype == CCB_F32)
       any_dw<float, float>(p, sms, st);
