@@ -244,16 +244,20 @@ struct P {
   i64 os, oe;           // strides of out: a row, an expert's matrix (dw)
   i64 split_stride;     // elements from one part's result to the next
   int rows, experts, n, k, splits, format;
+  int a2, b2;           // whether one copy takes two 64-wide blocks of an MN-major operand
+  int box;              // rows of a copy of tokens
 };
 
-// Acquires at cluster scope: what the pair's other CTA wrote before it arrived.
-__device__ __forceinline__ bool try_wait(ccb::u64* bar, unsigned parity) {
+// Barriers and tiles are addressed by 32-bit shared addresses throughout: one
+// thread issues the copies and one the MMAs, at some five cycles an
+// instruction, so every instruction of their loops counts (a step of the
+// contraction is 512 cycles of the tensor pipe).
+__device__ __forceinline__ bool try_wait(unsigned bar, unsigned parity) {
   unsigned ok;
-  asm volatile(
-      "{\n .reg .pred q;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 q, [%1], %2;\n selp.u32 %0, 1, 0, q;\n}\n"
-      : "=r"(ok)
-      : "r"(ccb::smem_u32(bar)), "r"(parity)
-      : "memory");
+  asm volatile("{\n .reg .pred q;\n mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n selp.u32 %0, 1, 0, q;\n}\n"
+               : "=r"(ok)
+               : "r"(bar), "r"(parity)
+               : "memory");
   return ok != 0;
 }
 // Bounded; once a wait has run out the thread's later ones hardly poll, so
@@ -262,16 +266,28 @@ struct Waiter {
   unsigned limit = ccb::MBAR_SPIN_LIMIT;
   unsigned* err;
   __device__ __forceinline__ explicit Waiter(unsigned* e) : err(e) {}
-  __device__ __forceinline__ void operator()(ccb::u64* bar, unsigned parity) {
+  __device__ __forceinline__ void operator()(unsigned bar, unsigned parity) {
+    if (try_wait(bar, parity)) return;
     for (unsigned it = 0; it < limit; ++it)
       if (try_wait(bar, parity)) return;
     if (err) atomicOr(err, kErrWait);
     limit = 64;
   }
 };
-
-__device__ __forceinline__ void load3(unsigned dst, const ccb::TmaDesc* map, int x, int y, int z, unsigned bar) {
-  ccb::tc2::tma_load_3d(dst, map, x, y, z, bar);
+__device__ __forceinline__ void expect(unsigned bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Arrivals on a barrier of either CTA. The relaxed one says that the other
+// CTA's producer has issued its copies; it orders nothing else, and a release
+// there costs a fence at every step (0.98 us a step with it, 0.45 without).
+__device__ __forceinline__ void arrive(unsigned bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_relaxed(unsigned bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void commit(unsigned bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void load4(unsigned dst, const ccb::TmaDesc* map, int x, int y, int z, int w, unsigned bar) {
   asm volatile(
@@ -286,15 +302,18 @@ __device__ __forceinline__ void mma(unsigned d, ccb::u64 a, ccb::u64 b, unsigned
       " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z));
 }
-// 16-bit operands, 128-byte swizzle. K-major: 128-byte rows of 64 along the
-// contraction, 8-row groups 1024 bytes apart, 16 of the contraction 32 bytes
-// further. MN-major: 64 along M or N are one 128-byte row, one row for each
-// step of the contraction, 8-row groups 1024 bytes apart, the next 64 along M
-// or N 8192 bytes on, 16 of the contraction 2048 bytes further.
-__device__ __forceinline__ ccb::u64 desc_k(unsigned tile, int kk) { return ccb::tc::desc_k(tile, kk); }
-__device__ __forceinline__ ccb::u64 desc_mn(unsigned tile, int kk) {
-  return ccb::tc::sdesc(tile + kk * 2048u, 8192u, 1024u, ccb::tc::LAYOUT_SW128);
+// Operand descriptors of 16-bit tiles with the 128-byte swizzle. K-major:
+// 128-byte rows of 64 along the contraction, 8-row groups 1024 bytes apart, 16
+// of the contraction 32 bytes further. MN-major: 64 along M or N are one
+// 128-byte row, one row for each step of the contraction, 8-row groups 1024
+// bytes apart, the next 64 along M or N 8192 bytes on, 16 of the contraction
+// 2048 bytes further. The start address is in units of 16 bytes.
+template <bool MN>
+__device__ __forceinline__ ccb::u64 desc(unsigned tile) {
+  return ccb::tc::sdesc(tile, MN ? 8192u : 16u, 1024u, ccb::tc::LAYOUT_SW128);
 }
+template <bool MN>
+__device__ __forceinline__ constexpr unsigned desc_step() { return (MN ? 2048u : 32u) >> 4; }
 
 struct Tile {
   int expert;      // -1: rows of no expert
@@ -307,24 +326,24 @@ struct Tile {
 enum { kForward = 0, kForwardT = 1, kDw = 2 };
 
 template <int MODE>
-__device__ __forceinline__ i64 tiles_of(const P& p, const Segments& g) {
-  const i64 nf = (p.n + kFeat - 1) / kFeat;
+__device__ __forceinline__ unsigned tiles_of(const P& p, const Segments& g) {
+  const unsigned nf = (p.n + kFeat - 1) / kFeat;
   if (MODE == kDw) return nf * ((p.k + kTok - 1) / kTok) * p.experts * p.splits;
   return nf * g.tile[p.experts + 2] * p.splits;
 }
 // Tile t: features innermost, then the parts of the contraction, then tokens:
 // the pairs work on one expert's matrix at a time, which stays in L2.
 template <int MODE>
-__device__ __forceinline__ Tile tile_at(const P& p, const Segments& g, i64 t) {
+__device__ __forceinline__ Tile tile_at(const P& p, const Segments& g, unsigned t) {
   Tile o;
-  const int nf = (p.n + kFeat - 1) / kFeat;
+  const unsigned nf = (p.n + kFeat - 1) / kFeat;
   o.f0 = (int)(t % nf) * kFeat;
   t /= nf;
-  o.split = (int)(t % p.splits);
-  t /= p.splits;
+  o.split = (int)(t % (unsigned)p.splits);
+  t /= (unsigned)p.splits;
   int steps;
   if (MODE == kDw) {
-    const int nc = (p.k + kTok - 1) / kTok;
+    const unsigned nc = (p.k + kTok - 1) / kTok;
     o.c0 = (int)(t % nc) * kTok;
     o.expert = (int)(t / nc);
     o.r0 = g.row[o.expert + 1];
@@ -342,14 +361,14 @@ __device__ __forceinline__ Tile tile_at(const P& p, const Segments& g, i64 t) {
     o.nn = max((o.r1 - o.r0 + 31) & ~31, 32);
     steps = o.expert < 0 ? 0 : (p.k + kBK - 1) / kBK;
   }
-  o.b0 = (int)((i64)steps * o.split / p.splits);
-  o.b1 = (int)((i64)steps * (o.split + 1) / p.splits);
+  o.b0 = steps * o.split / p.splits;
+  o.b1 = steps * (o.split + 1) / p.splits;
   return o;
 }
 // The last step of a dw tile that reaches past its expert's rows.
 template <int MODE>
 __device__ __forceinline__ bool clears(const Tile& o, int b) {
-  return MODE == kDw && (i64)(b + 1) * kBK > o.r1 - o.r0;
+  return MODE == kDw && o.r1 - o.r0 - b * kBK < kBK;
 }
 
 template <class TO, int MODE>
@@ -361,7 +380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
   Tail& s = *reinterpret_cast<Tail*>(smem + pad + kStages * kStageBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned rank = tc2::cta_rank();
-  const i64 pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const unsigned pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   lay_out(s.g, p.off, p.experts, p.rows, kTok, p.err);
   if (threadIdx.x == 0) {
@@ -384,47 +403,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
   tc2::cluster_sync();
   tc::fence_after();
   const unsigned tmem = s.tmem;
-  const i64 tiles = tiles_of<MODE>(p, s.g);
+  const unsigned tiles = tiles_of<MODE>(p, s.g);
   Waiter wait(p.err);
+  const unsigned full = smem_u32(&s.full[0]), empty = smem_u32(&s.empty[0]), part = smem_u32(&s.part[0]), accf = smem_u32(&s.accf[0]),
+                 acce = smem_u32(&s.acce[0]);
+  const unsigned lead_full = tc2::peer_addr(&s.full[0], 0), lead_acce = tc2::peer_addr(&s.acce[0], 0);
 
   if (warp == 0) {
     if (lane == 0) {
-      unsigned stage = 0, phase = 0;
-      for (i64 t = pair; t < tiles; t += pairs) {
+      unsigned st = 0, at = ring, phase = 1;  // 8 * stage, its address
+      for (unsigned t = pair; t < tiles; t += pairs) {
         const Tile o = tile_at<MODE>(p, s.g, t);
-        const int half = o.nn >> 1;
-        const unsigned boxes = MODE == kDw ? half / 64 : (half + 31) / 32, bytes = kABytes + boxes * (MODE == kDw ? 8192u : 4096u);
-        const int f = o.f0 + (int)rank * 128;
+        const int half = o.nn >> 1, f = o.f0 + (int)rank * 128, c = o.c0 + (int)rank * half, tok = o.r0 + (int)rank * half;
+        const int boxes = MODE == kDw ? (p.b2 ? 1 : half / 64) : (half + p.box - 1) / p.box;
+        const unsigned box = MODE == kDw ? (p.b2 ? 16384u : 8192u) : (unsigned)p.box * 128u, bytes = kABytes + boxes * box;
         for (int b = o.b0; b < o.b1; ++b) {
-          wait(&s.empty[stage], phase ^ 1u);
-          const unsigned sa = ring + stage * kStageBytes, sb = sa + kABytes;
-          unsigned bar;
+          wait(empty + st, phase);
+          unsigned bar = lead_full + st;
           if (clears<MODE>(o, b)) {
-            mbar_expect_tx(&s.part[stage], bytes);
-            bar = smem_u32(&s.part[stage]);
+            bar = part + st;
+            expect(bar, bytes);
+          } else if (rank == 0) {
+            expect(full + st, 2u * bytes);
           } else {
-            bar = tc2::peer_addr(&s.full[stage], 0);
-            if (rank == 0)
-              mbar_expect_tx(&s.full[stage], 2u * bytes);
-            else
-              tc2::arrive_leader(&s.full[stage]);
+            arrive_relaxed(bar);
           }
           const int k0 = b * kBK;
+          unsigned sb = at + kABytes;
           if (MODE == kDw) {
-            load3(sa, &p.ta, f, o.r0 + k0, 0, bar);
-            load3(sa + 8192u, &p.ta, f + 64, o.r0 + k0, 0, bar);
-            for (unsigned i = 0; i < boxes; ++i) load3(sb + i * 8192u, &p.tb, o.c0 + (int)rank * half + 64 * i, o.r0 + k0, 0, bar);
-          } else {
-            if (MODE == kForward) {
-              load4(sa, &p.ta, f, k0, o.expert, 0, bar);
-              load4(sa + 8192u, &p.ta, f + 64, k0, o.expert, 0, bar);
+            const int r = o.r0 + k0;
+            if (p.a2) {
+              load4(at, &p.ta, 0, r, f >> 6, 0, bar);
             } else {
-              load4(sa, &p.ta, k0, f, o.expert, 0, bar);
+              load4(at, &p.ta, f, r, 0, 0, bar);
+              load4(at + 8192u, &p.ta, f + 64, r, 0, 0, bar);
             }
-            for (unsigned i = 0; i < boxes; ++i) load3(sb + i * 4096u, &p.tb, k0, o.r0 + (int)rank * half + 32 * i, 0, bar);
+            if (p.b2) {
+              load4(sb, &p.tb, 0, r, c >> 6, 0, bar);
+            } else {
+              load4(sb, &p.tb, c, r, 0, 0, bar);
+              if (boxes > 1) load4(sb + 8192u, &p.tb, c + 64, r, 0, 0, bar);
+            }
+          } else {
+            if (MODE == kForwardT) {
+              load4(at, &p.ta, k0, f, o.expert, 0, bar);
+            } else if (p.a2) {
+              load4(at, &p.ta, 0, k0, f >> 6, o.expert, bar);
+            } else {
+              load4(at, &p.ta, f, k0, o.expert, 0, bar);
+              load4(at + 8192u, &p.ta, f + 64, k0, o.expert, 0, bar);
+            }
+            load4(sb, &p.tb, k0, tok, 0, 0, bar);
+            for (int i = 1; i < boxes; ++i) {
+              sb += box;
+              load4(sb, &p.tb, k0, tok + i * p.box, 0, 0, bar);
+            }
           }
-          if (++stage == kStages) {
-            stage = 0;
+          st += 8;
+          at += kStageBytes;
+          if (st == 8 * kStages) {
+            st = 0;
+            at = ring;
             phase ^= 1u;
           }
         }
@@ -432,42 +471,56 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      const unsigned base = (1u << 4) | ((unsigned)p.format << 7) | ((unsigned)p.format << 10) | ((MODE != kForwardT ? 1u : 0u) << 15) |
-                            ((MODE == kDw ? 1u : 0u) << 16) | (16u << 24);
-      unsigned stage = 0, phase = 0, it = 0;
-      for (i64 t = pair; t < tiles; t += pairs, ++it) {
+      constexpr bool amn = MODE != kForwardT, bmn = MODE == kDw;
+      const unsigned base = (1u << 4) | ((unsigned)p.format << 7) | ((unsigned)p.format << 10) | ((amn ? 1u : 0u) << 15) | ((bmn ? 1u : 0u) << 16) | (16u << 24);
+      const u64 a0 = desc<amn>(ring), b0 = desc<bmn>(ring + kABytes);
+      const unsigned empty0 = tc2::peer_addr(&s.empty[0], 0), empty1 = tc2::peer_addr(&s.empty[0], 1);
+      const unsigned accf0 = tc2::peer_addr(&s.accf[0], 0), accf1 = tc2::peer_addr(&s.accf[0], 1);
+      unsigned st = 0, phase = 0, it = 0;
+      u64 a = a0, bd = b0;
+      for (unsigned t = pair; t < tiles; t += pairs, ++it) {
         const Tile o = tile_at<MODE>(p, s.g, t);
-        const unsigned ab = it & 1u, aph = (it >> 1) & 1u, d = tmem + ab * kTok;
+        const unsigned ab = it & 1u, d = tmem + ab * kTok;
         const unsigned idesc = base | ((unsigned)(o.nn >> 3) << 17);
-        wait(&s.acce[ab], aph ^ 1u);
+        wait(acce + 8 * ab, ((it >> 1) & 1u) ^ 1u);
         tc::fence_after();
         for (int b = o.b0; b < o.b1; ++b) {
-          wait(&s.full[stage], phase);
+          wait(full + st, phase);
           tc::fence_after();
-          const unsigned sa = ring + stage * kStageBytes, sb = sa + kABytes;
-          const int kks = clears<MODE>(o, b) ? (o.r1 - o.r0 - b * kBK + 15) / 16 : kBK / 16;
-          for (int kk = 0; kk < kks; ++kk)
-            mma(d, MODE == kForwardT ? desc_k(sa, kk) : desc_mn(sa, kk), MODE == kDw ? desc_mn(sb, kk) : desc_k(sb, kk), idesc,
-                b > o.b0 || kk > 0 ? 1u : 0u);
-          tc2::commit_both(&s.empty[stage]);
-          if (++stage == kStages) {
-            stage = 0;
+          if (clears<MODE>(o, b)) {
+            asm volatile("fence.acq_rel.cluster;" ::: "memory");  // the other CTA's cleared rows
+            const int kks = (o.r1 - o.r0 - b * kBK + 15) / 16;
+            for (int kk = 0; kk < kks; ++kk) mma(d, a + kk * desc_step<amn>(), bd + kk * desc_step<bmn>(), idesc, b > o.b0 || kk > 0 ? 1u : 0u);
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < kBK / 16; ++kk) mma(d, a + kk * desc_step<amn>(), bd + kk * desc_step<bmn>(), idesc, b > o.b0 || kk > 0 ? 1u : 0u);
+          }
+          commit(empty0 + st);
+          commit(empty1 + st);
+          st += 8;
+          a += kStageBytes >> 4;
+          bd += kStageBytes >> 4;
+          if (st == 8 * kStages) {
+            st = 0;
+            a = a0;
+            bd = b0;
             phase ^= 1u;
           }
         }
-        tc2::commit_both(&s.accf[ab]);
+        commit(accf0 + 8 * ab);
+        commit(accf1 + 8 * ab);
       }
     }
   } else if (warp < 6) {
     const int q = warp & 3;
     unsigned it = 0;
-    for (i64 t = pair; t < tiles; t += pairs, ++it) {
+    for (unsigned t = pair; t < tiles; t += pairs, ++it) {
       const Tile o = tile_at<MODE>(p, s.g, t);
       const unsigned ab = it & 1u, aph = (it >> 1) & 1u;
       const int f = o.f0 + (int)rank * 128 + q * 32 + lane;
       const int count = MODE == kDw ? min(p.k - o.c0, o.nn) : o.r1 - o.r0;
       TO* out = static_cast<TO*>(p.out) + o.split * p.split_stride + f + (MODE == kDw ? o.expert * p.oe + (i64)o.c0 * p.os : (i64)o.r0 * p.os);
-      wait(&s.accf[ab], aph);
+      wait(accf + 8 * ab, aph);
       __syncwarp();
       tc::fence_after();
       for (int c = 0; c < count; c += 32) {
@@ -489,27 +542,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
       }
       tc::fence_before();
       __syncwarp();
-      if (lane == 0) tc2::arrive_leader(&s.acce[ab]);
+      if (lane == 0) arrive(lead_acce + 8 * ab);
     }
   } else if (MODE == kDw) {
+    // a lane has one 16-byte piece of each row: two 64-wide blocks of the M side, then the N side's
     unsigned stage = 0, phases = 0;  // bit i: parity of part[i]
-    for (i64 t = pair; t < tiles; t += pairs) {
+    for (unsigned t = pair; t < tiles; t += pairs) {
       const Tile o = tile_at<MODE>(p, s.g, t);
       for (int b = o.b0; b < o.b1; ++b) {
         if (clears<MODE>(o, b)) {
-          wait(&s.part[stage], (phases >> stage) & 1u);
+          wait(part + 8 * stage, (phases >> stage) & 1u);
           __syncwarp();
           phases ^= 1u << stage;
           const int left = o.r1 - o.r0 - b * kBK, to = (left + 15) & ~15;
-          unsigned char* at = smem + pad + stage * kStageBytes;
-          const int blocks = 2 + (o.nn >> 7);  // of 64 features: two of the M side, then the N side's
-          for (int i = lane; i < blocks * (to - left) * 8; i += 32) {
-            const int blk = i / ((to - left) * 8), j = i % ((to - left) * 8);
-            *reinterpret_cast<uint4*>(at + blk * 8192 + (left + j / 8) * 128 + (j % 8) * 16) = make_uint4(0, 0, 0, 0);
-          }
+          uint4* at = reinterpret_cast<uint4*>(smem + pad + stage * kStageBytes + (lane >> 3) * 8192 + (lane & 7) * 16);
+          for (int r = left; r < to; ++r) at[r * 8] = make_uint4(0, 0, 0, 0);
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) tc2::arrive_leader(&s.full[stage]);
+          if (lane == 0) arrive(lead_full + 8 * stage);
         }
         stage = stage + 1 == kStages ? 0 : stage + 1;
       }
@@ -626,15 +676,39 @@ bool on_tensor_cores(const ccb_nn_grouped_matmul_dw_t* a) {
 size_t workspace_of(const ccb_nn_grouped_matmul_t*) { return 0; }
 size_t workspace_of(const ccb_nn_grouped_matmul_dw_t*) { return 0; }
 
+// The map of an MN-major operand: `outer` matrices of `rows` (the contraction)
+// by `cols`. Where rows are whole 64-wide blocks, one copy takes two of them:
+// the blocks are a dimension of their own.
+bool encode_mn(ccb::TmaDesc* m, int fmt, const void* base, i64 cols, i64 rows, i64 outer, i64 stride, i64 outer_stride, int* two) {
+  *two = cols % 64 == 0;
+  if (*two) {
+    const i64 d[4] = {64, rows, cols / 64, outer}, st[3] = {stride, 64, outer_stride};
+    const int box[4] = {64, 64, 2, 1};
+    return tcg::encode(m, fmt, base, 4, d, st, box);
+  }
+  const i64 d[4] = {cols, rows, outer, 1}, st[3] = {stride, outer_stride, 8};
+  const int box[4] = {64, 64, 1, 1};
+  return tcg::encode(m, fmt, base, 4, d, st, box);
+}
+
 int tensor_forward(const ccb_nn_grouped_matmul_t* a, int sms, cudaStream_t st, const char* me) {
   tcg::P p = {};
   const int fmt = a->dtype == CCB_BF16;
-  const i64 xd[3] = {a->k, a->rows, 1}, xs[2] = {a->x_stride, 8};
-  const int xb[3] = {64, 32, 1};
-  const i64 wd[4] = {a->transpose_w ? a->k : a->n, a->transpose_w ? a->n : a->k, a->experts, 1}, ws[3] = {a->w_row_stride, a->w_stride, 8};
-  const int wb[4] = {64, a->transpose_w ? 128 : 64, 1, 1};
-  if (!tcg::encode(&p.tb, fmt, a->x, 3, xd, xs, xb) || !tcg::encode(&p.ta, fmt, a->w, 4, wd, ws, wb))
-    return fail(CCB_ERR_DRIVER, me, "cuTensorMapEncodeTiled refused x or w");
+  // tokens come in boxes of about half of what an expert has on average: a
+  // box is one copy, and a larger one than needed is read in vain
+  const i64 mean = a->rows / (a->experts < a->rows ? a->experts : a->rows);
+  p.box = mean <= 16 ? 16 : mean <= 64 ? 64 : 128;
+  const i64 xd[4] = {a->k, a->rows, 1, 1}, xs[3] = {a->x_stride, 8, 8};
+  const int xb[4] = {64, p.box, 1, 1};
+  bool ok = tcg::encode(&p.tb, fmt, a->x, 4, xd, xs, xb);
+  if (a->transpose_w) {
+    const i64 wd[4] = {a->k, a->n, a->experts, 1}, ws[3] = {a->w_row_stride, a->w_stride, 8};
+    const int wb[4] = {64, 128, 1, 1};
+    ok = ok && tcg::encode(&p.ta, fmt, a->w, 4, wd, ws, wb);
+  } else {
+    ok = ok && encode_mn(&p.ta, fmt, a->w, a->n, a->k, a->experts, a->w_row_stride, a->w_stride, &p.a2);
+  }
+  if (!ok) return fail(CCB_ERR_DRIVER, me, "cuTensorMapEncodeTiled refused x or w");
   p.off = a->offsets;
   p.out = a->out;
   p.err = a->err;
@@ -652,9 +726,7 @@ int tensor_forward(const ccb_nn_grouped_matmul_t* a, int sms, cudaStream_t st, c
 int tensor_dw(const ccb_nn_grouped_matmul_dw_t* a, int sms, cudaStream_t st, const char* me) {
   tcg::P p = {};
   const int fmt = a->dtype == CCB_BF16;
-  const i64 xd[3] = {a->k, a->rows, 1}, xs[2] = {a->x_stride, 8}, yd[3] = {a->n, a->rows, 1}, ys[2] = {a->dy_stride, 8};
-  const int box[3] = {64, 64, 1};
-  if (!tcg::encode(&p.tb, fmt, a->x, 3, xd, xs, box) || !tcg::encode(&p.ta, fmt, a->dy, 3, yd, ys, box))
+  if (!encode_mn(&p.tb, fmt, a->x, a->k, a->rows, 1, a->x_stride, 8, &p.b2) || !encode_mn(&p.ta, fmt, a->dy, a->n, a->rows, 1, a->dy_stride, 8, &p.a2))
     return fail(CCB_ERR_DRIVER, me, "cuTensorMapEncodeTiled refused x or dy");
   p.off = a->offsets;
   p.out = a->out;
