@@ -2,6 +2,8 @@
 // expert. The row ranges of the experts live in device memory, so every block
 // lays the tiles out for itself: it clamps the offsets, counts the row tiles
 // of each segment and scans the counts in shared memory.
+#include <type_traits>
+
 #include "ccb_skel.cuh"
 #include "dyn.hpp"
 #include "nn_common.cuh"
@@ -214,11 +216,11 @@ void any_dw(const GroupDwP& p, int sms, cudaStream_t st) {
 //
 // Warps of each CTA: 0 TMA producer (a ring of 6 stages, 64 of the contraction
 // each: 128 features of the M side and half of the N side), 1 MMA issuer (of
-// the even CTA, for both), 2-5 drain one of two accumulators while the other
-// fills, 6 (dw) clears the rows past an expert's end: the contraction runs
+// the even CTA, for both), 2-9 drain one of two accumulators while the other
+// fills, 10 (dw) clears the rows past an expert's end: the contraction runs
 // over rows there, so what the next expert holds must not reach the sum. Both
 // CTAs' copies complete on the even CTA's barrier; copies whose rows have to
-// be cleared complete on the CTA's own, and warp 6 passes them on.
+// be cleared complete on the CTA's own, and warp 10 passes them on.
 //
 // Every tile is dealt out round-robin; a segment's rows are cut evenly, so
 // that no tile is a short remainder.
@@ -226,15 +228,17 @@ namespace tcg {
 constexpr int kFeat = 256, kTok = 256, kBK = 64, kStages = 6;
 constexpr unsigned kABytes = 128 * kBK * 2, kBBytes = 128 * kBK * 2, kStageBytes = kABytes + kBBytes;
 constexpr unsigned kTmemCols = 512;
-constexpr int kThreads = 224;
+constexpr int kDrain = 8, kThreads = 32 * (3 + kDrain);  // draining warps; all
 constexpr unsigned kErrWait = 16u;
 
 struct Tail {  // after the ring
   ccb::u64 full[kStages], empty[kStages], part[kStages], accf[2], acce[2];
   unsigned tmem;
+  alignas(128) unsigned char out[kDrain][2048];  // a draining warp's 32 tokens x 32 features
   Segments g;
 };
 constexpr unsigned kSmem = kStages * kStageBytes + sizeof(Tail) + 1024;
+static_assert(kSmem <= 232448, "shared memory of a block");
 
 struct P {
   ccb::TmaDesc ta, tb;  // M side, N side
@@ -246,6 +250,7 @@ struct P {
   int rows, experts, n, k, splits, format;
   int a2, b2;           // whether one copy takes two 64-wide blocks of an MN-major operand
   int box;              // rows of a copy of tokens
+  int vec;              // out takes 16-byte stores
 };
 
 // Barriers and tiles are addressed by 32-bit shared addresses throughout: one
@@ -277,11 +282,15 @@ struct Waiter {
 __device__ __forceinline__ void expect(unsigned bar, unsigned bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Arrivals on a barrier of either CTA. The relaxed one says that the other
-// CTA's producer has issued its copies; it orders nothing else, and a release
-// there costs a fence at every step (0.98 us a step with it, 0.45 without).
+// Arrivals on a barrier of either CTA. A release at cluster scope waits until
+// every earlier store of the thread, those to `out` too, has been performed,
+// some 3 us under load, so none is asked for where nothing in memory is handed
+// over: the other CTA's producer says that its copies are issued (their bytes
+// are counted by the barrier itself), a draining warp that its loads from the
+// accumulator are done (they are: tcgen05.wait::ld). The clearing warp hands
+// over shared memory that its proxy fence has already made visible.
 __device__ __forceinline__ void arrive(unsigned bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void arrive_relaxed(unsigned bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -314,6 +323,106 @@ __device__ __forceinline__ ccb::u64 desc(unsigned tile) {
 }
 template <bool MN>
 __device__ __forceinline__ constexpr unsigned desc_step() { return (MN ? 2048u : 32u) >> 4; }
+
+// 32 lanes x 32 columns of the accumulator in the fragments of 8x8 matrices:
+// v[16 h + 4 j + 2 i + b] is feature 16 h + 8 i + lane / 4, token 8 j + 2 (lane % 4) + b.
+__device__ __forceinline__ void load_fragments(unsigned taddr, unsigned* v) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[16 * h]), "=r"(v[16 * h + 1]), "=r"(v[16 * h + 2]), "=r"(v[16 * h + 3]), "=r"(v[16 * h + 4]), "=r"(v[16 * h + 5]),
+                   "=r"(v[16 * h + 6]), "=r"(v[16 * h + 7]), "=r"(v[16 * h + 8]), "=r"(v[16 * h + 9]), "=r"(v[16 * h + 10]), "=r"(v[16 * h + 11]),
+                   "=r"(v[16 * h + 12]), "=r"(v[16 * h + 13]), "=r"(v[16 * h + 14]), "=r"(v[16 * h + 15])
+                 : "r"(taddr + ((unsigned)(16 * h) << 16)));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+template <class TO>
+__device__ __forceinline__ unsigned pack(unsigned lo, unsigned hi) {
+  unsigned r;
+  if constexpr (sizeof(TO) == 2) {
+    if constexpr (std::is_same<TO, __half>::value)
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(__uint_as_float(hi)), "f"(__uint_as_float(lo)));
+    else
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(__uint_as_float(hi)), "f"(__uint_as_float(lo)));
+  } else {
+    r = 0;
+  }
+  return r;
+}
+// A warp's 32 features x 32 tokens to `out` (its first feature and token), in
+// 16 bits: turned through shared memory so that a lane stores 16 bytes of one
+// token (four packed transposing stores of 8x8 matrices; 64-byte rows, their
+// 16-byte pieces swapped by row pair against bank conflicts). Written in
+// phases, each of independent instructions: a warp alone on its scheduler pays
+// every latency.
+template <class TO>
+__device__ __forceinline__ void drain16(unsigned taddr, bool zero, unsigned buf, TO* out, i64 os, int tokens, int feats, bool vec, int lane) {
+  unsigned v[32], h[16];
+  if (zero) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = 0;
+  } else {
+    load_fragments(taddr, v);
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) h[i] = pack<TO>(v[2 * i], v[2 * i + 1]);
+  // token 8 j + lane % 8, piece lane / 8: the swap depends on the lane alone
+  const unsigned put = buf + (lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(put + j * 512), "r"(h[2 * j]), "r"(h[2 * j + 1]),
+                 "r"(h[8 + 2 * j]), "r"(h[8 + 2 * j + 1])
+                 : "memory");
+  __syncwarp();
+  // token 8 j + lane / 4, piece lane % 4
+  const unsigned get = buf + (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
+  uint4 w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[j].x), "=r"(w[j].y), "=r"(w[j].z), "=r"(w[j].w) : "r"(get + j * 512) : "memory");
+  __syncwarp();
+  const int f = (lane & 3) * 8, tok = lane >> 2;
+  TO* dst = out + tok * os + f;
+  if (vec && tokens >= 32 && feats >= 32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + 8 * j * os) = w[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (8 * j + tok >= tokens || f >= feats) continue;
+      TO* at = dst + 8 * j * os;
+      if (vec && f + 8 <= feats) {
+        *reinterpret_cast<uint4*>(at) = w[j];
+      } else {
+        const unsigned u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (f + i < feats) reinterpret_cast<unsigned short*>(at)[i] = (unsigned short)(u[i >> 1] >> (16 * (i & 1)));
+      }
+    }
+  }
+}
+// The same in 32 bits: lanes are features, a store is one token's 128 bytes.
+__device__ __forceinline__ void drain32(unsigned taddr, bool zero, float* out, i64 os, int tokens, int feats, int lane) {
+  float v[32];
+  if (zero) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+  } else {
+    ccb::tc::ld32(taddr, v);
+  }
+  if (lane < feats) {
+    float* dst = out + lane;
+    if (tokens >= 32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) dst[i * os] = v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < tokens) dst[i * os] = v[i];
+    }
+  }
+}
 
 struct Tile {
   int expert;      // -1: rows of no expert
@@ -391,7 +500,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.accf[i], 1);
-      mbar_init(&s.acce[i], 8);  // four draining warps of each CTA
+      mbar_init(&s.acce[i], 2 * kDrain);  // the draining warps of both CTAs
     }
     mbar_fence_init();
   }
@@ -488,7 +597,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
           wait(full + st, phase);
           tc::fence_after();
           if (clears<MODE>(o, b)) {
-            asm volatile("fence.acq_rel.cluster;" ::: "memory");  // the other CTA's cleared rows
             const int kks = (o.r1 - o.r0 - b * kBK + 15) / 16;
             for (int kk = 0; kk < kks; ++kk) mma(d, a + kk * desc_step<amn>(), bd + kk * desc_step<bmn>(), idesc, b > o.b0 || kk > 0 ? 1u : 0u);
           } else {
@@ -511,38 +619,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
         commit(accf1 + 8 * ab);
       }
     }
-  } else if (warp < 6) {
-    const int q = warp & 3;
+  } else if (warp < 2 + kDrain) {
+    const int q = warp & 3, other = (warp - 2) >> 2;  // its quarter of the lanes; every other 32 columns
     unsigned it = 0;
     for (unsigned t = pair; t < tiles; t += pairs, ++it) {
       const Tile o = tile_at<MODE>(p, s.g, t);
       const unsigned ab = it & 1u, aph = (it >> 1) & 1u;
-      const int f = o.f0 + (int)rank * 128 + q * 32 + lane;
+      const int f = o.f0 + (int)rank * 128 + q * 32;
       const int count = MODE == kDw ? min(p.k - o.c0, o.nn) : o.r1 - o.r0;
       TO* out = static_cast<TO*>(p.out) + o.split * p.split_stride + f + (MODE == kDw ? o.expert * p.oe + (i64)o.c0 * p.os : (i64)o.r0 * p.os);
+      const unsigned buf = smem_u32(s.out[warp - 2]);
+      const unsigned acc = tmem + ((unsigned)(q * 32) << 16) + ab * kTok;
       wait(accf + 8 * ab, aph);
       __syncwarp();
       tc::fence_after();
-      for (int c = 0; c < count; c += 32) {
-        float v[32];
-        __syncwarp();
-        tc::ld32(tmem + ((unsigned)(q * 32) << 16) + ab * kTok + c, v);
-        if (o.b0 >= o.b1) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0.0f;
-        }
-        if (f < p.n) {
-          TO* dst = out + (i64)c * p.os;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (c + i < count) *dst = from_f<TO>(v[i]);
-            dst += p.os;
-          }
+      if (f < p.n) {
+        for (int c = 32 * other; c < count; c += 32 * (kDrain / 4)) {
+          if constexpr (sizeof(TO) == 2)
+            drain16<TO>(acc + c, o.b0 >= o.b1, buf, out + c * p.os, p.os, count - c, p.n - f, p.vec, lane);
+          else
+            drain32(acc + c, o.b0 >= o.b1, out + c * p.os, p.os, count - c, p.n - f, lane);
+          __syncwarp();
         }
       }
       tc::fence_before();
       __syncwarp();
-      if (lane == 0) arrive(lead_acce + 8 * ab);
+      if (lane == 0) arrive_relaxed(lead_acce + 8 * ab);
     }
   } else if (MODE == kDw) {
     // a lane has one 16-byte piece of each row: two 64-wide blocks of the M side, then the N side's
@@ -557,7 +659,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
           const int left = o.r1 - o.r0 - b * kBK, to = (left + 15) & ~15;
           uint4* at = reinterpret_cast<uint4*>(smem + pad + stage * kStageBytes + (lane >> 3) * 8192 + (lane & 7) * 16);
           for (int r = left; r < to; ++r) at[r * 8] = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
+          asm volatile("fence.proxy.async;" ::: "memory");
           __syncwarp();
           if (lane == 0) arrive(lead_full + 8 * stage);
         }
@@ -673,8 +775,57 @@ bool on_tensor_cores(const ccb_nn_grouped_matmul_t* a) {
 bool on_tensor_cores(const ccb_nn_grouped_matmul_dw_t* a) {
   return a->dtype != CCB_F32 && a->rows > 0 && tma_ok(a->x, a->rows, a->x_stride) && tma_ok(a->dy, a->rows, a->dy_stride);
 }
-size_t workspace_of(const ccb_nn_grouped_matmul_t*) { return 0; }
-size_t workspace_of(const ccb_nn_grouped_matmul_dw_t*) { return 0; }
+
+// In how many parts a contraction of `steps` is cut where there are too few
+// tiles to fill the 74 pairs: the cheapest by a model of waves of tiles
+// (0.35 us a step; a part's result is written and read in F32 at 5 TB/s, and
+// their sum is a launch). `tiles` is the most that the sizes can give, since
+// only the device knows which experts have rows.
+int parts_of(i64 tiles, i64 steps, i64 result) {
+  constexpr double kStep = 0.35, kSum = 2.5, kByte = 1.0 / 5e6;
+  constexpr i64 kPairs = 74;
+  int best = 1;
+  double least = 0.0;
+  for (int s = 1; s <= 32 && (s == 1 || steps / s >= 4); ++s) {
+    const double t = (double)((tiles * s + kPairs - 1) / kPairs) * (double)((steps + s - 1) / s) * kStep + (s > 1 ? kSum + (double)result * s * 8 * kByte : 0.0);
+    if (s == 1 || t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
+}
+i64 ceil_div(i64 a, i64 b) { return (a + b - 1) / b; }
+int parts_of(const ccb_nn_grouped_matmul_t* a) {
+  if (!on_tensor_cores(a) || a->rows == 0 || a->n == 0) return 1;
+  const i64 tiles = ceil_div(a->n, tcg::kFeat) * ((a->experts < a->rows ? a->experts : a->rows) + a->rows / tcg::kTok);
+  return parts_of(tiles, ceil_div(a->k, tcg::kBK), a->rows * a->n);
+}
+int parts_of(const ccb_nn_grouped_matmul_dw_t* a) {
+  if (!on_tensor_cores(a) || a->k == 0 || a->n == 0) return 1;
+  return parts_of(ceil_div(a->n, tcg::kFeat) * ceil_div(a->k, tcg::kTok) * a->experts, ceil_div(a->rows, a->experts * tcg::kBK), a->experts * a->k * a->n);
+}
+template <class A>
+size_t parts_bytes(const A* a, i64 result) {
+  const int parts = parts_of(a);
+  return parts > 1 ? (size_t)parts * result * sizeof(float) : 0;
+}
+size_t workspace_of(const ccb_nn_grouped_matmul_t* a) { return parts_bytes(a, a->rows * a->n); }
+size_t workspace_of(const ccb_nn_grouped_matmul_dw_t* a) { return parts_bytes(a, a->experts * a->k * a->n); }
+// "" if the workspace is enough
+template <class A>
+std::string check_workspace(const A* a) {
+  const size_t need = workspace_of(a);
+  if (need == 0 || (a->workspace && aligned(a->workspace, 16) && a->workspace_bytes >= need)) return "";
+  return "workspace of " + std::to_string(a->workspace_bytes) + " bytes: " + std::to_string(need) + " are needed, 16-byte aligned";
+}
+
+template <class TO>
+int sum_parts(const tcg::P& p, TO* out, i64 rows, i64 cols, i64 os, i64 mats, i64 oe, int sms, cudaStream_t st, const char* me) {
+  const i64 blocks = ceil_div(rows * cols * mats, 256), most = (i64)sms * 8;
+  tcg::add_parts<TO><<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(static_cast<const float*>(p.out), p.split_stride, p.splits, out, rows, cols, os, mats, oe);
+  return launched(me);
+}
 
 // The map of an MN-major operand: `outer` matrices of `rows` (the contraction)
 // by `cols`. Where rows are whole 64-wide blocks, one copy takes two of them:
@@ -717,8 +868,17 @@ int tensor_forward(const ccb_nn_grouped_matmul_t* a, int sms, cudaStream_t st, c
   p.experts = (int)a->experts;
   p.n = (int)a->n;
   p.k = (int)a->k;
-  p.splits = 1;
+  p.splits = parts_of(a);
   p.format = fmt;
+  p.vec = aligned(a->out, 16) && a->out_stride % 8 == 0;
+  if (p.splits > 1) {
+    p.out = a->workspace;
+    p.os = a->n;
+    p.split_stride = a->rows * a->n;
+    if (const int rc = a->transpose_w ? tcg::go<float, tcg::kForwardT>(p, sms, st, me) : tcg::go<float, tcg::kForward>(p, sms, st, me)) return rc;
+    return fmt ? sum_parts(p, (__nv_bfloat16*)a->out, a->rows, a->n, a->out_stride, 1, 0, sms, st, me)
+               : sum_parts(p, (__half*)a->out, a->rows, a->n, a->out_stride, 1, 0, sms, st, me);
+  }
   if (a->transpose_w) return fmt ? tcg::go<__nv_bfloat16, tcg::kForwardT>(p, sms, st, me) : tcg::go<__half, tcg::kForwardT>(p, sms, st, me);
   return fmt ? tcg::go<__nv_bfloat16, tcg::kForward>(p, sms, st, me) : tcg::go<__half, tcg::kForward>(p, sms, st, me);
 }
@@ -737,8 +897,19 @@ int tensor_dw(const ccb_nn_grouped_matmul_dw_t* a, int sms, cudaStream_t st, con
   p.experts = (int)a->experts;
   p.n = (int)a->n;
   p.k = (int)a->k;
-  p.splits = 1;
+  p.splits = parts_of(a);
   p.format = fmt;
+  p.vec = aligned(a->out, 16) && a->out_row_stride % 8 == 0 && (a->experts == 1 || a->out_stride % 8 == 0);
+  if (p.splits > 1) {
+    p.out = a->workspace;
+    p.os = a->n;
+    p.oe = a->k * a->n;
+    p.split_stride = a->experts * p.oe;
+    if (const int rc = tcg::go<float, tcg::kDw>(p, sms, st, me)) return rc;
+    if (a->out_dtype == CCB_F32) return sum_parts(p, (float*)a->out, a->k, a->n, a->out_row_stride, a->experts, a->out_stride, sms, st, me);
+    return fmt ? sum_parts(p, (__nv_bfloat16*)a->out, a->k, a->n, a->out_row_stride, a->experts, a->out_stride, sms, st, me)
+               : sum_parts(p, (__half*)a->out, a->k, a->n, a->out_row_stride, a->experts, a->out_stride, sms, st, me);
+  }
   if (a->out_dtype == CCB_F32) return tcg::go<float, tcg::kDw>(p, sms, st, me);
   return fmt ? tcg::go<__nv_bfloat16, tcg::kDw>(p, sms, st, me) : tcg::go<__half, tcg::kDw>(p, sms, st, me);
 }
@@ -779,6 +950,8 @@ extern "C" int ccb_nn_grouped_matmul(const ccb_nn_grouped_matmul_t* a, void* str
     if (a->rows == 0 || a->n == 0) return CCB_OK;
     if (!a->offsets || !a->out || (a->k > 0 && (!a->x || !a->w))) return fail(CCB_ERR_INVALID, me, "null pointer");
     if (!aligned(a->offsets, 4) || !aligned(a->err, 4)) return fail(CCB_ERR_INVALID, me, "offsets or err is not aligned to 4 bytes");
+    const std::string small = check_workspace(a);
+    if (!small.empty()) return fail(CCB_ERR_INVALID, me, small);
     int sms = 0;
     if (const int rc = sm_count(me, &sms)) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -803,6 +976,8 @@ extern "C" int ccb_nn_grouped_matmul_dw(const ccb_nn_grouped_matmul_dw_t* a, voi
     if (a->k == 0 || a->n == 0) return CCB_OK;
     if (!a->offsets || !a->out || (a->rows > 0 && (!a->x || !a->dy))) return fail(CCB_ERR_INVALID, me, "null pointer");
     if (!aligned(a->offsets, 4) || !aligned(a->err, 4)) return fail(CCB_ERR_INVALID, me, "offsets or err is not aligned to 4 bytes");
+    const std::string small = check_workspace(a);
+    if (!small.empty()) return fail(CCB_ERR_INVALID, me, small);
     int sms = 0;
     if (const int rc = sm_count(me, &sms)) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
