@@ -305,11 +305,9 @@ __device__ __forceinline__ void load4(unsigned dst, const ccb::TmaDesc* map, int
       : "memory");
 }
 __device__ __forceinline__ void mma(unsigned d, ccb::u64 a, ccb::u64 b, unsigned idesc, unsigned accumulate) {
-  const unsigned z = 0;
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z), "r"(z));
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+               "r"(accumulate)
+               : "memory");
 }
 // Operand descriptors of 16-bit tiles with the 128-byte swizzle. K-major:
 // 128-byte rows of 64 along the contraction, 8-row groups 1024 bytes apart, 16
@@ -424,6 +422,17 @@ __device__ __forceinline__ void drain32(unsigned taddr, bool zero, float* out, i
   }
 }
 
+// One thread of a converged warp. The loops that issue copies and MMAs are run
+// by whole warps and only the instructions themselves by the elected thread:
+// with one lane in the loop the compiler cannot keep descriptors, barriers and
+// counters in uniform registers (a step's MMAs and commits took 407 cycles so,
+// 157 this way; a 256 x 256 x 64 step is 512 cycles of the tensor pipe).
+__device__ __forceinline__ bool elect_one() {
+  unsigned ok;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(ok));
+  return ok != 0;
+}
+
 struct Tile {
   int expert;      // -1: rows of no expert
   int r0, r1;      // rows: of the result (forward), of the contraction (dw)
@@ -519,15 +528,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
   const unsigned lead_full = tc2::peer_addr(&s.full[0], 0), lead_acce = tc2::peer_addr(&s.acce[0], 0);
 
   if (warp == 0) {
-    if (lane == 0) {
-      unsigned st = 0, at = ring, phase = 1;  // 8 * stage, its address
-      for (unsigned t = pair; t < tiles; t += pairs) {
-        const Tile o = tile_at<MODE>(p, s.g, t);
-        const int half = o.nn >> 1, f = o.f0 + (int)rank * 128, c = o.c0 + (int)rank * half, tok = o.r0 + (int)rank * half;
-        const int boxes = MODE == kDw ? (p.b2 ? 1 : half / 64) : (half + p.box - 1) / p.box;
-        const unsigned box = MODE == kDw ? (p.b2 ? 16384u : 8192u) : (unsigned)p.box * 128u, bytes = kABytes + boxes * box;
-        for (int b = o.b0; b < o.b1; ++b) {
-          wait(empty + st, phase);
+    const bool one = elect_one();
+    unsigned st = 0, at = ring, phase = 1;  // 8 * stage, its address
+    for (unsigned t = pair; t < tiles; t += pairs) {
+      const Tile o = tile_at<MODE>(p, s.g, t);
+      const int half = o.nn >> 1, f = o.f0 + (int)rank * 128, c = o.c0 + (int)rank * half, tok = o.r0 + (int)rank * half;
+      const int boxes = MODE == kDw ? (p.b2 ? 1 : half / 64) : (half + p.box - 1) / p.box;
+      const unsigned box = MODE == kDw ? (p.b2 ? 16384u : 8192u) : (unsigned)p.box * 128u, bytes = kABytes + boxes * box;
+      for (int b = o.b0; b < o.b1; ++b) {
+        wait(empty + st, phase);
+        if (one) {
           unsigned bar = lead_full + st;
           if (clears<MODE>(o, b)) {
             bar = part + st;
@@ -568,19 +578,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
               load4(sb, &p.tb, k0, tok + i * p.box, 0, 0, bar);
             }
           }
-          st += 8;
-          at += kStageBytes;
-          if (st == 8 * kStages) {
-            st = 0;
-            at = ring;
-            phase ^= 1u;
-          }
+        }
+        __syncwarp();
+        st += 8;
+        at += kStageBytes;
+        if (st == 8 * kStages) {
+          st = 0;
+          at = ring;
+          phase ^= 1u;
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr bool amn = MODE != kForwardT, bmn = MODE == kDw;
+      const bool one = elect_one();
       const unsigned base = (1u << 4) | ((unsigned)p.format << 7) | ((unsigned)p.format << 10) | ((amn ? 1u : 0u) << 15) | ((bmn ? 1u : 0u) << 16) | (16u << 24);
       const u64 a0 = desc<amn>(ring), b0 = desc<bmn>(ring + kABytes);
       const unsigned empty0 = tc2::peer_addr(&s.empty[0], 0), empty1 = tc2::peer_addr(&s.empty[0], 1);
@@ -596,15 +608,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
         for (int b = o.b0; b < o.b1; ++b) {
           wait(full + st, phase);
           tc::fence_after();
-          if (clears<MODE>(o, b)) {
-            const int kks = (o.r1 - o.r0 - b * kBK + 15) / 16;
-            for (int kk = 0; kk < kks; ++kk) mma(d, a + kk * desc_step<amn>(), bd + kk * desc_step<bmn>(), idesc, b > o.b0 || kk > 0 ? 1u : 0u);
-          } else {
+          if (one) {
+            if (clears<MODE>(o, b)) {
+              const int kks = (o.r1 - o.r0 - b * kBK + 15) / 16;
+              for (int kk = 0; kk < kks; ++kk) mma(d, a + kk * desc_step<amn>(), bd + kk * desc_step<bmn>(), idesc, b > o.b0 || kk > 0 ? 1u : 0u);
+            } else {
 #pragma unroll
-            for (int kk = 0; kk < kBK / 16; ++kk) mma(d, a + kk * desc_step<amn>(), bd + kk * desc_step<bmn>(), idesc, b > o.b0 || kk > 0 ? 1u : 0u);
+              for (int kk = 0; kk < kBK / 16; ++kk) mma(d, a + kk * desc_step<amn>(), bd + kk * desc_step<bmn>(), idesc, b > o.b0 || kk > 0 ? 1u : 0u);
+            }
+            commit(empty0 + st);
+            commit(empty1 + st);
           }
-          commit(empty0 + st);
-          commit(empty1 + st);
+          __syncwarp();
           st += 8;
           a += kStageBytes >> 4;
           bd += kStageBytes >> 4;
@@ -615,8 +630,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
             phase ^= 1u;
           }
         }
-        commit(accf0 + 8 * ab);
-        commit(accf1 + 8 * ab);
+        if (one) {
+          commit(accf0 + 8 * ab);
+          commit(accf1 + 8 * ab);
+        }
+        __syncwarp();
       }
     }
   } else if (warp < 2 + kDrain) {
