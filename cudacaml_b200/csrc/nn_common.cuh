@@ -11,6 +11,7 @@
 #include <cstdint>
 #include <exception>
 #include <string>
+#include <type_traits>
 
 #include "../../include/ccb.h"
 
@@ -87,6 +88,17 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// Two results in one 32-bit word of a 16-bit type.
+template <class T>
+__device__ __forceinline__ unsigned pack2(float lo, float hi) {
+  unsigned r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 
 // Element i of a vector whose type is known at run time (weights, biases).
 __device__ __forceinline__ float load_as(const void* p, int dtype, i64 i) {

@@ -334,19 +334,6 @@ __device__ __forceinline__ void load_fragments(unsigned taddr, unsigned* v) {
                  : "r"(taddr + ((unsigned)(16 * h) << 16)));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-template <class TO>
-__device__ __forceinline__ unsigned pack(unsigned lo, unsigned hi) {
-  unsigned r;
-  if constexpr (sizeof(TO) == 2) {
-    if constexpr (std::is_same<TO, __half>::value)
-      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(__uint_as_float(hi)), "f"(__uint_as_float(lo)));
-    else
-      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(__uint_as_float(hi)), "f"(__uint_as_float(lo)));
-  } else {
-    r = 0;
-  }
-  return r;
-}
 // A warp's 32 features x 32 tokens to `out` (its first feature and token), in
 // 16 bits: turned through shared memory so that a lane stores 16 bytes of one
 // token (four packed transposing stores of 8x8 matrices; 64-byte rows, their
@@ -363,7 +350,7 @@ __device__ __forceinline__ void drain16(unsigned taddr, bool zero, unsigned buf,
     load_fragments(taddr, v);
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) h[i] = pack<TO>(v[2 * i], v[2 * i + 1]);
+  for (int i = 0; i < 16; ++i) h[i] = pack2<TO>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
   // token 8 j + lane % 8, piece lane / 8: the swap depends on the lane alone
   const unsigned put = buf + (lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4);
 #pragma unroll

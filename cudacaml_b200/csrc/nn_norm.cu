@@ -11,6 +11,9 @@
 // with the terms in brackets for the layer norm only. Statistics and sums are
 // F32; the layer norm's variance is of the centred row (a second pass), since
 // mean(v^2) - mean(v)^2 cancels where the mean is large.
+#include <initializer_list>
+#include <type_traits>
+
 #include "nn_common.cuh"
 
 namespace ccb_nn {
@@ -189,17 +192,561 @@ __global__ void __launch_bounds__(kBlock) norm_back_any(const __grid_constant__ 
   }
 }
 
-// Column sums of the blocks' partials, in block order.
-__global__ void __launch_bounds__(kBlock) norm_back_sum(const __grid_constant__ BackP p, int blocks) {
-  float* out = p.vec[blockIdx.y];
-  const i64 c = (i64)blockIdx.x * kBlock + threadIdx.x;
-  if (!out || c >= p.cols) return;
-  float t = 0.0f;
-  for (int i = 0; i < blocks; ++i) t += p.part[((i64)i * kVecs + blockIdx.y) * p.cols + c];
-  out[c] = t;
+// -------------------------------------------------------- rows read once
+// A group of `tpr` threads (whole warps) holds a row of up to 8 * tpr columns,
+// 8 elements a thread. VEC (cols a multiple of 8; pointers and strides of 16
+// bytes): consecutive ones, copied asynchronously to a place of the thread's
+// own in shared memory one or more rows ahead, so that no registers and no
+// barrier stand between loads in flight and the row in hand. Otherwise single
+// elements tpr apart, in registers. A block holds blockDim.x / tpr rows at a
+// time and takes every grid-th set; groups meet at barriers of their own.
+constexpr int kE = 8;
+
+template <bool VEC>
+struct Place {
+  int t, tpr, cols;
+  __device__ __forceinline__ int at(int i) const { return VEC ? t * kE + i : i * tpr + t; }
+  __device__ __forceinline__ bool on(int i) const { return VEC ? t * kE < cols : i * tpr + t < cols; }
+  // Where a thread has several pieces: the k-th.
+  __device__ __forceinline__ Place piece(int k) const { return {VEC ? t + k * tpr : t + k * kE * tpr, tpr, cols}; }
+};
+
+// A thread's 8 elements of one row of A: in shared memory, or in registers.
+template <class A, bool VEC>
+struct Piece {
+  static constexpr unsigned kBytes = kE * sizeof(A);
+  static __device__ __forceinline__ void fetch(unsigned to, const A* row, const Place<VEC>& w) {
+    if (!w.on(0)) return;
+#pragma unroll
+    for (unsigned j = 0; j < kBytes; j += 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + j), "l"(reinterpret_cast<const char*>(row + w.at(0)) + j) : "memory");
+  }
+  // As F32; `from` is the thread's place.
+  static __device__ __forceinline__ void get(float* v, unsigned from) {
+    unsigned u[kBytes / 4];
+#pragma unroll
+    for (unsigned j = 0; j < kBytes / 16; ++j)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u[4 * j]), "=r"(u[4 * j + 1]), "=r"(u[4 * j + 2]), "=r"(u[4 * j + 3]) : "r"(from + 16 * j));
+#pragma unroll
+    for (int i = 0; i < kE; ++i) {
+      if constexpr (sizeof(A) == 4)
+        v[i] = __uint_as_float(u[i]);
+      else if constexpr (std::is_same<A, __nv_bfloat16>::value)
+        v[i] = __uint_as_float(i & 1 ? u[i >> 1] & 0xFFFF0000u : u[i >> 1] << 16);
+      else
+        v[i] = __half2float(__ushort_as_half((unsigned short)(i & 1 ? u[i >> 1] >> 16 : u[i >> 1])));
+    }
+  }
+};
+template <class A, bool VEC>
+__device__ __forceinline__ void load8(float* v, const A* row, const Place<VEC>& w) {
+#pragma unroll
+  for (int i = 0; i < kE; ++i) v[i] = w.on(i) ? to_f<A>(row[w.at(i)]) : 0.0f;
+}
+template <class A, bool VEC>
+__device__ __forceinline__ void store8(A* row, const float* v, const Place<VEC>& w) {
+  if constexpr (VEC) {
+    if (!w.on(0)) return;
+    A* p = row + w.at(0);
+    if constexpr (sizeof(A) == 4) {
+      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint4 u;
+      u.x = pack2<A>(v[0], v[1]);
+      u.y = pack2<A>(v[2], v[3]);
+      u.z = pack2<A>(v[4], v[5]);
+      u.w = pack2<A>(v[6], v[7]);
+      *reinterpret_cast<uint4*>(p) = u;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kE; ++i)
+      if (w.on(i)) row[w.at(i)] = from_f<A>(v[i]);
+  }
+}
+// A vector over the columns, of a type known at run time; `none` where there
+// is no vector or no column. It stays in L1 from row to row.
+template <bool VEC>
+__device__ __forceinline__ void vec8(float* v, const void* p, int dtype, float none, const Place<VEC>& w) {
+#pragma unroll
+  for (int j = 0; j < kE; ++j) v[j] = none;
+  if (!p) return;
+  if constexpr (VEC) {
+    if (!w.on(0)) return;
+    if (dtype == CCB_F32) {
+      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + w.at(0));
+      const float4 a = q[0], b = q[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(p) + w.at(0));
+      const unsigned q[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < kE; ++j) {
+        const unsigned h = j & 1 ? q[j >> 1] >> 16 : q[j >> 1] & 0xFFFFu;
+        v[j] = dtype == CCB_BF16 ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kE; ++j)
+      if (w.on(j)) v[j] = load_as(p, dtype, w.at(j));
+  }
 }
 
-constexpr i64 kBackBlocks = 296;  // most blocks (and partial sums) of the gradient
+// Sums of N values over a group, the same bits in every thread: warps by
+// shuffles, then their results in warp order, in two buffers in turn, so that
+// one barrier a sum is enough.
+struct Group {
+  float* s;  // [2][warps][4]
+  int warps, id, threads, turn;
+  __device__ __forceinline__ Group(float* all, int tpr) : warps(tpr >> 5), id(threadIdx.x / tpr), threads(tpr), turn(0) { s = all + id * warps * 8; }
+  template <int N>
+  __device__ __forceinline__ void sum(float* v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+    if (warps == 1) return;
+    float* b = s + turn * warps * 4;
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) {
+      const int warp = (threadIdx.x >> 5) - id * warps;
+#pragma unroll
+      for (int n = 0; n < N; ++n) b[warp * 4 + n] = v[n];
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory");
+    float t[N] = {};
+    for (int i = 0; i < warps; ++i) {
+      const float4 w = *reinterpret_cast<const float4*>(b + 4 * i);
+      const float u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int n = 0; n < N; ++n) t[n] += u[n];
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = t[n];
+  }
+};
+
+// Which of the thread's elements of a row are kept, as bits. e0: the row's
+// first index. 8 consecutive ones span two of the generator's blocks, or three.
+template <bool VEC>
+__device__ __forceinline__ unsigned keep_bits(const Drop& d, u64 e0, const Place<VEC>& w) {
+  if (!d.on) return 0xffu;
+  unsigned bits = 0, u[4];
+  if constexpr (VEC) {
+    e0 += (u64)w.at(0);
+    const int shift = (int)(e0 & 3);
+    const u64 q = e0 >> 2;
+    for (int b = 0; b < (shift ? 3 : 2); ++b) {
+      philox4(d, q + b, u);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bits |= (u[j] > d.last ? 1u : 0u) << (4 * b + j);
+    }
+    return bits >> shift;
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < kE; ++i) {
+      if (!w.on(i)) continue;
+      const u64 e = e0 + (u64)w.at(i);
+      philox4(d, e >> 2, u);
+      const unsigned j = (unsigned)e & 3u;
+      bits |= ((j == 0 ? u[0] : j == 1 ? u[1] : j == 2 ? u[2] : u[3]) > d.last ? 1u : 0u) << i;
+    }
+    return bits;
+  }
+}
+
+// act(g) from the hardware's exponential and reciprocal: a few units in the
+// last place, below the rounding of any 16-bit result and within 1e-6 in F32.
+__device__ __forceinline__ float fast_act(int act, float g) {
+  return act == 1 ? __fdividef(1.0f, 1.0f + __expf(-g)) : act == 2 ? tanhf(g) : g;
+}
+// The gate's row where it is not a matrix of T: one for all, or in f32.
+__device__ __forceinline__ const void* gate_row(const void* gate, int gdt, i64 gs, i64 r) {
+  return gate ? static_cast<const char*>(gate) + r * gs * (gdt == CCB_F32 ? 4 : 2) : nullptr;
+}
+
+template <class T, class TX, bool VEC>
+__global__ void __launch_bounds__(1024) norm_rows(const __grid_constant__ NormP p, int kind, int tpr, int ahead) {
+  __shared__ __align__(16) float s[32 * 8];
+  extern __shared__ __align__(16) unsigned char places[];
+  typedef Piece<TX, VEC> PX;
+  typedef Piece<T, VEC> PT;
+  constexpr unsigned kPlace = PX::kBytes + 2 * PT::kBytes;
+  Group g(s, tpr);
+  const Place<VEC> w = {(int)threadIdx.x - g.id * tpr, tpr, (int)p.cols};
+  const float inv = 1.0f / (float)p.cols, f = p.scale * p.d.factor;
+  const bool full = p.gate && p.gs != 0 && p.gdt != CCB_F32;
+  const i64 sets = blockDim.x / tpr, first = (i64)blockIdx.x * sets + g.id, step = (i64)gridDim.x * sets;
+  const unsigned mine = (unsigned)__cvta_generic_to_shared(places) + threadIdx.x * kPlace, next = blockDim.x * kPlace;
+  auto fetch = [&](i64 r, unsigned to) {
+    if (VEC && r < p.rows) {
+      PX::fetch(to, static_cast<const TX*>(p.x) + r * p.xs, w);
+      if (p.b) PT::fetch(to + PX::kBytes, static_cast<const T*>(p.b) + r * p.bs, w);
+      if (full) PT::fetch(to + PX::kBytes + PT::kBytes, static_cast<const T*>(p.gate) + r * p.gs, w);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if constexpr (VEC) {
+    if (!w.on(0))
+      for (unsigned j = 0; j < ahead * next; j += next)
+        for (unsigned i = 0; i < kPlace; i += 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(mine + j + i), "r"(0));
+    for (int a = 0; a + 1 < ahead; ++a) fetch(first + a * step, mine + a * next);
+  }
+  int slot = 0;
+  for (i64 r = first; r < p.rows; r += step) {
+    float y[kE], b[kE], gt[kE];
+    const unsigned here = mine + slot * next;
+    if constexpr (VEC) {
+      fetch(r + (ahead - 1) * step, mine + (slot == 0 ? ahead - 1 : slot - 1) * next);
+      if (++slot == ahead) slot = 0;
+      if (ahead == 1)
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+      else if (ahead == 2)
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else if (ahead == 3)
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else
+        asm volatile("cp.async.wait_group 3;" ::: "memory");
+      if (p.b) PT::get(b, here + PX::kBytes);
+    } else {
+      load8<TX>(y, static_cast<const TX*>(p.x) + r * p.xs, w);
+      if (p.b) load8<T>(b, static_cast<const T*>(p.b) + r * p.bs, w);
+      if (full) load8<T>(gt, static_cast<const T*>(p.gate) + r * p.gs, w);
+    }
+    if (p.b) {
+      float m2 = 0.0f, r2 = 1.0f, t[1];
+      if (p.post) {
+        if (kind == 1) {
+          t[0] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kE; ++i) t[0] += b[i];
+          g.sum<1>(t);
+          m2 = t[0] * inv;
+        }
+        t[0] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kE; ++i)
+          if (w.on(i)) t[0] += (b[i] - m2) * (b[i] - m2);
+        g.sum<1>(t);
+        r2 = rsqrtf(t[0] * inv + p.eps);
+      }
+      const unsigned keep = keep_bits<VEC>(p.d, p.d.base + (u64)(r * p.cols), w);
+      float v[kE];
+      vec8(v, p.w2, p.wdt, 1.0f, w);
+#pragma unroll
+      for (int i = 0; i < kE; ++i) b[i] = (b[i] - m2) * r2 * v[i];
+      if (p.c2) {
+        vec8(v, p.c2, p.wdt, 0.0f, w);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) b[i] += v[i];
+      }
+      if (p.gate) {
+        if (!full)
+          vec8(gt, gate_row(p.gate, p.gdt, p.gs, r), p.gdt, 0.0f, w);
+        else if constexpr (VEC)
+          PT::get(gt, here + PX::kBytes + PT::kBytes);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) b[i] *= fast_act(p.act, gt[i]);
+      }
+      if constexpr (VEC) PX::get(y, here);
+#pragma unroll
+      for (int i = 0; i < kE; ++i) y[i] += (keep >> i) & 1u ? f * b[i] : 0.0f;
+    } else if constexpr (VEC) {
+      PX::get(y, here);
+    }
+    if (p.y) store8<TX>(static_cast<TX*>(p.y) + r * p.ys, y, w);
+    if (!p.h) continue;
+    float m1 = 0.0f, t[1];
+    if (kind == 1) {
+      t[0] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kE; ++i)
+        if (w.on(i)) t[0] += y[i];
+      g.sum<1>(t);
+      m1 = t[0] * inv;
+    }
+    t[0] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kE; ++i)
+      if (w.on(i)) t[0] += (y[i] - m1) * (y[i] - m1);
+    g.sum<1>(t);
+    const float r1 = rsqrtf(t[0] * inv + p.eps);
+    float v[kE];
+    vec8(v, p.w1, p.wdt, 1.0f, w);
+#pragma unroll
+    for (int i = 0; i < kE; ++i) y[i] = (y[i] - m1) * r1 * v[i];
+    if (p.c1) {
+      vec8(v, p.c1, p.wdt, 0.0f, w);
+#pragma unroll
+      for (int i = 0; i < kE; ++i) y[i] += v[i];
+    }
+    store8<T>(static_cast<T*>(p.h) + r * p.hs, y, w);
+  }
+  if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// The gradient, PIECES times 8 elements a thread. MORE: also the sums of the
+// biases' and of a channel gate's gradient. A row takes two sums over it (the
+// statistics and the first norm's terms; the second norm's terms), three for
+// the layer norm; between them the row is read again from shared memory (VEC),
+// piece by piece, which leaves registers for the sums over rows: they stay in
+// them for all of a thread's rows.
+template <class T, class TX, bool VEC, int PIECES, bool MORE>
+__global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ BackP p, int kind, int tpr, int ahead) {
+  __shared__ __align__(16) float s[16 * 8];
+  extern __shared__ __align__(16) unsigned char places[];
+  typedef Piece<TX, VEC> PX;
+  typedef Piece<T, VEC> PT;
+  constexpr unsigned kY = 0, kDy = PX::kBytes, kDh = 2 * PX::kBytes, kB = kDh + PT::kBytes, kG = kB + PT::kBytes, kPlace = kG + PT::kBytes;
+  Group g(s, tpr);
+  const Place<VEC> w0 = {(int)threadIdx.x - g.id * tpr, tpr, (int)p.cols};
+  const float inv = 1.0f / (float)p.cols, f = p.scale * p.d.factor;
+  const bool full = p.gate && p.gs != 0 && p.gdt != CCB_F32, norm2 = p.b && p.post;
+  const i64 sets = blockDim.x / tpr, first = (i64)blockIdx.x * sets + g.id, step = (i64)gridDim.x * sets;
+  const unsigned piece = blockDim.x * kPlace, next = PIECES * piece, mine = (unsigned)__cvta_generic_to_shared(places) + threadIdx.x * kPlace;
+  float acc[MORE ? kVecs : 2][PIECES * kE];  // dw1, dw2, then dc1, dc2, dgate
+#pragma unroll
+  for (int v = 0; v < (MORE ? kVecs : 2); ++v)
+#pragma unroll
+    for (int i = 0; i < PIECES * kE; ++i) acc[v][i] = 0.0f;
+  auto fetch = [&](i64 r, unsigned to) {
+    if (VEC && r < p.rows) {
+#pragma unroll
+      for (int k = 0; k < PIECES; ++k) {
+        const Place<VEC> w = w0.piece(k);
+        const unsigned at = to + k * piece;
+        if (p.dh) {
+          PX::fetch(at + kY, static_cast<const TX*>(p.y) + r * p.ys, w);
+          PT::fetch(at + kDh, static_cast<const T*>(p.dh) + r * p.dhs, w);
+        }
+        if (p.dy) PX::fetch(at + kDy, static_cast<const TX*>(p.dy) + r * p.dys, w);
+        if (p.b) PT::fetch(at + kB, static_cast<const T*>(p.b) + r * p.bs, w);
+        if (full) PT::fetch(at + kG, static_cast<const T*>(p.gate) + r * p.gs, w);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if constexpr (VEC) {
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k)
+      if (!w0.piece(k).on(0))
+        for (unsigned j = 0; j < ahead * next; j += next)
+          for (unsigned i = 0; i < kPlace; i += 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(mine + j + k * piece + i), "r"(0) : "memory");
+    for (int a = 0; a + 1 < ahead; ++a) fetch(first + a * step, mine + a * next);
+  }
+  int slot = 0;
+  for (i64 r = first; r < p.rows; r += step) {
+    const unsigned here = mine + slot * next;
+    if constexpr (VEC) {
+      fetch(r + (ahead - 1) * step, mine + (slot == 0 ? ahead - 1 : slot - 1) * next);
+      if (++slot == ahead) slot = 0;
+      if (ahead == 1)
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+      else if (ahead == 2)
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else if (ahead == 3)
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else
+        asm volatile("cp.async.wait_group 3;" ::: "memory");
+    }
+    // the row's parts, by piece
+    auto get_x = [&](float* v, const void* m, i64 stride, unsigned at, int k) {
+      if constexpr (VEC)
+        PX::get(v, here + k * piece + at);
+      else
+        load8<TX>(v, static_cast<const TX*>(m) + r * stride, w0.piece(k));
+    };
+    auto get_t = [&](float* v, const void* m, i64 stride, unsigned at, int k) {
+      if constexpr (VEC)
+        PT::get(v, here + k * piece + at);
+      else
+        load8<T>(v, static_cast<const T*>(m) + r * stride, w0.piece(k));
+    };
+    float m1 = 0.0f, f1 = 0.0f, m2 = 0.0f;
+    if (kind == 1) {
+      float t[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < PIECES; ++k) {
+        float a[kE], b[kE];
+        if (p.dh) {
+          get_x(a, p.y, p.ys, kY, k);
+#pragma unroll
+          for (int i = 0; i < kE; ++i) t[0] += a[i];
+          get_t(a, p.dh, p.dhs, kDh, k);
+          vec8(b, p.w1, p.wdt, 1.0f, w0.piece(k));
+#pragma unroll
+          for (int i = 0; i < kE; ++i) t[1] += a[i] * b[i];
+        }
+        if (norm2) {
+          get_t(a, p.b, p.bs, kB, k);
+#pragma unroll
+          for (int i = 0; i < kE; ++i) t[2] += a[i];
+        }
+      }
+      g.sum<3>(t);
+      m1 = t[0] * inv;
+      f1 = t[1] * inv;
+      m2 = t[2] * inv;
+    }
+    float q[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+      const Place<VEC> w = w0.piece(k);
+      float a[kE], b[kE], c[kE];
+      if (p.dh) {
+        get_x(a, p.y, p.ys, kY, k);
+        get_t(b, p.dh, p.dhs, kDh, k);
+        vec8(c, p.w1, p.wdt, 1.0f, w);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) {
+          if (!w.on(i)) continue;
+          a[i] -= m1;
+          q[0] += a[i] * a[i];
+          q[1] += b[i] * c[i] * a[i];
+        }
+      }
+      if (norm2) {
+        get_t(a, p.b, p.bs, kB, k);
+#pragma unroll
+        for (int i = 0; i < kE; ++i)
+          if (w.on(i)) q[2] += (a[i] - m2) * (a[i] - m2);
+      }
+    }
+    g.sum<3>(q);
+    const float r1 = rsqrtf(q[0] * inv + p.eps), a1 = q[1] * inv * r1, r2 = norm2 ? rsqrtf(q[2] * inv + p.eps) : 1.0f;
+    float g2[PIECES][kE], t[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+      const Place<VEC> w = w0.piece(k);
+      float d[kE], a[kE], b[kE], c[kE];
+      if (p.dy)
+        get_x(d, p.dy, p.dys, kDy, k);
+      else
+#pragma unroll
+        for (int i = 0; i < kE; ++i) d[i] = 0.0f;
+      if (p.dh) {
+        get_x(a, p.y, p.ys, kY, k);
+        get_t(b, p.dh, p.dhs, kDh, k);
+        vec8(c, p.w1, p.wdt, 1.0f, w);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) {
+          const float hat = (a[i] - m1) * r1;
+          d[i] += r1 * (b[i] * c[i] - hat * a1 - f1);
+          acc[0][k * kE + i] += b[i] * hat;
+          if (MORE) acc[2][k * kE + i] += b[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kE; ++i)
+        if (!w.on(i)) d[i] = 0.0f;  // 0 - mean is not 0
+      if (p.dx) store8<TX>(static_cast<TX*>(p.dx) + r * p.dxs, d, w);
+      if (!p.b) continue;
+      const unsigned keep = keep_bits<VEC>(p.d, p.d.base + (u64)(r * p.cols), w);
+      get_t(b, p.b, p.bs, kB, k);
+      vec8(c, p.w2, p.wdt, 1.0f, w);
+#pragma unroll
+      for (int i = 0; i < kE; ++i) {
+        d[i] = (keep >> i) & 1u ? f * d[i] : 0.0f;  // dz
+        b[i] = (b[i] - m2) * r2;                    // hat
+      }
+      if (p.gate) {
+        if (full)
+          get_t(a, p.gate, p.gs, kG, k);
+        else
+          vec8(a, gate_row(p.gate, p.gdt, p.gs, r), p.gdt, 0.0f, w);
+        float u[kE];
+        vec8(u, p.c2, p.wdt, 0.0f, w);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) {
+          const float v = fast_act(p.act, a[i]);
+          u[i] = d[i] * (b[i] * c[i] + u[i]) * slope_of(p.act, v);
+          if (MORE) acc[4][k * kE + i] += u[i];
+          d[i] *= v;  // du
+        }
+        if (p.dgate) {
+          if (p.gdt == CCB_F32)
+            store8<float>(static_cast<float*>(p.dgate) + r * p.dgs, u, w);
+          else
+            store8<T>(static_cast<T*>(p.dgate) + r * p.dgs, u, w);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kE; ++i) {
+        acc[1][k * kE + i] += d[i] * b[i];
+        if (MORE) acc[3][k * kE + i] += d[i];
+        g2[k][i] = d[i] * c[i];
+        t[0] += g2[k][i] * b[i];
+        t[1] += g2[k][i];
+      }
+    }
+    if (!p.db) continue;
+    float a2 = 0.0f, f2 = 0.0f;
+    if (p.post) {
+      g.sum<2>(t);
+      a2 = t[0] * inv;
+      f2 = kind == 1 ? t[1] * inv : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+      if (p.post) {
+        float b[kE];
+        get_t(b, p.b, p.bs, kB, k);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) g2[k][i] = r2 * (g2[k][i] - (b[i] - m2) * r2 * a2 - f2);
+      }
+      store8<T>(static_cast<T*>(p.db) + r * p.dbs, g2[k], w0.piece(k));
+    }
+  }
+  if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
+  // the block's partial sums: its groups', in order
+  float* all = reinterpret_cast<float*>(places);
+#pragma unroll
+  for (int a = 0; a < (MORE ? kVecs : 2); ++a) {
+    const int v = a == 0 ? 0 : a == 1 ? 2 : a == 2 ? 1 : a;
+    if (!p.vec[v]) continue;
+    if (sets > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < PIECES * kE; ++i) all[i * blockDim.x + threadIdx.x] = acc[a][i];
+      __syncthreads();
+      if (g.id == 0)
+#pragma unroll
+        for (int i = 0; i < PIECES * kE; ++i)
+          for (int o = 1; o < (int)sets; ++o) acc[a][i] += all[i * blockDim.x + o * tpr + threadIdx.x];
+    }
+    float* part = p.part + ((i64)blockIdx.x * kVecs + v) * p.cols;
+    if (g.id == 0)
+#pragma unroll
+      for (int k = 0; k < PIECES; ++k) {
+        const Place<VEC> w = w0.piece(k);
+#pragma unroll
+        for (int i = 0; i < kE; ++i)
+          if (w.on(i)) part[w.at(i)] = acc[a][k * kE + i];
+      }
+  }
+}
+
+// Column sums of the blocks' partials: a warp's 32 columns, 8 warps that each
+// take every eighth block, their results added in order.
+__global__ void __launch_bounds__(kBlock) norm_back_sum(const __grid_constant__ BackP p, int blocks) {
+  __shared__ float s[kBlock];
+  float* out = p.vec[blockIdx.y];
+  if (!out) return;
+  const i64 c = (i64)blockIdx.x * 32 + (threadIdx.x & 31);
+  float t = 0.0f;
+  if (c < p.cols)
+    for (int i = threadIdx.x >> 5; i < blocks; i += kBlock / 32) t += p.part[((i64)i * kVecs + blockIdx.y) * p.cols + c];
+  s[threadIdx.x] = t;
+  __syncthreads();
+  if (threadIdx.x < 32 && c < p.cols) {
+    for (int i = 1; i < kBlock / 32; ++i) t += s[32 * i + threadIdx.x];
+    out[c] = t;
+  }
+}
+
+constexpr i64 kBackBlocks = 296;  // most blocks (and partial sums) of the gradient; at least the SMs
 
 size_t back_bytes(i64 rows, i64 cols) { return (size_t)(rows < kBackBlocks ? rows : kBackBlocks) * kVecs * (size_t)cols * sizeof(float); }
 
@@ -222,9 +769,60 @@ void by_type(int dtype, int x_dtype, int kind, A... a) {
 #undef CCB_NN_CASE
 }
 
+// How rows are held: threads of a row (0: too long for that), of a block, and
+// rows of one group that are in hand or on their way.
+struct Shape {
+  int tpr, block, ahead, smem;
+};
+// `most`: threads of a block. `place`: bytes a thread needs for its part of a
+// row; `room`: of a block; `least`: what it needs besides.
+Shape shape_of(i64 cols, int elems, int most, bool vec, int place, int room, int least) {
+  const i64 tpr = (cols + elems * 32 - 1) / (elems * 32) * 32;
+  if (tpr > most) return {0, 0, 0, 0};
+  const int groups = tpr >= 512 ? 1 : (int)(512 / tpr);
+  Shape f = {(int)tpr, (int)tpr * groups, 1, 0};
+  if (vec) {
+    const int row = f.block * place;
+    f.ahead = room / row < 1 ? 1 : room / row > 4 ? 4 : room / row;
+    f.smem = f.ahead * row;
+  }
+  if (f.smem < f.block * least) f.smem = f.block * least;
+  return f;
+}
+// 16-byte accesses along every row
+bool wide(i64 cols, std::initializer_list<const void*> ptrs, std::initializer_list<i64> strides) {
+  if (cols % 8 != 0) return false;
+  for (const void* q : ptrs)
+    if (!aligned(q, 16)) return false;
+  for (i64 t : strides)
+    if (t % 8 != 0) return false;
+  return true;
+}
+// Raises a kernel's shared-memory limit once for each device.
+template <class K>
+bool room_for(K* kernel, bool (&ready)[64]) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && __atomic_load_n(&ready[dev], __ATOMIC_RELAXED)) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024) != cudaSuccess) return false;
+  if (dev >= 0 && dev < 64) __atomic_store_n(&ready[dev], true, __ATOMIC_RELAXED);
+  return true;
+}
+
 template <class T, class TX, int KIND>
 struct Forward {
+  template <bool VEC>
+  static bool rows(const NormP& p, int sms, cudaStream_t st) {
+    static bool ready[64];
+    const Shape f = shape_of(p.cols, kE, 1024, VEC, kE * (sizeof(TX) + 2 * sizeof(T)), 104 * 1024, 0);
+    if (!f.tpr || !room_for(norm_rows<T, TX, VEC>, ready)) return false;
+    const i64 sets = (p.rows + f.block / f.tpr - 1) / (f.block / f.tpr), most = (i64)sms * (f.block > 512 ? 1 : 2);
+    norm_rows<T, TX, VEC><<<(unsigned)(sets < most ? sets : most), f.block, f.smem, st>>>(p, KIND, f.tpr, f.ahead);
+    return true;
+  }
   static void run(const NormP& p, int sms, cudaStream_t st) {
+    const bool v = wide(p.cols, {p.x, p.b, p.gate, p.w1, p.c1, p.w2, p.c2, p.y, p.h}, {p.xs, p.bs, p.gs, p.ys, p.hs});
+    if (v ? rows<true>(p, sms, st) : rows<false>(p, sms, st)) return;
     const i64 most = (i64)sms * 8;
     norm_any<T, TX, KIND><<<(unsigned)(p.rows < most ? p.rows : most), kBlock, 0, st>>>(p);
   }
@@ -232,11 +830,37 @@ struct Forward {
 
 template <class T, class TX, int KIND>
 struct Backward {
+  // The blocks of the launch, 0 if a row is too long.
+  template <bool VEC, int PIECES, bool MORE>
+  static int rows(const BackP& p, int sms, cudaStream_t st) {
+    static bool ready[64];
+    const Shape f = shape_of(p.cols, kE * PIECES, 512, VEC, PIECES * kE * (2 * sizeof(TX) + 3 * sizeof(T)), 216 * 1024, PIECES * kE * 4);
+    if (!f.tpr || !room_for(norm_back_rows<T, TX, VEC, PIECES, MORE>, ready)) return 0;
+    const i64 sets = (p.rows + f.block / f.tpr - 1) / (f.block / f.tpr);
+    const int most = sms < kBackBlocks ? sms : (int)kBackBlocks, grid = (int)(sets < most ? sets : most);
+    norm_back_rows<T, TX, VEC, PIECES, MORE><<<grid, f.block, f.smem, st>>>(p, KIND, f.tpr, f.ahead);
+    return grid;
+  }
+  // Rows of 16 elements a thread, so that a block of 512 threads (128 registers
+  // each) holds two of 4096 columns and one waits for its sums while the other
+  // computes; of 8 where two f32 rows and those on their way do not fit shared
+  // memory. The shape does not go by which sums over rows are asked for (all
+  // five spill some registers), so that the other results do not either.
+  template <bool MORE>
+  static int by_width(const BackP& p, int sms, cudaStream_t st) {
+    if (!wide(p.cols, {p.y, p.dy, p.dh, p.b, p.gate, p.w1, p.w2, p.c2, p.dx, p.db, p.dgate}, {p.ys, p.dys, p.dhs, p.bs, p.gs, p.dxs, p.dbs, p.dgs}))
+      return rows<false, 1, MORE>(p, sms, st);
+    if (p.cols <= 256 || (sizeof(TX) == 4 && p.cols <= 4096)) return rows<true, 1, MORE>(p, sms, st);
+    return rows<true, 2, MORE>(p, sms, st);
+  }
   static void run(const BackP& p, int sms, cudaStream_t st) {
-    const i64 grid = p.rows < kBackBlocks ? p.rows : kBackBlocks;
-    norm_back_any<T, TX, KIND><<<(unsigned)grid, kBlock, 0, st>>>(p);
+    int grid = p.vec[1] || p.vec[3] || p.vec[4] ? by_width<true>(p, sms, st) : by_width<false>(p, sms, st);
+    if (!grid) {
+      grid = (int)(p.rows < kBackBlocks ? p.rows : kBackBlocks);
+      norm_back_any<T, TX, KIND><<<grid, kBlock, 0, st>>>(p);
+    }
     if (p.vec[0] || p.vec[1] || p.vec[2] || p.vec[3] || p.vec[4])
-      norm_back_sum<<<dim3((unsigned)((p.cols + kBlock - 1) / kBlock), kVecs), kBlock, 0, st>>>(p, (int)grid);
+      norm_back_sum<<<dim3((unsigned)((p.cols + 31) / 32), kVecs), kBlock, 0, st>>>(p, grid);
   }
 };
 
