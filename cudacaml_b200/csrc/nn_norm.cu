@@ -193,13 +193,14 @@ __global__ void __launch_bounds__(kBlock) norm_back_any(const __grid_constant__ 
 }
 
 // -------------------------------------------------------- rows read once
-// A group of `tpr` threads (whole warps) holds a row of up to 8 * tpr columns,
-// 8 elements a thread. VEC (cols a multiple of 8; pointers and strides of 16
-// bytes): consecutive ones, copied asynchronously to a place of the thread's
-// own in shared memory one or more rows ahead, so that no registers and no
-// barrier stand between loads in flight and the row in hand. Otherwise single
-// elements tpr apart, in registers. A block holds blockDim.x / tpr rows at a
-// time and takes every grid-th set; groups meet at barriers of their own.
+// A group of `tpr` threads (whole warps) holds a row, PIECES times 8 elements
+// a thread, and copies the rows that come next into a ring in shared memory
+// meanwhile (cp.async: no registers, and nothing waits for the loads). VEC
+// (cols a multiple of 8; pointers and strides of 16 bytes): a thread's elements
+// are consecutive, and it copies and reads its own alone, so that there is no
+// barrier. Otherwise they are tpr apart, and the group copies the 16-byte
+// pieces of memory that hold the row between its threads. A block holds
+// blockDim.x / tpr rows at a time and takes every grid-th set.
 constexpr int kE = 8;
 
 template <bool VEC>
@@ -211,38 +212,70 @@ struct Place {
   __device__ __forceinline__ Place piece(int k) const { return {VEC ? t + k * tpr : t + k * kE * tpr, tpr, cols}; }
 };
 
-// A thread's 8 elements of one row of A: in shared memory, or in registers.
-template <class A, bool VEC>
-struct Piece {
-  static constexpr unsigned kBytes = kE * sizeof(A);
+// Bytes of one matrix's part of a slot of the ring. VEC: planes of 16 bytes
+// for each thread of the block (free of bank conflicts whatever a place
+// holds); else a row and its unaligned ends for each group.
+template <class A, bool VEC, int PIECES>
+__host__ __device__ inline unsigned part_bytes(int cols, int block, int tpr) {
+  return VEC ? (unsigned)(PIECES * (sizeof(A) / 2) * block * 16) : (unsigned)(block / tpr) * (((unsigned)cols * (unsigned)sizeof(A) + 31u) & ~15u);
+}
+template <class A, bool VEC, int PIECES>
+struct Part {
+  // `to`: the thread's place (VEC) or the group's, in the matrix's part.
   static __device__ __forceinline__ void fetch(unsigned to, const A* row, const Place<VEC>& w) {
-    if (!w.on(0)) return;
+    if constexpr (VEC) {
 #pragma unroll
-    for (unsigned j = 0; j < kBytes; j += 16)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + j), "l"(reinterpret_cast<const char*>(row + w.at(0)) + j) : "memory");
+      for (int k = 0; k < PIECES; ++k) {
+        if (!w.piece(k).on(0)) break;
+#pragma unroll
+        for (int h = 0; h < (int)sizeof(A) / 2; ++h)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (k * (int)sizeof(A) / 2 + h) * blockDim.x * 16),
+                       "l"(reinterpret_cast<const char*>(row + w.piece(k).at(0)) + 16 * h)
+                       : "memory");
+      }
+    } else {
+      const u64 a = reinterpret_cast<u64>(row);
+      const int bytes = (int)(a & 15) + w.cols * (int)sizeof(A);
+      for (int c = w.t * 16; c < bytes; c += w.tpr * 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + c), "l"((a & ~15ull) + c), "r"(min(16, bytes - c)) : "memory");
+    }
   }
-  // As F32; `from` is the thread's place.
-  static __device__ __forceinline__ void get(float* v, unsigned from) {
-    unsigned u[kBytes / 4];
+  // Piece k as F32, from the place that `row` was copied to.
+  static __device__ __forceinline__ void get(float* v, unsigned from, const A* row, const Place<VEC>& w, int k) {
+    if constexpr (VEC) {
+      unsigned u[kE * sizeof(A) / 4];
 #pragma unroll
-    for (unsigned j = 0; j < kBytes / 16; ++j)
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u[4 * j]), "=r"(u[4 * j + 1]), "=r"(u[4 * j + 2]), "=r"(u[4 * j + 3]) : "r"(from + 16 * j));
+      for (int h = 0; h < (int)sizeof(A) / 2; ++h)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(u[4 * h]), "=r"(u[4 * h + 1]), "=r"(u[4 * h + 2]), "=r"(u[4 * h + 3])
+                     : "r"(from + (k * (int)sizeof(A) / 2 + h) * blockDim.x * 16));
 #pragma unroll
-    for (int i = 0; i < kE; ++i) {
-      if constexpr (sizeof(A) == 4)
-        v[i] = __uint_as_float(u[i]);
-      else if constexpr (std::is_same<A, __nv_bfloat16>::value)
-        v[i] = __uint_as_float(i & 1 ? u[i >> 1] & 0xFFFF0000u : u[i >> 1] << 16);
-      else
-        v[i] = __half2float(__ushort_as_half((unsigned short)(i & 1 ? u[i >> 1] >> 16 : u[i >> 1])));
+      for (int i = 0; i < kE; ++i) {
+        if constexpr (sizeof(A) == 4)
+          v[i] = __uint_as_float(u[i]);
+        else if constexpr (std::is_same<A, __nv_bfloat16>::value)
+          v[i] = __uint_as_float(i & 1 ? u[i >> 1] & 0xFFFF0000u : u[i >> 1] << 16);
+        else
+          v[i] = __half2float(__ushort_as_half((unsigned short)(i & 1 ? u[i >> 1] >> 16 : u[i >> 1])));
+      }
+    } else {
+      const Place<VEC> q = w.piece(k);
+      const unsigned at = from + (unsigned)(reinterpret_cast<u64>(row) & 15);
+#pragma unroll
+      for (int i = 0; i < kE; ++i) {
+        v[i] = 0.0f;
+        if (!q.on(i)) continue;
+        if constexpr (sizeof(A) == 4) {
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[i]) : "r"(at + 4 * q.at(i)));
+        } else {
+          unsigned short h;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at + 2 * q.at(i)));
+          v[i] = std::is_same<A, __nv_bfloat16>::value ? __uint_as_float((unsigned)h << 16) : __half2float(__ushort_as_half(h));
+        }
+      }
     }
   }
 };
-template <class A, bool VEC>
-__device__ __forceinline__ void load8(float* v, const A* row, const Place<VEC>& w) {
-#pragma unroll
-  for (int i = 0; i < kE; ++i) v[i] = w.on(i) ? to_f<A>(row[w.at(i)]) : 0.0f;
-}
 template <class A, bool VEC>
 __device__ __forceinline__ void store8(A* row, const float* v, const Place<VEC>& w) {
   if constexpr (VEC) {
@@ -266,41 +299,53 @@ __device__ __forceinline__ void store8(A* row, const float* v, const Place<VEC>&
   }
 }
 // A vector over the columns, of a type known at run time; `none` where there
-// is no vector or no column. It stays in L1 from row to row.
+// is no vector or no column.
 template <bool VEC>
 __device__ __forceinline__ void vec8(float* v, const void* p, int dtype, float none, const Place<VEC>& w) {
 #pragma unroll
-  for (int j = 0; j < kE; ++j) v[j] = none;
-  if (!p) return;
-  if constexpr (VEC) {
-    if (!w.on(0)) return;
-    if (dtype == CCB_F32) {
-      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + w.at(0));
-      const float4 a = q[0], b = q[1];
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(p) + w.at(0));
-      const unsigned q[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < kE; ++j) {
-        const unsigned h = j & 1 ? q[j >> 1] >> 16 : q[j >> 1] & 0xFFFFu;
-        v[j] = dtype == CCB_BF16 ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kE; ++j)
-      if (w.on(j)) v[j] = load_as(p, dtype, w.at(j));
-  }
+  for (int j = 0; j < kE; ++j) v[j] = p && w.on(j) ? load_as(p, dtype, w.at(j)) : none;
 }
+// The vectors over the columns, kept in F32 in shared memory from row to row
+// (beside the ring there is no L1 left to keep them), as 16-byte halves in
+// planes of a group's threads; the groups share them.
+struct Kept {
+  unsigned at, plane;
+  __device__ __forceinline__ void put(int slot, const float* v) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + (2 * slot + h) * plane), "f"(v[4 * h]), "f"(v[4 * h + 1]), "f"(v[4 * h + 2]), "f"(v[4 * h + 3])
+                   : "memory");
+  }
+  __device__ __forceinline__ void get(int slot, float* v) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[4 * h]), "=f"(v[4 * h + 1]), "=f"(v[4 * h + 2]), "=f"(v[4 * h + 3]) : "r"(at + (2 * slot + h) * plane));
+  }
+};
+// How a launch holds its rows: threads of a row, slots of the ring and their
+// bytes, where the vectors are kept and where the generator's words go.
+struct Hold {
+  int tpr, ahead;
+  unsigned slot, kept, words;
+};
 
-// Sums of N values over a group, the same bits in every thread: warps by
-// shuffles, then their results in warp order, in two buffers in turn, so that
-// one barrier a sum is enough.
+// Sums of N values over a group, the same bits in every thread: by shuffles in
+// each warp, then over the warps' results, in two buffers in turn, so that one
+// barrier a sum is enough.
 struct Group {
   float* s;  // [2][warps][4]
-  int warps, id, threads, turn;
-  __device__ __forceinline__ Group(float* all, int tpr) : warps(tpr >> 5), id(threadIdx.x / tpr), threads(tpr), turn(0) { s = all + id * warps * 8; }
+  int warps, span, id, threads, turn;
+  __device__ __forceinline__ void meet() const {
+    if (warps == 1)
+      __syncwarp();
+    else
+      asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory");
+  }
+  __device__ __forceinline__ Group(float* all, int tpr) : warps(tpr >> 5), id(threadIdx.x / tpr), threads(tpr), turn(0) {
+    s = all + id * warps * 8;
+    span = 1;
+    while (span < warps) span *= 2;
+  }
   template <int N>
   __device__ __forceinline__ void sum(float* v) {
 #pragma unroll
@@ -310,260 +355,386 @@ struct Group {
     if (warps == 1) return;
     float* b = s + turn * warps * 4;
     turn ^= 1;
-    if ((threadIdx.x & 31) == 0) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) {
       const int warp = (threadIdx.x >> 5) - id * warps;
 #pragma unroll
       for (int n = 0; n < N; ++n) b[warp * 4 + n] = v[n];
     }
     asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory");
-    float t[N] = {};
-    for (int i = 0; i < warps; ++i) {
-      const float4 w = *reinterpret_cast<const float4*>(b + 4 * i);
-      const float u[4] = {w.x, w.y, w.z, w.w};
+    const int l = lane & (span - 1);
 #pragma unroll
-      for (int n = 0; n < N; ++n) t[n] += u[n];
-    }
+    for (int n = 0; n < N; ++n) v[n] = l < warps ? b[l * 4 + n] : 0.0f;
 #pragma unroll
-    for (int n = 0; n < N; ++n) v[n] = t[n];
+    for (int o = 16; o > 0; o >>= 1)
+      if (o < span)
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
   }
 };
 
-// Which of the thread's elements of a row are kept, as bits. e0: the row's
-// first index. 8 consecutive ones span two of the generator's blocks, or three.
+// The generator's words of a thread's 8 elements of a row whose first index is
+// e0. Consecutive elements (VEC): two of its blocks, or three where the index
+// is no multiple of 4. Single ones: a warp's 32 elements of one step lie in at
+// most 9 blocks, so the warp computes the 72 of all steps between its lanes
+// and hands the words out through its part of shared memory.
+constexpr int kWarpWords = 9 * kE * 4;
 template <bool VEC>
-__device__ __forceinline__ unsigned keep_bits(const Drop& d, u64 e0, const Place<VEC>& w) {
-  if (!d.on) return 0xffu;
-  unsigned bits = 0, u[4];
+__device__ __forceinline__ void words8(unsigned* u, const Drop& d, u64 e0, const Place<VEC>& w, unsigned char* places) {
   if constexpr (VEC) {
     e0 += (u64)w.at(0);
-    const int shift = (int)(e0 & 3);
     const u64 q = e0 >> 2;
-    for (int b = 0; b < (shift ? 3 : 2); ++b) {
-      philox4(d, q + b, u);
+    philox4(d, q, u);
+    philox4(d, q + 1, u + 4);
+    const int shift = (int)(e0 & 3);
+    if (shift) {
+      unsigned x[4];
+      philox4(d, q + 2, x);
+      for (int k = 0; k < shift; ++k) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) bits |= (u[j] > d.last ? 1u : 0u) << (4 * b + j);
+        for (int i = 0; i < kE - 1; ++i) u[i] = u[i + 1];
+        u[kE - 1] = x[0];
+        x[0] = x[1], x[1] = x[2], x[2] = x[3];
+      }
     }
-    return bits >> shift;
   } else {
-#pragma unroll 1
-    for (int i = 0; i < kE; ++i) {
-      if (!w.on(i)) continue;
-      const u64 e = e0 + (u64)w.at(i);
-      philox4(d, e >> 2, u);
-      const unsigned j = (unsigned)e & 3u;
-      bits |= ((j == 0 ? u[0] : j == 1 ? u[1] : j == 2 ? u[2] : u[3]) > d.last ? 1u : 0u) << i;
+    uint4* out = reinterpret_cast<uint4*>(places) + (threadIdx.x >> 5) * (kWarpWords / 4);
+    const int lane = threadIdx.x & 31;
+    const u64 e = e0 + (u64)(w.t - lane);  // the warp's first element of step 0
+    __syncwarp();
+    for (int b = lane; b < 9 * kE; b += 32) {
+      const int i = b / 9;
+      unsigned x[4];
+      philox4(d, ((e + (u64)(i * w.tpr)) >> 2) + (u64)(b - 9 * i), x);
+      out[b] = make_uint4(x[0], x[1], x[2], x[3]);
     }
-    return bits;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kE; ++i) u[i] = reinterpret_cast<const unsigned*>(out)[36 * i + (int)((e + (u64)(i * w.tpr)) & 3) + lane];
   }
 }
 
 // act(g) from the hardware's exponential and reciprocal: a few units in the
 // last place, below the rounding of any 16-bit result and within 1e-6 in F32.
-__device__ __forceinline__ float fast_act(int act, float g) {
-  return act == 1 ? __fdividef(1.0f, 1.0f + __expf(-g)) : act == 2 ? tanhf(g) : g;
+__device__ __forceinline__ void act8(int act, float* g) {
+  if (act == 1) {
+#pragma unroll
+    for (int i = 0; i < kE; ++i) {
+      float e;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g[i] * -1.4426950408889634f));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(g[i]) : "f"(1.0f + e));
+    }
+  } else if (act == 2) {
+#pragma unroll
+    for (int i = 0; i < kE; ++i) g[i] = tanhf(g[i]);
+  }
+}
+// act'(g) times v, from a = act(g)
+__device__ __forceinline__ void slope8(int act, const float* a, float* v) {
+  if (act == 1) {
+#pragma unroll
+    for (int i = 0; i < kE; ++i) v[i] *= a[i] * (1.0f - a[i]);
+  } else if (act == 2) {
+#pragma unroll
+    for (int i = 0; i < kE; ++i) v[i] *= 1.0f - a[i] * a[i];
+  }
 }
 // The gate's row where it is not a matrix of T: one for all, or in f32.
 __device__ __forceinline__ const void* gate_row(const void* gate, int gdt, i64 gs, i64 r) {
   return gate ? static_cast<const char*>(gate) + r * gs * (gdt == CCB_F32 ? 4 : 2) : nullptr;
 }
 
-template <class T, class TX, bool VEC>
-__global__ void __launch_bounds__(1024) norm_rows(const __grid_constant__ NormP p, int kind, int tpr, int ahead) {
-  __shared__ __align__(16) float s[32 * 8];
-  extern __shared__ __align__(16) unsigned char places[];
-  typedef Piece<TX, VEC> PX;
-  typedef Piece<T, VEC> PT;
-  constexpr unsigned kPlace = PX::kBytes + 2 * PT::kBytes;
-  Group g(s, tpr);
-  const Place<VEC> w = {(int)threadIdx.x - g.id * tpr, tpr, (int)p.cols};
-  const float inv = 1.0f / (float)p.cols, f = p.scale * p.d.factor;
-  const bool full = p.gate && p.gs != 0 && p.gdt != CCB_F32;
-  const i64 sets = blockDim.x / tpr, first = (i64)blockIdx.x * sets + g.id, step = (i64)gridDim.x * sets;
-  const unsigned mine = (unsigned)__cvta_generic_to_shared(places) + threadIdx.x * kPlace, next = blockDim.x * kPlace;
-  auto fetch = [&](i64 r, unsigned to) {
-    if (VEC && r < p.rows) {
-      PX::fetch(to, static_cast<const TX*>(p.x) + r * p.xs, w);
-      if (p.b) PT::fetch(to + PX::kBytes, static_cast<const T*>(p.b) + r * p.bs, w);
-      if (full) PT::fetch(to + PX::kBytes + PT::kBytes, static_cast<const T*>(p.gate) + r * p.gs, w);
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  if constexpr (VEC) {
-    if (!w.on(0))
-      for (unsigned j = 0; j < ahead * next; j += next)
-        for (unsigned i = 0; i < kPlace; i += 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(mine + j + i), "r"(0));
-    for (int a = 0; a + 1 < ahead; ++a) fetch(first + a * step, mine + a * next);
+// Row r of a matrix: one 32 x 32 -> 64 product (the launch sees to it that a
+// row's bytes fit) instead of a 64-bit one, and no pointer kept from row to row.
+template <class A>
+__device__ __forceinline__ const A* row_at(const void* m, unsigned r, i64 stride) {
+  return reinterpret_cast<const A*>(static_cast<const char*>(m) + (u64)r * (unsigned)(stride * (i64)sizeof(A)));
+}
+template <class A>
+__device__ __forceinline__ A* row_at(void* m, unsigned r, i64 stride) {
+  return reinterpret_cast<A*>(static_cast<char*>(m) + (u64)r * (unsigned)(stride * (i64)sizeof(A)));
+}
+// Waits until at most n of the thread's groups of copies are on their way.
+__device__ __forceinline__ void copied(int n) {
+  if (n == 1)
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else if (n == 2)
+    asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+// The row in hand is in its slot and the next one's copies are issued: one
+// slot ahead of a full ring, since the slot before the row in hand is free.
+template <bool VEC, class F>
+__device__ __forceinline__ void turn_ring(const Group& g, int ahead, F fetch) {
+  if (ahead == 1) {
+    if (!VEC) g.meet();
+    fetch();
+    copied(0);
+    if (!VEC) g.meet();
+  } else if (VEC) {
+    fetch();
+    copied(ahead - 1);
+  } else {
+    copied(ahead - 2);
+    g.meet();  // everyone's copies are in, and everyone is done with the row before
+    fetch();
   }
-  int slot = 0;
-  for (i64 r = first; r < p.rows; r += step) {
-    float y[kE], b[kE], gt[kE];
-    const unsigned here = mine + slot * next;
-    if constexpr (VEC) {
-      fetch(r + (ahead - 1) * step, mine + (slot == 0 ? ahead - 1 : slot - 1) * next);
-      if (++slot == ahead) slot = 0;
-      if (ahead == 1)
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-      else if (ahead == 2)
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else if (ahead == 3)
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
-      else
-        asm volatile("cp.async.wait_group 3;" ::: "memory");
-      if (p.b) PT::get(b, here + PX::kBytes);
-    } else {
-      load8<TX>(y, static_cast<const TX*>(p.x) + r * p.xs, w);
-      if (p.b) load8<T>(b, static_cast<const T*>(p.b) + r * p.bs, w);
-      if (full) load8<T>(gt, static_cast<const T*>(p.gate) + r * p.gs, w);
-    }
-    if (p.b) {
-      float m2 = 0.0f, r2 = 1.0f, t[1];
-      if (p.post) {
-        if (kind == 1) {
-          t[0] = 0.0f;
+}
+
+template <class T, class TX, bool VEC, int PIECES>
+__global__ void __launch_bounds__(512) norm_rows(const __grid_constant__ NormP p, int kind, const Hold hold) {
+  __shared__ __align__(16) float s[16 * 8];
+  extern __shared__ __align__(16) unsigned char places[];
+  typedef Part<TX, VEC, PIECES> PX;
+  typedef Part<T, VEC, PIECES> PT;
+  const int tpr = hold.tpr, ahead = hold.ahead;
+  Group g(s, tpr);
+  const Place<VEC> w0 = {(int)threadIdx.x - g.id * tpr, tpr, (int)p.cols};
+  const float inv = 1.0f / (float)p.cols, f = p.scale * p.d.factor;
+  const bool channel = p.gate && p.gs == 0, full = p.gate && !channel && p.gdt != CCB_F32;
+  const unsigned sets = blockDim.x / tpr, first = blockIdx.x * sets + g.id, step = gridDim.x * sets, rows = (unsigned)p.rows;
+  const unsigned all = (unsigned)__cvta_generic_to_shared(places);
+  const unsigned ox = VEC ? threadIdx.x * 16 : g.id * (part_bytes<TX, VEC, PIECES>(p.cols, blockDim.x, tpr) / sets);
+  const unsigned ob = part_bytes<TX, VEC, PIECES>(p.cols, blockDim.x, tpr) + (VEC ? threadIdx.x * 16 : g.id * (part_bytes<T, VEC, PIECES>(p.cols, blockDim.x, tpr) / sets));
+  const unsigned og = ob + part_bytes<T, VEC, PIECES>(p.cols, blockDim.x, tpr), end = all + ahead * hold.slot;
+  // kept, for each piece: w2, w1, then c2, c1 and a channel gate's act, as far as there are any
+  const Kept kept = {all + hold.kept + w0.t * 16, (unsigned)tpr * 16};
+  const int c1_at = 2 + (p.c2 != nullptr), gate_at = c1_at + (p.c1 != nullptr), slots = gate_at + channel;
+  if (g.id == 0) {
 #pragma unroll
-          for (int i = 0; i < kE; ++i) t[0] += b[i];
-          g.sum<1>(t);
-          m2 = t[0] * inv;
-        }
-        t[0] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kE; ++i)
-          if (w.on(i)) t[0] += (b[i] - m2) * (b[i] - m2);
-        g.sum<1>(t);
-        r2 = rsqrtf(t[0] * inv + p.eps);
-      }
-      const unsigned keep = keep_bits<VEC>(p.d, p.d.base + (u64)(r * p.cols), w);
+    for (int k = 0; k < PIECES; ++k) {
+      const Place<VEC> w = w0.piece(k);
       float v[kE];
       vec8(v, p.w2, p.wdt, 1.0f, w);
-#pragma unroll
-      for (int i = 0; i < kE; ++i) b[i] = (b[i] - m2) * r2 * v[i];
+      kept.put(k * slots, v);
+      vec8(v, p.w1, p.wdt, 1.0f, w);
+      kept.put(k * slots + 1, v);
       if (p.c2) {
         vec8(v, p.c2, p.wdt, 0.0f, w);
-#pragma unroll
-        for (int i = 0; i < kE; ++i) b[i] += v[i];
+        kept.put(k * slots + 2, v);
       }
-      if (p.gate) {
-        if (!full)
-          vec8(gt, gate_row(p.gate, p.gdt, p.gs, r), p.gdt, 0.0f, w);
-        else if constexpr (VEC)
-          PT::get(gt, here + PX::kBytes + PT::kBytes);
-#pragma unroll
-        for (int i = 0; i < kE; ++i) b[i] *= fast_act(p.act, gt[i]);
+      if (p.c1) {
+        vec8(v, p.c1, p.wdt, 0.0f, w);
+        kept.put(k * slots + c1_at, v);
       }
-      if constexpr (VEC) PX::get(y, here);
-#pragma unroll
-      for (int i = 0; i < kE; ++i) y[i] += (keep >> i) & 1u ? f * b[i] : 0.0f;
-    } else if constexpr (VEC) {
-      PX::get(y, here);
+      if (channel) {
+        vec8(v, p.gate, p.gdt, 0.0f, w);
+        act8(p.act, v);
+        kept.put(k * slots + gate_at, v);
+      }
     }
-    if (p.y) store8<TX>(static_cast<TX*>(p.y) + r * p.ys, y, w);
+  }
+  unsigned coming = first, to = all;
+  auto fetch = [&]() {
+    if (coming < rows) {
+      PX::fetch(to + ox, row_at<TX>(p.x, coming, p.xs), w0);
+      if (p.b) PT::fetch(to + ob, row_at<T>(p.b, coming, p.bs), w0);
+      if (full) PT::fetch(to + og, row_at<T>(p.gate, coming, p.gs), w0);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    coming += step;
+    to = to + hold.slot == end ? all : to + hold.slot;
+  };
+  if constexpr (VEC)  // columns that there are not read as 0
+    for (unsigned j = all + threadIdx.x * 16; j < end; j += blockDim.x * 16) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(j), "r"(0) : "memory");
+  __syncthreads();
+  for (int a = 0; a + 1 < ahead; ++a) fetch();
+  unsigned here = all;
+  for (unsigned r = first; r < rows; r += step) {
+    turn_ring<VEC>(g, ahead, fetch);
+    float y[PIECES][kE], t[1];
+    float m2 = 0.0f, r2 = 1.0f;
+    const T* brow = row_at<T>(p.b, r, p.bs);
+    if (p.b && p.post) {
+      if (kind == 1) {
+        t[0] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+          float b[kE];
+          PT::get(b, here + ob, brow, w0, k);
+#pragma unroll
+          for (int i = 0; i < kE; ++i) t[0] += b[i];
+        }
+        g.sum<1>(t);
+        m2 = t[0] * inv;
+      }
+      t[0] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < PIECES; ++k) {
+        float b[kE];
+        PT::get(b, here + ob, brow, w0, k);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) {
+          if (kind == 1) b[i] = w0.piece(k).on(i) ? b[i] - m2 : 0.0f;
+          t[0] += b[i] * b[i];
+        }
+      }
+      g.sum<1>(t);
+      r2 = rsqrtf(t[0] * inv + p.eps);
+    }
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+      const Place<VEC> w = w0.piece(k);
+      if (p.b) {
+        float b[kE], v[kE];
+        PT::get(b, here + ob, brow, w0, k);
+        kept.get(k * slots, v);
+        if (kind == 1) {
+#pragma unroll
+          for (int i = 0; i < kE; ++i) b[i] -= m2;
+        }
+#pragma unroll
+        for (int i = 0; i < kE; ++i) b[i] = b[i] * r2 * v[i];
+        if (p.c2) {
+          kept.get(k * slots + 2, v);
+#pragma unroll
+          for (int i = 0; i < kE; ++i) b[i] += v[i];
+        }
+        if (p.gate) {
+          if (channel) {
+            kept.get(k * slots + gate_at, v);
+          } else {
+            if (full)
+              PT::get(v, here + og, row_at<T>(p.gate, r, p.gs), w0, k);
+            else
+              vec8(v, gate_row(p.gate, p.gdt, p.gs, r), p.gdt, 0.0f, w);
+            act8(p.act, v);
+          }
+#pragma unroll
+          for (int i = 0; i < kE; ++i) b[i] *= v[i];
+        }
+        PX::get(y[k], here + ox, row_at<TX>(p.x, r, p.xs), w0, k);
+        if (p.d.on) {
+          unsigned u[kE];
+          words8<VEC>(u, p.d, p.d.base + (u64)r * (unsigned)p.cols, w, places + hold.words);
+#pragma unroll
+          for (int i = 0; i < kE; ++i) y[k][i] += u[i] > p.d.last ? f * b[i] : 0.0f;
+        } else {
+#pragma unroll
+          for (int i = 0; i < kE; ++i) y[k][i] += f * b[i];
+        }
+      } else {
+        PX::get(y[k], here + ox, row_at<TX>(p.x, r, p.xs), w0, k);
+      }
+      if (p.y) store8<TX>(row_at<TX>(p.y, r, p.ys), y[k], w);
+    }
+    here = here + hold.slot == end ? all : here + hold.slot;
     if (!p.h) continue;
-    float m1 = 0.0f, t[1];
+    float m1 = 0.0f;
     if (kind == 1) {
       t[0] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kE; ++i)
-        if (w.on(i)) t[0] += y[i];
+      for (int k = 0; k < PIECES; ++k)
+#pragma unroll
+        for (int i = 0; i < kE; ++i)
+          if (w0.piece(k).on(i)) t[0] += y[k][i];
       g.sum<1>(t);
       m1 = t[0] * inv;
     }
     t[0] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kE; ++i)
-      if (w.on(i)) t[0] += (y[i] - m1) * (y[i] - m1);
+    for (int k = 0; k < PIECES; ++k)
+#pragma unroll
+      for (int i = 0; i < kE; ++i) {
+        if (kind == 1) y[k][i] -= m1;
+        if (w0.piece(k).on(i)) t[0] += y[k][i] * y[k][i];
+      }
     g.sum<1>(t);
     const float r1 = rsqrtf(t[0] * inv + p.eps);
-    float v[kE];
-    vec8(v, p.w1, p.wdt, 1.0f, w);
 #pragma unroll
-    for (int i = 0; i < kE; ++i) y[i] = (y[i] - m1) * r1 * v[i];
-    if (p.c1) {
-      vec8(v, p.c1, p.wdt, 0.0f, w);
+    for (int k = 0; k < PIECES; ++k) {
+      float v[kE];
+      kept.get(k * slots + 1, v);
 #pragma unroll
-      for (int i = 0; i < kE; ++i) y[i] += v[i];
+      for (int i = 0; i < kE; ++i) y[k][i] = y[k][i] * r1 * v[i];
+      if (p.c1) {
+        kept.get(k * slots + c1_at, v);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) y[k][i] += v[i];
+      }
+      store8<T>(row_at<T>(p.h, r, p.hs), y[k], w0.piece(k));
     }
-    store8<T>(static_cast<T*>(p.h) + r * p.hs, y, w);
   }
-  if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// The gradient, PIECES times 8 elements a thread. MORE: also the sums of the
-// biases' and of a channel gate's gradient. A row takes two sums over it (the
-// statistics and the first norm's terms; the second norm's terms), three for
-// the layer norm; between them the row is read again from shared memory (VEC),
-// piece by piece, which leaves registers for the sums over rows: they stay in
-// them for all of a thread's rows.
+// The gradient. MORE: also the sums of the biases' and of a channel gate's
+// gradient. A row takes two sums over it (the statistics and the first norm's
+// terms; the second norm's terms), three for the layer norm; between them the
+// row is read again from the ring, piece by piece, which leaves registers for
+// the sums over rows: they stay in them for all of a thread's rows.
 template <class T, class TX, bool VEC, int PIECES, bool MORE>
-__global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ BackP p, int kind, int tpr, int ahead) {
+__global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ BackP p, int kind, const Hold hold) {
   __shared__ __align__(16) float s[16 * 8];
   extern __shared__ __align__(16) unsigned char places[];
-  typedef Piece<TX, VEC> PX;
-  typedef Piece<T, VEC> PT;
-  constexpr unsigned kY = 0, kDy = PX::kBytes, kDh = 2 * PX::kBytes, kB = kDh + PT::kBytes, kG = kB + PT::kBytes, kPlace = kG + PT::kBytes;
+  typedef Part<TX, VEC, PIECES> PX;
+  typedef Part<T, VEC, PIECES> PT;
+  const int tpr = hold.tpr, ahead = hold.ahead;
   Group g(s, tpr);
   const Place<VEC> w0 = {(int)threadIdx.x - g.id * tpr, tpr, (int)p.cols};
   const float inv = 1.0f / (float)p.cols, f = p.scale * p.d.factor;
-  const bool full = p.gate && p.gs != 0 && p.gdt != CCB_F32, norm2 = p.b && p.post;
-  const i64 sets = blockDim.x / tpr, first = (i64)blockIdx.x * sets + g.id, step = (i64)gridDim.x * sets;
-  const unsigned piece = blockDim.x * kPlace, next = PIECES * piece, mine = (unsigned)__cvta_generic_to_shared(places) + threadIdx.x * kPlace;
+  const bool channel = p.gate && p.gs == 0, full = p.gate && !channel && p.gdt != CCB_F32, norm2 = p.b && p.post;
+  const unsigned sets = blockDim.x / tpr, first = blockIdx.x * sets + g.id, step = gridDim.x * sets, rows = (unsigned)p.rows;
+  const unsigned all = (unsigned)__cvta_generic_to_shared(places), end = all + ahead * hold.slot;
+  const unsigned nx = part_bytes<TX, VEC, PIECES>(p.cols, blockDim.x, tpr), nt = part_bytes<T, VEC, PIECES>(p.cols, blockDim.x, tpr);
+  const unsigned oy = VEC ? threadIdx.x * 16 : g.id * (nx / sets), ody = oy + nx, odh = 2 * nx + (VEC ? threadIdx.x * 16 : g.id * (nt / sets)), ob = odh + nt,
+                 og = ob + nt;
   float acc[MORE ? kVecs : 2][PIECES * kE];  // dw1, dw2, then dc1, dc2, dgate
 #pragma unroll
   for (int v = 0; v < (MORE ? kVecs : 2); ++v)
 #pragma unroll
     for (int i = 0; i < PIECES * kE; ++i) acc[v][i] = 0.0f;
-  auto fetch = [&](i64 r, unsigned to) {
-    if (VEC && r < p.rows) {
+  // kept, for each piece: w1, w2, then c2 and a channel gate's act, as far as there are any
+  const Kept kept = {all + hold.kept + w0.t * 16, (unsigned)tpr * 16};
+  const int gate_at = 2 + (p.c2 != nullptr), slots = gate_at + channel;
+  if (g.id == 0) {
 #pragma unroll
-      for (int k = 0; k < PIECES; ++k) {
-        const Place<VEC> w = w0.piece(k);
-        const unsigned at = to + k * piece;
-        if (p.dh) {
-          PX::fetch(at + kY, static_cast<const TX*>(p.y) + r * p.ys, w);
-          PT::fetch(at + kDh, static_cast<const T*>(p.dh) + r * p.dhs, w);
-        }
-        if (p.dy) PX::fetch(at + kDy, static_cast<const TX*>(p.dy) + r * p.dys, w);
-        if (p.b) PT::fetch(at + kB, static_cast<const T*>(p.b) + r * p.bs, w);
-        if (full) PT::fetch(at + kG, static_cast<const T*>(p.gate) + r * p.gs, w);
+    for (int k = 0; k < PIECES; ++k) {
+      const Place<VEC> w = w0.piece(k);
+      float v[kE];
+      vec8(v, p.w1, p.wdt, 1.0f, w);
+      kept.put(k * slots, v);
+      vec8(v, p.w2, p.wdt, 1.0f, w);
+      kept.put(k * slots + 1, v);
+      if (p.c2) {
+        vec8(v, p.c2, p.wdt, 0.0f, w);
+        kept.put(k * slots + 2, v);
+      }
+      if (channel) {
+        vec8(v, p.gate, p.gdt, 0.0f, w);
+        act8(p.act, v);
+        kept.put(k * slots + gate_at, v);
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  if constexpr (VEC) {
-#pragma unroll
-    for (int k = 0; k < PIECES; ++k)
-      if (!w0.piece(k).on(0))
-        for (unsigned j = 0; j < ahead * next; j += next)
-          for (unsigned i = 0; i < kPlace; i += 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(mine + j + k * piece + i), "r"(0) : "memory");
-    for (int a = 0; a + 1 < ahead; ++a) fetch(first + a * step, mine + a * next);
   }
-  int slot = 0;
-  for (i64 r = first; r < p.rows; r += step) {
-    const unsigned here = mine + slot * next;
-    if constexpr (VEC) {
-      fetch(r + (ahead - 1) * step, mine + (slot == 0 ? ahead - 1 : slot - 1) * next);
-      if (++slot == ahead) slot = 0;
-      if (ahead == 1)
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-      else if (ahead == 2)
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else if (ahead == 3)
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
-      else
-        asm volatile("cp.async.wait_group 3;" ::: "memory");
+  unsigned coming = first, to = all;
+  auto fetch = [&]() {
+    if (coming < rows) {
+      if (p.dh) {
+        PX::fetch(to + oy, row_at<TX>(p.y, coming, p.ys), w0);
+        PT::fetch(to + odh, row_at<T>(p.dh, coming, p.dhs), w0);
+      }
+      if (p.dy) PX::fetch(to + ody, row_at<TX>(p.dy, coming, p.dys), w0);
+      if (p.b) PT::fetch(to + ob, row_at<T>(p.b, coming, p.bs), w0);
+      if (full) PT::fetch(to + og, row_at<T>(p.gate, coming, p.gs), w0);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    coming += step;
+    to = to + hold.slot == end ? all : to + hold.slot;
+  };
+  if constexpr (VEC)  // columns that there are not read as 0
+    for (unsigned j = all + threadIdx.x * 16; j < end; j += blockDim.x * 16) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(j), "r"(0) : "memory");
+  __syncthreads();
+  for (int a = 0; a + 1 < ahead; ++a) fetch();
+  unsigned here = all;
+  for (unsigned r = first; r < rows; r += step) {
+    turn_ring<VEC>(g, ahead, fetch);
     // the row's parts, by piece
-    auto get_x = [&](float* v, const void* m, i64 stride, unsigned at, int k) {
-      if constexpr (VEC)
-        PX::get(v, here + k * piece + at);
-      else
-        load8<TX>(v, static_cast<const TX*>(m) + r * stride, w0.piece(k));
-    };
-    auto get_t = [&](float* v, const void* m, i64 stride, unsigned at, int k) {
-      if constexpr (VEC)
-        PT::get(v, here + k * piece + at);
-      else
-        load8<T>(v, static_cast<const T*>(m) + r * stride, w0.piece(k));
-    };
+    auto get_y = [&](float* v, int k) { PX::get(v, here + oy, row_at<TX>(p.y, r, p.ys), w0, k); };
+    auto get_dy = [&](float* v, int k) { PX::get(v, here + ody, row_at<TX>(p.dy, r, p.dys), w0, k); };
+    auto get_dh = [&](float* v, int k) { PT::get(v, here + odh, row_at<T>(p.dh, r, p.dhs), w0, k); };
+    auto get_b = [&](float* v, int k) { PT::get(v, here + ob, row_at<T>(p.b, r, p.bs), w0, k); };
     float m1 = 0.0f, f1 = 0.0f, m2 = 0.0f;
     if (kind == 1) {
       float t[3] = {0.0f, 0.0f, 0.0f};
@@ -571,16 +742,16 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
       for (int k = 0; k < PIECES; ++k) {
         float a[kE], b[kE];
         if (p.dh) {
-          get_x(a, p.y, p.ys, kY, k);
+          get_y(a, k);
 #pragma unroll
           for (int i = 0; i < kE; ++i) t[0] += a[i];
-          get_t(a, p.dh, p.dhs, kDh, k);
-          vec8(b, p.w1, p.wdt, 1.0f, w0.piece(k));
+          get_dh(a, k);
+          kept.get(k * slots, b);
 #pragma unroll
           for (int i = 0; i < kE; ++i) t[1] += a[i] * b[i];
         }
         if (norm2) {
-          get_t(a, p.b, p.bs, kB, k);
+          get_b(a, k);
 #pragma unroll
           for (int i = 0; i < kE; ++i) t[2] += a[i];
         }
@@ -596,22 +767,23 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
       const Place<VEC> w = w0.piece(k);
       float a[kE], b[kE], c[kE];
       if (p.dh) {
-        get_x(a, p.y, p.ys, kY, k);
-        get_t(b, p.dh, p.dhs, kDh, k);
-        vec8(c, p.w1, p.wdt, 1.0f, w);
+        get_y(a, k);
+        get_dh(b, k);
+        kept.get(k * slots, c);
 #pragma unroll
         for (int i = 0; i < kE; ++i) {
-          if (!w.on(i)) continue;
-          a[i] -= m1;
+          if (kind == 1) a[i] = w.on(i) ? a[i] - m1 : 0.0f;
           q[0] += a[i] * a[i];
           q[1] += b[i] * c[i] * a[i];
         }
       }
       if (norm2) {
-        get_t(a, p.b, p.bs, kB, k);
+        get_b(a, k);
 #pragma unroll
-        for (int i = 0; i < kE; ++i)
-          if (w.on(i)) q[2] += (a[i] - m2) * (a[i] - m2);
+        for (int i = 0; i < kE; ++i) {
+          if (kind == 1) a[i] = w.on(i) ? a[i] - m2 : 0.0f;
+          q[2] += a[i] * a[i];
+        }
       }
     }
     g.sum<3>(q);
@@ -622,54 +794,78 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
       const Place<VEC> w = w0.piece(k);
       float d[kE], a[kE], b[kE], c[kE];
       if (p.dy)
-        get_x(d, p.dy, p.dys, kDy, k);
+        get_dy(d, k);
       else
 #pragma unroll
         for (int i = 0; i < kE; ++i) d[i] = 0.0f;
       if (p.dh) {
-        get_x(a, p.y, p.ys, kY, k);
-        get_t(b, p.dh, p.dhs, kDh, k);
-        vec8(c, p.w1, p.wdt, 1.0f, w);
+        get_y(a, k);
+        get_dh(b, k);
+        kept.get(k * slots, c);
+        if (kind == 1) {
+#pragma unroll
+          for (int i = 0; i < kE; ++i) a[i] = w.on(i) ? a[i] - m1 : 0.0f;
+        }
 #pragma unroll
         for (int i = 0; i < kE; ++i) {
-          const float hat = (a[i] - m1) * r1;
+          const float hat = a[i] * r1;
           d[i] += r1 * (b[i] * c[i] - hat * a1 - f1);
           acc[0][k * kE + i] += b[i] * hat;
           if (MORE) acc[2][k * kE + i] += b[i];
         }
       }
-#pragma unroll
-      for (int i = 0; i < kE; ++i)
-        if (!w.on(i)) d[i] = 0.0f;  // 0 - mean is not 0
-      if (p.dx) store8<TX>(static_cast<TX*>(p.dx) + r * p.dxs, d, w);
+      if (p.dx) store8<TX>(row_at<TX>(p.dx, r, p.dxs), d, w);
       if (!p.b) continue;
-      const unsigned keep = keep_bits<VEC>(p.d, p.d.base + (u64)(r * p.cols), w);
-      get_t(b, p.b, p.bs, kB, k);
-      vec8(c, p.w2, p.wdt, 1.0f, w);
+      if (p.d.on) {
+        unsigned u[kE];
+        words8<VEC>(u, p.d, p.d.base + (u64)r * (unsigned)p.cols, w, places + hold.words);
 #pragma unroll
-      for (int i = 0; i < kE; ++i) {
-        d[i] = (keep >> i) & 1u ? f * d[i] : 0.0f;  // dz
-        b[i] = (b[i] - m2) * r2;                    // hat
+        for (int i = 0; i < kE; ++i) d[i] = u[i] > p.d.last ? f * d[i] : 0.0f;  // dz
+      } else {
+#pragma unroll
+        for (int i = 0; i < kE; ++i) d[i] *= f;
       }
-      if (p.gate) {
-        if (full)
-          get_t(a, p.gate, p.gs, kG, k);
-        else
-          vec8(a, gate_row(p.gate, p.gdt, p.gs, r), p.gdt, 0.0f, w);
-        float u[kE];
-        vec8(u, p.c2, p.wdt, 0.0f, w);
+      get_b(b, k);
+      kept.get(k * slots + 1, c);
+      if (kind == 1) {  // 0 - mean is not 0
 #pragma unroll
         for (int i = 0; i < kE; ++i) {
-          const float v = fast_act(p.act, a[i]);
-          u[i] = d[i] * (b[i] * c[i] + u[i]) * slope_of(p.act, v);
+          b[i] -= m2;
+          if (!w.on(i)) b[i] = d[i] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kE; ++i) b[i] *= r2;  // hat
+      if (p.gate) {
+        if (channel) {
+          kept.get(k * slots + gate_at, a);
+        } else {
+          if (full)
+            PT::get(a, here + og, row_at<T>(p.gate, r, p.gs), w0, k);
+          else
+            vec8(a, gate_row(p.gate, p.gdt, p.gs, r), p.gdt, 0.0f, w);
+          act8(p.act, a);
+        }
+        float u[kE];
+        if (p.c2) {
+          kept.get(k * slots + 2, u);
+#pragma unroll
+          for (int i = 0; i < kE; ++i) u[i] = d[i] * (b[i] * c[i] + u[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kE; ++i) u[i] = d[i] * b[i] * c[i];
+        }
+        slope8(p.act, a, u);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) {
           if (MORE) acc[4][k * kE + i] += u[i];
-          d[i] *= v;  // du
+          d[i] *= a[i];  // du
         }
         if (p.dgate) {
           if (p.gdt == CCB_F32)
-            store8<float>(static_cast<float*>(p.dgate) + r * p.dgs, u, w);
+            store8<float>(row_at<float>(p.dgate, r, p.dgs), u, w);
           else
-            store8<T>(static_cast<T*>(p.dgate) + r * p.dgs, u, w);
+            store8<T>(row_at<T>(p.dgate, r, p.dgs), u, w);
         }
       }
 #pragma unroll
@@ -678,30 +874,35 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
         if (MORE) acc[3][k * kE + i] += d[i];
         g2[k][i] = d[i] * c[i];
         t[0] += g2[k][i] * b[i];
-        t[1] += g2[k][i];
+        if (kind == 1) t[1] += g2[k][i];
       }
     }
-    if (!p.db) continue;
-    float a2 = 0.0f, f2 = 0.0f;
-    if (p.post) {
-      g.sum<2>(t);
-      a2 = t[0] * inv;
-      f2 = kind == 1 ? t[1] * inv : 0.0f;
-    }
-#pragma unroll
-    for (int k = 0; k < PIECES; ++k) {
+    if (p.db) {
+      float a2 = 0.0f, f2 = 0.0f;
       if (p.post) {
-        float b[kE];
-        get_t(b, p.b, p.bs, kB, k);
-#pragma unroll
-        for (int i = 0; i < kE; ++i) g2[k][i] = r2 * (g2[k][i] - (b[i] - m2) * r2 * a2 - f2);
+        if (kind == 1)
+          g.sum<2>(t);
+        else
+          g.sum<1>(t);
+        a2 = t[0] * inv * r2 * r2;
+        f2 = kind == 1 ? t[1] * inv * r2 : 0.0f;
       }
-      store8<T>(static_cast<T*>(p.db) + r * p.dbs, g2[k], w0.piece(k));
+#pragma unroll
+      for (int k = 0; k < PIECES; ++k) {
+        if (p.post) {
+          float b[kE];
+          get_b(b, k);
+#pragma unroll
+          for (int i = 0; i < kE; ++i) g2[k][i] = r2 * g2[k][i] - (b[i] - m2) * a2 - f2;
+        }
+        store8<T>(row_at<T>(p.db, r, p.dbs), g2[k], w0.piece(k));
+      }
     }
+    here = here + hold.slot == end ? all : here + hold.slot;
   }
-  if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
+  asm volatile("cp.async.wait_all;" ::: "memory");
   // the block's partial sums: its groups', in order
-  float* all = reinterpret_cast<float*>(places);
+  float* turn = reinterpret_cast<float*>(places);
 #pragma unroll
   for (int a = 0; a < (MORE ? kVecs : 2); ++a) {
     const int v = a == 0 ? 0 : a == 1 ? 2 : a == 2 ? 1 : a;
@@ -709,12 +910,12 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
     if (sets > 1) {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < PIECES * kE; ++i) all[i * blockDim.x + threadIdx.x] = acc[a][i];
+      for (int i = 0; i < PIECES * kE; ++i) turn[i * blockDim.x + threadIdx.x] = acc[a][i];
       __syncthreads();
       if (g.id == 0)
 #pragma unroll
         for (int i = 0; i < PIECES * kE; ++i)
-          for (int o = 1; o < (int)sets; ++o) acc[a][i] += all[i * blockDim.x + o * tpr + threadIdx.x];
+          for (int o = 1; o < (int)sets; ++o) acc[a][i] += turn[i * blockDim.x + o * tpr + threadIdx.x];
     }
     float* part = p.part + ((i64)blockIdx.x * kVecs + v) * p.cols;
     if (g.id == 0)
@@ -769,25 +970,42 @@ void by_type(int dtype, int x_dtype, int kind, A... a) {
 #undef CCB_NN_CASE
 }
 
-// How rows are held: threads of a row (0: too long for that), of a block, and
-// rows of one group that are in hand or on their way.
+// How rows are held, the block's threads (0: rows are too long) and its shared
+// memory. `part(block, tpr)`: bytes of a slot of the ring; `vectors`: kept ones;
+// `least`: bytes a thread needs at the end, in the same place. As many groups
+// as 512 threads hold, fewer where their rows and the next ones do not fit.
 struct Shape {
-  int tpr, block, ahead, smem;
+  Hold hold;
+  int block, smem;
 };
-// `most`: threads of a block. `place`: bytes a thread needs for its part of a
-// row; `room`: of a block; `least`: what it needs besides.
-Shape shape_of(i64 cols, int elems, int most, bool vec, int place, int room, int least) {
-  const i64 tpr = (cols + elems * 32 - 1) / (elems * 32) * 32;
-  if (tpr > most) return {0, 0, 0, 0};
-  const int groups = tpr >= 512 ? 1 : (int)(512 / tpr);
-  Shape f = {(int)tpr, (int)tpr * groups, 1, 0};
-  if (vec) {
-    const int row = f.block * place;
-    f.ahead = room / row < 1 ? 1 : room / row > 4 ? 4 : room / row;
-    f.smem = f.ahead * row;
-  }
-  if (f.smem < f.block * least) f.smem = f.block * least;
+constexpr int kMostShared = 220 * 1024;
+template <class P>
+Shape shape_of(i64 cols, int pieces, bool vec, int vectors, int least, P part) {
+  Shape f = {};
+  const i64 tpr = (cols + pieces * kE * 32 - 1) / (pieces * kE * 32) * 32;
+  if (tpr > 512) return f;
+  f.hold.tpr = (int)tpr;
+  const int kept = (int)tpr * pieces * kE * 4 * vectors;
+  for (int want = 2; want >= 1 && !f.block; --want)
+    for (int groups = 512 / (int)tpr; groups >= 1 && !f.block; --groups) {
+      const int block = groups * (int)tpr, slot = (int)part(block, (int)tpr), words = vec ? 0 : block / 32 * kWarpWords * 4;
+      const int ahead = (kMostShared - kept - words) / slot;
+      if (ahead < want) continue;
+      f.block = block;
+      f.hold.ahead = ahead > 3 ? 3 : ahead;
+      f.hold.slot = (unsigned)slot;
+      f.hold.kept = (unsigned)(f.hold.ahead * slot);
+      f.hold.words = f.hold.kept + (unsigned)kept;
+      f.smem = (int)f.hold.words + words;
+      if (f.smem < block * least) f.smem = block * least;
+    }
   return f;
+}
+// Row strides that 32-bit products reach
+bool near(std::initializer_list<i64> strides) {
+  for (i64 t : strides)
+    if (t >= (1ll << 30)) return false;
+  return true;
 }
 // 16-byte accesses along every row
 bool wide(i64 cols, std::initializer_list<const void*> ptrs, std::initializer_list<i64> strides) {
@@ -804,25 +1022,36 @@ bool room_for(K* kernel, bool (&ready)[64]) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && __atomic_load_n(&ready[dev], __ATOMIC_RELAXED)) return true;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024) != cudaSuccess) return false;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) return false;
   if (dev >= 0 && dev < 64) __atomic_store_n(&ready[dev], true, __ATOMIC_RELAXED);
   return true;
 }
 
 template <class T, class TX, int KIND>
 struct Forward {
-  template <bool VEC>
+  template <bool VEC, int PIECES>
   static bool rows(const NormP& p, int sms, cudaStream_t st) {
     static bool ready[64];
-    const Shape f = shape_of(p.cols, kE, 1024, VEC, kE * (sizeof(TX) + 2 * sizeof(T)), 104 * 1024, 0);
-    if (!f.tpr || !room_for(norm_rows<T, TX, VEC>, ready)) return false;
-    const i64 sets = (p.rows + f.block / f.tpr - 1) / (f.block / f.tpr), most = (i64)sms * (f.block > 512 ? 1 : 2);
-    norm_rows<T, TX, VEC><<<(unsigned)(sets < most ? sets : most), f.block, f.smem, st>>>(p, KIND, f.tpr, f.ahead);
+    const int matrices = (p.b != nullptr) + (p.gate && p.gs != 0 && p.gdt != CCB_F32);
+    const Shape f = shape_of(p.cols, PIECES, VEC, 2 + (p.c1 != nullptr) + (p.c2 != nullptr) + (p.gate && p.gs == 0), 0, [&](int block, int tpr) {
+      return part_bytes<TX, VEC, PIECES>(p.cols, block, tpr) + matrices * part_bytes<T, VEC, PIECES>(p.cols, block, tpr);
+    });
+    if (!f.block || !room_for(norm_rows<T, TX, VEC, PIECES>, ready)) return false;
+    const i64 groups = f.block / f.hold.tpr, sets = (p.rows + groups - 1) / groups;
+    norm_rows<T, TX, VEC, PIECES><<<(unsigned)(sets < sms ? sets : sms), f.block, f.smem, st>>>(p, KIND, f.hold);
     return true;
   }
+  static bool by_width(const NormP& p, int sms, cudaStream_t st) {
+    if (!near({p.xs, p.bs, p.gs, p.ys, p.hs})) return false;
+    if (!wide(p.cols, {p.x, p.b, p.gate, p.y, p.h}, {p.xs, p.bs, p.gs, p.ys, p.hs})) return rows<false, 1>(p, sms, st);
+    // What a thread does once a row (its sums, addresses, copies) is some 300
+    // instructions: 32 elements share them, fewer where a warp holds the row.
+    // The shape goes by the columns alone: a row's result does not depend on
+    // the rows beside it.
+    return p.cols <= 256 ? rows<true, 1>(p, sms, st) : p.cols <= 512 ? rows<true, 2>(p, sms, st) : rows<true, 4>(p, sms, st);
+  }
   static void run(const NormP& p, int sms, cudaStream_t st) {
-    const bool v = wide(p.cols, {p.x, p.b, p.gate, p.w1, p.c1, p.w2, p.c2, p.y, p.h}, {p.xs, p.bs, p.gs, p.ys, p.hs});
-    if (v ? rows<true>(p, sms, st) : rows<false>(p, sms, st)) return;
+    if (by_width(p, sms, st)) return;
     const i64 most = (i64)sms * 8;
     norm_any<T, TX, KIND><<<(unsigned)(p.rows < most ? p.rows : most), kBlock, 0, st>>>(p);
   }
@@ -834,23 +1063,26 @@ struct Backward {
   template <bool VEC, int PIECES, bool MORE>
   static int rows(const BackP& p, int sms, cudaStream_t st) {
     static bool ready[64];
-    const Shape f = shape_of(p.cols, kE * PIECES, 512, VEC, PIECES * kE * (2 * sizeof(TX) + 3 * sizeof(T)), 216 * 1024, PIECES * kE * 4);
-    if (!f.tpr || !room_for(norm_back_rows<T, TX, VEC, PIECES, MORE>, ready)) return 0;
-    const i64 sets = (p.rows + f.block / f.tpr - 1) / (f.block / f.tpr);
+    const Shape f = shape_of(p.cols, PIECES, VEC, 2 + (p.c2 != nullptr) + (p.gate && p.gs == 0), PIECES * kE * 4, [&](int block, int tpr) {
+      return 2 * part_bytes<TX, VEC, PIECES>(p.cols, block, tpr) + 3 * part_bytes<T, VEC, PIECES>(p.cols, block, tpr);
+    });
+    if (!f.block || !room_for(norm_back_rows<T, TX, VEC, PIECES, MORE>, ready)) return 0;
+    const i64 groups = f.block / f.hold.tpr, sets = (p.rows + groups - 1) / groups;
     const int most = sms < kBackBlocks ? sms : (int)kBackBlocks, grid = (int)(sets < most ? sets : most);
-    norm_back_rows<T, TX, VEC, PIECES, MORE><<<grid, f.block, f.smem, st>>>(p, KIND, f.tpr, f.ahead);
+    norm_back_rows<T, TX, VEC, PIECES, MORE><<<grid, f.block, f.smem, st>>>(p, KIND, f.hold);
     return grid;
   }
   // Rows of 16 elements a thread, so that a block of 512 threads (128 registers
   // each) holds two of 4096 columns and one waits for its sums while the other
-  // computes; of 8 where two f32 rows and those on their way do not fit shared
-  // memory. The shape does not go by which sums over rows are asked for (all
-  // five spill some registers), so that the other results do not either.
+  // computes; of 8 where there are few columns. The shape does not go by the
+  // rows or by which sums over them are asked for (all five spill some
+  // registers), so that a row's results do not either.
   template <bool MORE>
   static int by_width(const BackP& p, int sms, cudaStream_t st) {
-    if (!wide(p.cols, {p.y, p.dy, p.dh, p.b, p.gate, p.w1, p.w2, p.c2, p.dx, p.db, p.dgate}, {p.ys, p.dys, p.dhs, p.bs, p.gs, p.dxs, p.dbs, p.dgs}))
+    if (!near({p.ys, p.dys, p.dhs, p.bs, p.gs, p.dxs, p.dbs, p.dgs})) return 0;
+    if (!wide(p.cols, {p.y, p.dy, p.dh, p.b, p.gate, p.dx, p.db, p.dgate}, {p.ys, p.dys, p.dhs, p.bs, p.gs, p.dxs, p.dbs, p.dgs}))
       return rows<false, 1, MORE>(p, sms, st);
-    if (p.cols <= 256 || (sizeof(TX) == 4 && p.cols <= 4096)) return rows<true, 1, MORE>(p, sms, st);
+    if (p.cols <= 256) return rows<true, 1, MORE>(p, sms, st);
     return rows<true, 2, MORE>(p, sms, st);
   }
   static void run(const BackP& p, int sms, cudaStream_t st) {
