@@ -114,17 +114,22 @@ __device__ __forceinline__ float load_as(const void* p, int dtype, i64 i) {
 // serves four elements. It is dropped when its word is below
 // round(p * 2^32). The ten round keys depend on the seed alone and are laid
 // out by the host, so a round is two 32x32 -> 64 products and two
-// three-operand XORs.
+// three-operand XORs. The products bound the generator (one of them takes the
+// multiplier for four cycles a warp): where all of a tensor's counters share
+// q's high word, the second product of round one and the first of round two
+// are constants, so the host computes them and 18 products are left of 20.
 struct Drop {
   unsigned key[20];
   u64 offset, base;
   unsigned last;   // words <= last are dropped
   float factor;    // 1 / (1 - p); 0 for p = 1
   int on;          // 0: no element is dropped
+  int same;        // one high word for all: round two's constants hold
+  unsigned c2, c0, hi, c3;
 };
 
-// p is in [0, 1].
-inline Drop make_drop(double p, u64 seed, u64 offset, u64 base) {
+// p is in [0, 1]; n elements from `base` on.
+inline Drop make_drop(double p, u64 seed, u64 offset, u64 base, u64 n) {
   Drop d = {};
   unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
   for (int i = 0; i < 10; ++i) {
@@ -139,23 +144,67 @@ inline Drop make_drop(double p, u64 seed, u64 offset, u64 base) {
   d.on = t >= 1.0;
   d.last = d.on ? (unsigned)(u64)(t - 1.0) : 0u;
   d.factor = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f;
+  // the last block that a vector of 8 touches lies up to 11 elements on
+  const u64 end = base + n + 11 < base ? ~0ull : base + n + 11;
+  d.same = (base >> 34) == (end >> 34);
+  const u64 b = (u64)0xCD9E8D57u * (unsigned)offset;
+  const unsigned r1c0 = (unsigned)(b >> 32) ^ (unsigned)(base >> 34) ^ d.key[0];
+  const u64 a = (u64)0xD2511F53u * r1c0;
+  d.c2 = (unsigned)(offset >> 32) ^ d.key[1];
+  d.c0 = (unsigned)b ^ d.key[2];
+  d.hi = (unsigned)(a >> 32) ^ d.key[3];
+  d.c3 = (unsigned)a;
   return d;
 }
 
-__device__ __forceinline__ void philox4(const Drop& d, u64 q, unsigned w[4]) {
-  unsigned c0 = (unsigned)q, c1 = (unsigned)(q >> 32), c2 = (unsigned)d.offset, c3 = (unsigned)(d.offset >> 32);
-#pragma unroll
-  for (int i = 0; i < 10; ++i) {
-    const u64 a = (u64)0xD2511F53u * c0, b = (u64)0xCD9E8D57u * c2;
-    c0 = (unsigned)(b >> 32) ^ c1 ^ d.key[2 * i];
+__device__ __forceinline__ void philox_round(const Drop& d, int i, unsigned& c0, unsigned& c1, unsigned& c2, unsigned& c3) {
+  const u64 a = (u64)0xD2511F53u * c0, b = (u64)0xCD9E8D57u * c2;
+  c0 = (unsigned)(b >> 32) ^ c1 ^ d.key[2 * i];
+  c1 = (unsigned)b;
+  c2 = (unsigned)(a >> 32) ^ c3 ^ d.key[2 * i + 1];
+  c3 = (unsigned)a;
+}
+__device__ __forceinline__ void philox4(const Drop& d, u64 q, unsigned* w) {
+  unsigned c0, c1, c2, c3;
+  if (d.same) {
+    const u64 a = (u64)0xD2511F53u * (unsigned)q;
+    const u64 b = (u64)0xCD9E8D57u * ((unsigned)(a >> 32) ^ d.c2);
+    c0 = (unsigned)(b >> 32) ^ d.c0;
     c1 = (unsigned)b;
-    c2 = (unsigned)(a >> 32) ^ c3 ^ d.key[2 * i + 1];
-    c3 = (unsigned)a;
+    c2 = (unsigned)a ^ d.hi;
+    c3 = d.c3;
+  } else {
+    c0 = (unsigned)q;
+    c1 = (unsigned)(q >> 32);
+    c2 = (unsigned)d.offset;
+    c3 = (unsigned)(d.offset >> 32);
+    philox_round(d, 0, c0, c1, c2, c3);
+    philox_round(d, 1, c0, c1, c2, c3);
   }
+#pragma unroll
+  for (int i = 2; i < 10; ++i) philox_round(d, i, c0, c1, c2, c3);
   w[0] = c0;
   w[1] = c1;
   w[2] = c2;
   w[3] = c3;
+}
+// The words of the 8 elements from e0 on: two blocks, or three where the index
+// is no multiple of 4.
+__device__ __forceinline__ void philox8(const Drop& d, u64 e0, unsigned* w) {
+  const u64 q = e0 >> 2;
+  philox4(d, q, w);
+  philox4(d, q + 1, w + 4);
+  const int shift = (int)(e0 & 3);
+  if (shift) {
+    unsigned x[4];
+    philox4(d, q + 2, x);
+    for (int k = 0; k < shift; ++k) {
+#pragma unroll
+      for (int i = 0; i < 7; ++i) w[i] = w[i + 1];
+      w[7] = x[0];
+      x[0] = x[1], x[1] = x[2], x[2] = x[3];
+    }
+  }
 }
 // v / (1 - p), or 0 (whatever v holds) where the word says so.
 __device__ __forceinline__ float dropped(const Drop& d, unsigned word, float v) { return word > d.last ? v * d.factor : 0.0f; }

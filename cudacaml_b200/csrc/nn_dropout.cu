@@ -16,6 +16,20 @@ struct DropoutP {
   Drop d;
 };
 
+// Element i of 8, in one 16-byte word or two.
+template <class T>
+__device__ __forceinline__ float element(const uint4* u, int i) {
+  const uint4 q = u[sizeof(T) == 4 ? i >> 2 : 0];
+  const int j = sizeof(T) == 4 ? i & 3 : i >> 1;
+  const unsigned w = j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w;
+  if constexpr (sizeof(T) == 4)
+    return __uint_as_float(w);
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16);
+  else
+    return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w >> 16 : w)));
+}
+
 // Any alignment, stride and base: a thread takes one block of the generator,
 // the up to four elements of the tensor that lie in it.
 template <class T>
@@ -43,9 +57,67 @@ __global__ void __launch_bounds__(256) dropout_any(const __grid_constant__ Dropo
   }
 }
 
+// 8 consecutive elements of a row by 16-byte accesses: pointers and strides of
+// 16 bytes, and rows of whole pieces of 8 (dense rows are one long row, whose
+// last elements the first threads take).
+template <class T>
+__global__ void __launch_bounds__(256) dropout_wide(const __grid_constant__ DropoutP p, unsigned pieces, u64 total) {
+  const u64 step = (u64)gridDim.x * blockDim.x, first = (u64)blockIdx.x * blockDim.x + threadIdx.x;
+  for (u64 v = first; v < total; v += step) {
+    u64 r = 0, c = v;
+    if (p.rows > 1) {  // total is below 2^32
+      r = (unsigned)v / pieces;
+      c = (unsigned)v - (unsigned)r * pieces;
+    }
+    c *= 8;
+    const T* x = static_cast<const T*>(p.x) + r * p.xs + c;
+    const T* res = static_cast<const T*>(p.res) + r * p.rs + c;
+    T* out = static_cast<T*>(p.out) + r * p.os + c;
+    constexpr int kWords = 2 * sizeof(T);
+    uint4 a[kWords / 4], b[kWords / 4] = {};
+#pragma unroll
+    for (int i = 0; i < kWords / 4; ++i) a[i] = reinterpret_cast<const uint4*>(x)[i];
+    if (p.res)
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) b[i] = reinterpret_cast<const uint4*>(res)[i];
+    unsigned w[8];
+    if (p.d.on) philox8(p.d, p.d.base + r * (u64)p.cols + c, w);
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[i] = element<T>(a, i) * p.d.factor;
+      if (p.d.on && w[i] <= p.d.last) y[i] = 0.0f;
+      if (p.res) y[i] += element<T>(b, i);
+    }
+#pragma unroll
+    for (int i = 0; i < kWords / 4; ++i) {
+      uint4 o;
+      if constexpr (sizeof(T) == 4)
+        o = make_uint4(__float_as_uint(y[4 * i]), __float_as_uint(y[4 * i + 1]), __float_as_uint(y[4 * i + 2]), __float_as_uint(y[4 * i + 3]));
+      else
+        o = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
+      reinterpret_cast<uint4*>(out)[i] = o;
+    }
+  }
+  if (p.rows == 1) {
+    const u64 e = (u64)p.cols / 8 * 8 + first;
+    if (e < (u64)p.cols) {
+      float y = dropped_at(p.d, p.d.base + e, to_f<T>(static_cast<const T*>(p.x)[e]));
+      if (p.res) y += to_f<T>(static_cast<const T*>(p.res)[e]);
+      static_cast<T*>(p.out)[e] = from_f<T>(y);
+    }
+  }
+}
+
 template <class T>
 void go(const DropoutP& p, int sms, cudaStream_t st) {
   const u64 n = (u64)p.rows * (u64)p.cols;
+  const bool lines = p.rows == 1 || (p.cols % 8 == 0 && p.xs % 8 == 0 && p.os % 8 == 0 && (!p.res || p.rs % 8 == 0) && n / 8 < (1ull << 32));
+  if (lines && aligned(p.x, 16) && aligned(p.out, 16) && aligned(p.res, 16)) {
+    const u64 total = n / 8, want = total / 256 + 1, most = (u64)sms * 16;
+    dropout_wide<T><<<(unsigned)(want < most ? want : most), 256, 0, st>>>(p, (unsigned)(p.cols / 8), total);
+    return;
+  }
   const u64 blocks = n / 4 + 2;
   const u64 want = (blocks + 255) / 256, most = (u64)sms * 32;
   dropout_any<T><<<(unsigned)(want < most ? want : most), 256, 0, st>>>(p);
@@ -77,7 +149,7 @@ extern "C" int ccb_nn_dropout(const ccb_nn_dropout_t* a, void* stream) {
     int sms = 0;
     if (const int rc = sm_count(me, &sms)) return rc;
     DropoutP p = {a->x, a->residual, a->out, a->rows, a->cols, a->x_stride, a->residual_stride, a->out_stride,
-                  make_drop(a->p, a->seed, a->offset, a->base)};
+                  make_drop(a->p, a->seed, a->offset, a->base, (u64)n)};
     // dense rows are one long row
     if (p.rows > 1 && p.xs == p.cols && p.os == p.cols && (!p.res || p.rs == p.cols)) {
       p.cols = n;

@@ -382,21 +382,7 @@ constexpr int kWarpWords = 9 * kE * 4;
 template <bool VEC>
 __device__ __forceinline__ void words8(unsigned* u, const Drop& d, u64 e0, const Place<VEC>& w, unsigned char* places) {
   if constexpr (VEC) {
-    e0 += (u64)w.at(0);
-    const u64 q = e0 >> 2;
-    philox4(d, q, u);
-    philox4(d, q + 1, u + 4);
-    const int shift = (int)(e0 & 3);
-    if (shift) {
-      unsigned x[4];
-      philox4(d, q + 2, x);
-      for (int k = 0; k < shift; ++k) {
-#pragma unroll
-        for (int i = 0; i < kE - 1; ++i) u[i] = u[i + 1];
-        u[kE - 1] = x[0];
-        x[0] = x[1], x[1] = x[2], x[2] = x[3];
-      }
-    }
+    philox8(d, e0 + (u64)w.at(0), u);
   } else {
     uint4* out = reinterpret_cast<uint4*>(places) + (threadIdx.x >> 5) * (kWarpWords / 4);
     const int lane = threadIdx.x & 31;
@@ -978,7 +964,7 @@ struct Shape {
   Hold hold;
   int block, smem;
 };
-constexpr int kMostShared = 220 * 1024;
+constexpr int kMostShared = 226 * 1024;
 template <class P>
 Shape shape_of(i64 cols, int pieces, bool vec, int vectors, int least, P part) {
   Shape f = {};
@@ -1048,7 +1034,7 @@ struct Forward {
     // instructions: 32 elements share them, fewer where a warp holds the row.
     // The shape goes by the columns alone: a row's result does not depend on
     // the rows beside it.
-    return p.cols <= 256 ? rows<true, 1>(p, sms, st) : p.cols <= 512 ? rows<true, 2>(p, sms, st) : rows<true, 4>(p, sms, st);
+    return p.cols <= 256 ? rows<true, 1>(p, sms, st) : p.cols <= 512 || (p.cols > 2048 && p.cols <= 4096) || sizeof(TX) == 4 ? rows<true, 2>(p, sms, st) : rows<true, 4>(p, sms, st);
   }
   static void run(const NormP& p, int sms, cudaStream_t st) {
     if (by_width(p, sms, st)) return;
@@ -1082,7 +1068,7 @@ struct Backward {
     if (!near({p.ys, p.dys, p.dhs, p.bs, p.gs, p.dxs, p.dbs, p.dgs})) return 0;
     if (!wide(p.cols, {p.y, p.dy, p.dh, p.b, p.gate, p.dx, p.db, p.dgate}, {p.ys, p.dys, p.dhs, p.bs, p.gs, p.dxs, p.dbs, p.dgs}))
       return rows<false, 1, MORE>(p, sms, st);
-    if (p.cols <= 256) return rows<true, 1, MORE>(p, sms, st);
+    if (p.cols <= 256 || (sizeof(TX) == 4 && p.cols <= 4096)) return rows<true, 1, MORE>(p, sms, st);
     return rows<true, 2, MORE>(p, sms, st);
   }
   static void run(const BackP& p, int sms, cudaStream_t st) {
@@ -1159,7 +1145,7 @@ extern "C" int ccb_nn_block_norm(const ccb_nn_block_norm_t* a, void* stream) {
     if (const int rc = sm_count(me, &sms)) return rc;
     const NormP p = {a->x, a->branch, a->gate, a->pre_weight, a->pre_bias, a->post_weight, a->post_bias, a->y, a->h, a->rows, a->cols,
                      a->x_stride, a->branch_stride, a->gate_stride, a->y_stride, a->h_stride, (float)a->eps, (float)a->scale, a->gate_dtype,
-                     a->weight_dtype, a->act, a->post_norm, make_drop(a->p, a->seed, a->offset, a->base)};
+                     a->weight_dtype, a->act, a->post_norm, make_drop(a->p, a->seed, a->offset, a->base, (u64)a->rows * (u64)a->cols)};
     by_type<Forward>(a->dtype, a->x_dtype, a->kind, p, sms, static_cast<cudaStream_t>(stream));
     return launched(me);
   })
@@ -1222,7 +1208,7 @@ extern "C" int ccb_nn_block_norm_backward(const ccb_nn_block_norm_backward_t* a,
                      {(float*)a->dpre_weight, (float*)a->dpre_bias, (float*)a->dpost_weight, (float*)a->dpost_bias, channel ? (float*)a->dgate : nullptr},
                      (float*)a->workspace, a->rows, a->cols, a->y_stride, a->dy_stride, a->dh_stride, a->branch_stride, a->gate_stride, a->dx_stride,
                      a->dbranch_stride, a->dgate_stride, (float)a->eps, (float)a->scale, a->gate_dtype, a->weight_dtype, a->act, a->post_norm,
-                     make_drop(a->p, a->seed, a->offset, a->base)};
+                     make_drop(a->p, a->seed, a->offset, a->base, (u64)a->rows * (u64)a->cols)};
     by_type<Backward>(a->dtype, a->x_dtype, a->kind, p, sms, st);
     return launched(me);
   })
