@@ -248,6 +248,7 @@ struct P {
   i64 os, oe;           // strides of out: a row, an expert's matrix (dw)
   i64 split_stride;     // elements from one part's result to the next
   int rows, experts, n, k, splits, format;
+  int terms;            // products of planes that make up one of the operands: 1, or 6 for f32
   int a2, b2;           // whether one copy takes two 64-wide blocks of an MN-major operand
   int box;              // rows of a copy of tokens
   int vec;              // out takes 16-byte stores
@@ -425,9 +426,28 @@ struct Tile {
   int r0, r1;      // rows: of the result (forward), of the contraction (dw)
   int f0, c0;      // first feature; first column of x (dw)
   int nn;          // N of the MMA
-  int b0, b1;      // steps of the contraction
+  int kt;          // steps of the contraction of one term
+  int b0, b1;      // steps of all terms
   int split;
 };
+// Step b of a tile: `kb`-th of the contraction in term `term`.
+struct Step {
+  int kb, term;
+  __device__ __forceinline__ explicit Step(const Tile& o) : kb(o.kt ? o.b0 % o.kt : 0), term(o.kt ? o.b0 / o.kt : 0) {}
+  __device__ __forceinline__ void next(const Tile& o) {
+    if (++kb == o.kt) {
+      kb = 0;
+      ++term;
+    }
+  }
+};
+// The planes of a term: f32 operands are sums hi + mid + lo of three 16-bit
+// planes, and the six products down to 2^-16 of the largest are added up from
+// the smallest, so that the accumulator's rounding is that of the last term's
+// steps.
+__device__ __forceinline__ int plane_m(int terms, int term) { return terms == 1 ? 0 : (0x001102 >> (4 * term)) & 15; }
+__device__ __forceinline__ int plane_n(int terms, int term) { return terms == 1 ? 0 : (0x010120 >> (4 * term)) & 15; }
+
 enum { kForward = 0, kForwardT = 1, kDw = 2 };
 
 template <int MODE>
@@ -446,7 +466,6 @@ __device__ __forceinline__ Tile tile_at(const P& p, const Segments& g, unsigned 
   t /= nf;
   o.split = (int)(t % (unsigned)p.splits);
   t /= (unsigned)p.splits;
-  int steps;
   if (MODE == kDw) {
     const unsigned nc = (p.k + kTok - 1) / kTok;
     o.c0 = (int)(t % nc) * kTok;
@@ -454,7 +473,7 @@ __device__ __forceinline__ Tile tile_at(const P& p, const Segments& g, unsigned 
     o.r0 = g.row[o.expert + 1];
     o.r1 = g.row[o.expert + 2];
     o.nn = p.k - o.c0 > kTok / 2 ? kTok : kTok / 2;
-    steps = (o.r1 - o.r0 + kBK - 1) / kBK;
+    o.kt = (o.r1 - o.r0 + kBK - 1) / kBK;
   } else {
     const int s = segment_of(g, p.experts + 2, (int)t);
     const int first = g.row[s], rows = g.row[s + 1] - first, parts = g.tile[s + 1] - g.tile[s], i = (int)t - g.tile[s];
@@ -464,16 +483,17 @@ __device__ __forceinline__ Tile tile_at(const P& p, const Segments& g, unsigned 
     o.r1 = first + min((i + 1) * each, rows);
     o.c0 = 0;
     o.nn = max((o.r1 - o.r0 + 31) & ~31, 32);
-    steps = o.expert < 0 ? 0 : (p.k + kBK - 1) / kBK;
+    o.kt = o.expert < 0 ? 0 : (p.k + kBK - 1) / kBK;
   }
-  o.b0 = steps * o.split / p.splits;
-  o.b1 = steps * (o.split + 1) / p.splits;
+  const int steps = o.kt * p.terms;
+  o.b0 = (int)((i64)steps * o.split / p.splits);
+  o.b1 = (int)((i64)steps * (o.split + 1) / p.splits);
   return o;
 }
-// The last step of a dw tile that reaches past its expert's rows.
+// Whether a step of a dw tile reaches past its expert's rows.
 template <int MODE>
-__device__ __forceinline__ bool clears(const Tile& o, int b) {
-  return MODE == kDw && o.r1 - o.r0 - b * kBK < kBK;
+__device__ __forceinline__ bool clears(const Tile& o, const Step& at) {
+  return MODE == kDw && o.r1 - o.r0 - at.kb * kBK < kBK;
 }
 
 template <class TO, int MODE>
@@ -522,11 +542,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
       const int half = o.nn >> 1, f = o.f0 + (int)rank * 128, c = o.c0 + (int)rank * half, tok = o.r0 + (int)rank * half;
       const int boxes = MODE == kDw ? (p.b2 ? 1 : half / 64) : (half + p.box - 1) / p.box;
       const unsigned box = MODE == kDw ? (p.b2 ? 16384u : 8192u) : (unsigned)p.box * 128u, bytes = kABytes + boxes * box;
-      for (int b = o.b0; b < o.b1; ++b) {
+      Step in(o);
+      for (int b = o.b0; b < o.b1; ++b, in.next(o)) {
         wait(empty + st, phase);
         if (one) {
           unsigned bar = lead_full + st;
-          if (clears<MODE>(o, b)) {
+          const int pm = plane_m(p.terms, in.term), pn = plane_n(p.terms, in.term);
+          if (clears<MODE>(o, in)) {
             bar = part + st;
             expect(bar, bytes);
           } else if (rank == 0) {
@@ -534,35 +556,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
           } else {
             arrive_relaxed(bar);
           }
-          const int k0 = b * kBK;
+          const int k0 = in.kb * kBK;
           unsigned sb = at + kABytes;
           if (MODE == kDw) {
             const int r = o.r0 + k0;
             if (p.a2) {
-              load4(at, &p.ta, 0, r, f >> 6, 0, bar);
+              load4(at, &p.ta, 0, r, f >> 6, pm, bar);
             } else {
-              load4(at, &p.ta, f, r, 0, 0, bar);
-              load4(at + 8192u, &p.ta, f + 64, r, 0, 0, bar);
+              load4(at, &p.ta, f, r, pm, 0, bar);
+              load4(at + 8192u, &p.ta, f + 64, r, pm, 0, bar);
             }
             if (p.b2) {
-              load4(sb, &p.tb, 0, r, c >> 6, 0, bar);
+              load4(sb, &p.tb, 0, r, c >> 6, pn, bar);
             } else {
-              load4(sb, &p.tb, c, r, 0, 0, bar);
-              if (boxes > 1) load4(sb + 8192u, &p.tb, c + 64, r, 0, 0, bar);
+              load4(sb, &p.tb, c, r, pn, 0, bar);
+              if (boxes > 1) load4(sb + 8192u, &p.tb, c + 64, r, pn, 0, bar);
             }
           } else {
+            const int e = pm * p.experts + o.expert;
             if (MODE == kForwardT) {
-              load4(at, &p.ta, k0, f, o.expert, 0, bar);
+              load4(at, &p.ta, k0, f, e, 0, bar);
             } else if (p.a2) {
-              load4(at, &p.ta, 0, k0, f >> 6, o.expert, bar);
+              load4(at, &p.ta, 0, k0, f >> 6, e, bar);
             } else {
-              load4(at, &p.ta, f, k0, o.expert, 0, bar);
-              load4(at + 8192u, &p.ta, f + 64, k0, o.expert, 0, bar);
+              load4(at, &p.ta, f, k0, e, 0, bar);
+              load4(at + 8192u, &p.ta, f + 64, k0, e, 0, bar);
             }
-            load4(sb, &p.tb, k0, tok, 0, 0, bar);
+            load4(sb, &p.tb, k0, tok, pn, 0, bar);
             for (int i = 1; i < boxes; ++i) {
               sb += box;
-              load4(sb, &p.tb, k0, tok + i * p.box, 0, 0, bar);
+              load4(sb, &p.tb, k0, tok + i * p.box, pn, 0, bar);
             }
           }
         }
@@ -592,12 +615,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
         const unsigned idesc = base | ((unsigned)(o.nn >> 3) << 17);
         wait(acce + 8 * ab, ((it >> 1) & 1u) ^ 1u);
         tc::fence_after();
-        for (int b = o.b0; b < o.b1; ++b) {
+        Step in(o);
+        for (int b = o.b0; b < o.b1; ++b, in.next(o)) {
           wait(full + st, phase);
           tc::fence_after();
           if (one) {
-            if (clears<MODE>(o, b)) {
-              const int kks = (o.r1 - o.r0 - b * kBK + 15) / 16;
+            if (clears<MODE>(o, in)) {
+              const int kks = (o.r1 - o.r0 - in.kb * kBK + 15) / 16;
               for (int kk = 0; kk < kks; ++kk) mma(d, a + kk * desc_step<amn>(), bd + kk * desc_step<bmn>(), idesc, b > o.b0 || kk > 0 ? 1u : 0u);
             } else {
 #pragma unroll
@@ -656,12 +680,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
     unsigned stage = 0, phases = 0;  // bit i: parity of part[i]
     for (unsigned t = pair; t < tiles; t += pairs) {
       const Tile o = tile_at<MODE>(p, s.g, t);
-      for (int b = o.b0; b < o.b1; ++b) {
-        if (clears<MODE>(o, b)) {
+      Step in(o);
+      for (int b = o.b0; b < o.b1; ++b, in.next(o)) {
+        if (clears<MODE>(o, in)) {
           wait(part + 8 * stage, (phases >> stage) & 1u);
           __syncwarp();
           phases ^= 1u << stage;
-          const int left = o.r1 - o.r0 - b * kBK, to = (left + 15) & ~15;
+          const int left = o.r1 - o.r0 - in.kb * kBK, to = (left + 15) & ~15;
           uint4* at = reinterpret_cast<uint4*>(smem + pad + stage * kStageBytes + (lane >> 3) * 8192 + (lane & 7) * 16);
           for (int r = left; r < to; ++r) at[r * 8] = make_uint4(0, 0, 0, 0);
           asm volatile("fence.proxy.async;" ::: "memory");
@@ -768,17 +793,80 @@ std::string check_dw(const ccb_nn_grouped_matmul_dw_t* a) {
   return bad;
 }
 
-// Whether a matrix can be read by the copy engine: 16-byte aligned, rows too.
-bool tma_ok(const void* p, i64 rows, i64 stride) { return aligned(p, 16) && (rows <= 1 || (stride % 8 == 0 && stride < (1ll << 38))); }
 
-// The tensor cores take 16-bit operands that the copy engine can read.
-bool on_tensor_cores(const ccb_nn_grouped_matmul_t* a) {
-  const i64 wr = a->transpose_w ? a->n : a->k;
-  return a->dtype != CCB_F32 && a->k > 0 && tma_ok(a->x, a->rows, a->x_stride) && tma_ok(a->w, wr, a->w_row_stride) &&
-         tma_ok(a->w, a->experts, a->w_stride);
+// ---------------------------------------------------------------- packing
+// Operands that the tensor cores cannot take as they lie: f32, cut into three
+// bf16 planes by truncation (8 significant bits each, so that hi + mid + lo is
+// the number itself and no plane rounds up past the largest), and 16-bit ones
+// whose rows are not aligned, copied. Rows of a plane are dense but for the
+// last 16 bytes. A number that is not finite is its first plane alone.
+template <class T>
+__global__ void __launch_bounds__(256) pack_planes(const T* in, i64 stride, i64 row_stride, unsigned short* out, i64 mats, i64 rows, unsigned cols, unsigned ld) {
+  const unsigned pieces = ld / 8;
+  const i64 total = mats * rows * pieces, plane = mats * rows * ld;
+  for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < total; i += (i64)gridDim.x * 256) {
+    const i64 row = i / pieces, m = row / rows;
+    const unsigned c = (unsigned)(i - row * pieces) * 8;
+    const T* p = in + m * stride + (row - m * rows) * row_stride + c;
+    unsigned short* o = out + row * ld + c;
+    if constexpr (sizeof(T) == 4) {
+      unsigned short v[3][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = c + j < cols ? (float)p[j] : 0.0f;
+        const float hi = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+        const bool fine = (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u;
+        const float r = fine ? x - hi : 0.0f, mid = __uint_as_float(__float_as_uint(r) & 0xFFFF0000u), lo = r - mid;
+        // a NaN keeps a bit of its fraction
+        v[0][j] = (unsigned short)((__float_as_uint(x) >> 16) | (x != x ? 0x40u : 0u));
+        v[1][j] = (unsigned short)(__float_as_uint(mid) >> 16);
+        v[2][j] = (unsigned short)(__float_as_uint(lo) >> 16);
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(o + k * plane) = *reinterpret_cast<const uint4*>(v[k]);
+    } else {
+      unsigned short v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? reinterpret_cast<const unsigned short*>(p)[j] : (unsigned short)0;
+      *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(v);
+    }
+  }
 }
-bool on_tensor_cores(const ccb_nn_grouped_matmul_dw_t* a) {
-  return a->dtype != CCB_F32 && a->rows > 0 && tma_ok(a->x, a->rows, a->x_stride) && tma_ok(a->dy, a->rows, a->dy_stride);
+
+// A stack of matrices as the copy engine reads it: in place, or packed.
+struct Operand {
+  const void* p;
+  i64 mats, rows, cols, stride, row_stride;  // elements
+  int planes;
+  bool packs;
+  i64 ld() const { return packs ? (cols + 7) / 8 * 8 : row_stride; }
+  size_t bytes() const { return packs ? ((size_t)planes * mats * rows * ld() * 2 + 255) / 256 * 256 : 0; }
+};
+i64 ceil_div(i64 a, i64 b) { return (a + b - 1) / b; }
+// 16-byte aligned rows of 16-bit elements
+bool lies_well(const void* p, i64 mats, i64 rows, i64 stride, i64 row_stride) {
+  return aligned(p, 16) && (rows <= 1 || (row_stride % 8 == 0 && row_stride < (1ll << 38))) && (mats <= 1 || (stride % 8 == 0 && stride < (1ll << 38)));
+}
+Operand operand(int dtype, const void* p, i64 mats, i64 rows, i64 cols, i64 stride, i64 row_stride) {
+  Operand o = {p, mats, rows, cols, stride, row_stride, dtype == CCB_F32 ? 3 : 1, false};
+  o.packs = dtype == CCB_F32 || !lies_well(p, mats, rows, stride, row_stride);
+  return o;
+}
+// Packs the operand into `room` if it has to be (and moves `room` on).
+int settle(Operand* o, int dtype, char** room, int sms, cudaStream_t st, const char* me) {
+  if (!o->packs) return CCB_OK;
+  const i64 ld = o->ld(), work = ceil_div(o->mats * o->rows * (ld / 8), 256), most = (i64)sms * 16;
+  const unsigned grid = (unsigned)(work < most ? work : most);
+  unsigned short* out = reinterpret_cast<unsigned short*>(*room);
+  if (dtype == CCB_F32)
+    pack_planes<float><<<grid, 256, 0, st>>>(static_cast<const float*>(o->p), o->stride, o->row_stride, out, o->mats, o->rows, (unsigned)o->cols, (unsigned)ld);
+  else
+    pack_planes<__half><<<grid, 256, 0, st>>>(static_cast<const __half*>(o->p), o->stride, o->row_stride, out, o->mats, o->rows, (unsigned)o->cols, (unsigned)ld);
+  *room += o->bytes();
+  o->p = out;
+  o->row_stride = ld;
+  o->stride = o->rows * ld;
+  return launched(me);
 }
 
 // In how many parts a contraction of `steps` is cut where there are too few
@@ -800,27 +888,41 @@ int parts_of(i64 tiles, i64 steps, i64 result) {
   }
   return best;
 }
-i64 ceil_div(i64 a, i64 b) { return (a + b - 1) / b; }
-int parts_of(const ccb_nn_grouped_matmul_t* a) {
-  if (!on_tensor_cores(a) || a->rows == 0 || a->n == 0) return 1;
-  const i64 tiles = ceil_div(a->n, tcg::kFeat) * ((a->experts < a->rows ? a->experts : a->rows) + a->rows / tcg::kTok);
-  return parts_of(tiles, ceil_div(a->k, tcg::kBK), a->rows * a->n);
+
+// What a call does, by its sizes, types, strides and alignment alone.
+struct Plan {
+  bool tensor;     // on the tensor cores
+  Operand w, x;    // M side, N side
+  int parts;       // of the contraction
+  i64 result;      // elements of one part's
+  size_t bytes() const { return tensor ? w.bytes() + x.bytes() + (parts > 1 ? (size_t)parts * result * sizeof(float) : 0) : 0; }
+};
+Plan plan_of(const ccb_nn_grouped_matmul_t* a) {
+  Plan p = {};
+  if (a->rows == 0 || a->n == 0 || a->k == 0) return p;
+  const i64 some = a->experts < a->rows ? a->experts : a->rows;
+  p.w = operand(a->dtype, a->w, a->experts, a->transpose_w ? a->n : a->k, a->transpose_w ? a->k : a->n, a->w_stride, a->w_row_stride);
+  p.x = operand(a->dtype, a->x, 1, a->rows, a->k, 0, a->x_stride);
+  // Packing reads and writes every expert's matrix: it pays from some rows an expert on.
+  p.tensor = !p.w.packs || a->rows >= 16 * some;
+  p.result = a->rows * a->n;
+  p.parts = parts_of(ceil_div(a->n, tcg::kFeat) * (some + a->rows / tcg::kTok), ceil_div(a->k, tcg::kBK) * (p.w.planes == 3 ? 6 : 1), p.result);
+  return p;
 }
-int parts_of(const ccb_nn_grouped_matmul_dw_t* a) {
-  if (!on_tensor_cores(a) || a->k == 0 || a->n == 0) return 1;
-  return parts_of(ceil_div(a->n, tcg::kFeat) * ceil_div(a->k, tcg::kTok) * a->experts, ceil_div(a->rows, a->experts * tcg::kBK), a->experts * a->k * a->n);
+Plan plan_of(const ccb_nn_grouped_matmul_dw_t* a) {
+  Plan p = {};
+  if (a->rows == 0 || a->n == 0 || a->k == 0) return p;
+  p.w = operand(a->dtype, a->dy, 1, a->rows, a->n, 0, a->dy_stride);
+  p.x = operand(a->dtype, a->x, 1, a->rows, a->k, 0, a->x_stride);
+  p.tensor = true;
+  p.result = a->experts * a->k * a->n;
+  p.parts = parts_of(ceil_div(a->n, tcg::kFeat) * ceil_div(a->k, tcg::kTok) * a->experts, ceil_div(a->rows, a->experts * tcg::kBK) * (p.w.planes == 3 ? 6 : 1), p.result);
+  return p;
 }
-template <class A>
-size_t parts_bytes(const A* a, i64 result) {
-  const int parts = parts_of(a);
-  return parts > 1 ? (size_t)parts * result * sizeof(float) : 0;
-}
-size_t workspace_of(const ccb_nn_grouped_matmul_t* a) { return parts_bytes(a, a->rows * a->n); }
-size_t workspace_of(const ccb_nn_grouped_matmul_dw_t* a) { return parts_bytes(a, a->experts * a->k * a->n); }
 // "" if the workspace is enough
 template <class A>
-std::string check_workspace(const A* a) {
-  const size_t need = workspace_of(a);
+std::string check_workspace(const A* a, const Plan& p) {
+  const size_t need = p.bytes();
   if (need == 0 || (a->workspace && aligned(a->workspace, 16) && a->workspace_bytes >= need)) return "";
   return "workspace of " + std::to_string(a->workspace_bytes) + " bytes: " + std::to_string(need) + " are needed, 16-byte aligned";
 }
@@ -847,76 +949,88 @@ bool encode_mn(ccb::TmaDesc* m, int fmt, const void* base, i64 cols, i64 rows, i
   return tcg::encode(m, fmt, base, 4, d, st, box);
 }
 
-int tensor_forward(const ccb_nn_grouped_matmul_t* a, int sms, cudaStream_t st, const char* me) {
+// The parts that both directions share.
+tcg::P tensor_params(const Plan& plan, const int* off, unsigned* err, int dtype, i64 rows, i64 experts, i64 k, i64 n) {
   tcg::P p = {};
-  const int fmt = a->dtype == CCB_BF16;
+  p.off = off;
+  p.err = err;
+  p.rows = (int)rows;
+  p.experts = (int)experts;
+  p.n = (int)n;
+  p.k = (int)k;
+  p.splits = plan.parts;
+  p.format = dtype != CCB_F16;
+  p.terms = dtype == CCB_F32 ? 6 : 1;
+  return p;
+}
+
+int tensor_forward(const ccb_nn_grouped_matmul_t* a, Plan plan, int sms, cudaStream_t st, const char* me) {
+  tcg::P p = tensor_params(plan, a->offsets, a->err, a->dtype, a->rows, a->experts, a->k, a->n);
+  char* room = static_cast<char*>(a->workspace);
+  if (const int rc = settle(&plan.w, a->dtype, &room, sms, st, me)) return rc;
+  if (const int rc = settle(&plan.x, a->dtype, &room, sms, st, me)) return rc;
   // tokens come in boxes of about half of what an expert has on average: a
   // box is one copy, and a larger one than needed is read in vain
   const i64 mean = a->rows / (a->experts < a->rows ? a->experts : a->rows);
   p.box = mean <= 16 ? 16 : mean <= 64 ? 64 : 128;
-  const i64 xd[4] = {a->k, a->rows, 1, 1}, xs[3] = {a->x_stride, 8, 8};
+  const i64 xd[4] = {a->k, a->rows, plan.x.planes, 1}, xs[3] = {plan.x.row_stride, a->rows * plan.x.row_stride, 8};
   const int xb[4] = {64, p.box, 1, 1};
-  bool ok = tcg::encode(&p.tb, fmt, a->x, 4, xd, xs, xb);
+  bool ok = tcg::encode(&p.tb, p.format, plan.x.p, 4, xd, xs, xb);
   if (a->transpose_w) {
-    const i64 wd[4] = {a->k, a->n, a->experts, 1}, ws[3] = {a->w_row_stride, a->w_stride, 8};
+    const i64 wd[4] = {a->k, a->n, a->experts * plan.w.planes, 1}, ws[3] = {plan.w.row_stride, plan.w.stride, 8};
     const int wb[4] = {64, 128, 1, 1};
-    ok = ok && tcg::encode(&p.ta, fmt, a->w, 4, wd, ws, wb);
+    ok = ok && tcg::encode(&p.ta, p.format, plan.w.p, 4, wd, ws, wb);
   } else {
-    ok = ok && encode_mn(&p.ta, fmt, a->w, a->n, a->k, a->experts, a->w_row_stride, a->w_stride, &p.a2);
+    ok = ok && encode_mn(&p.ta, p.format, plan.w.p, a->n, a->k, a->experts * plan.w.planes, plan.w.row_stride, plan.w.stride, &p.a2);
   }
   if (!ok) return fail(CCB_ERR_DRIVER, me, "cuTensorMapEncodeTiled refused x or w");
-  p.off = a->offsets;
   p.out = a->out;
-  p.err = a->err;
   p.os = a->out_stride;
-  p.rows = (int)a->rows;
-  p.experts = (int)a->experts;
-  p.n = (int)a->n;
-  p.k = (int)a->k;
-  p.splits = parts_of(a);
-  p.format = fmt;
   p.vec = aligned(a->out, 16) && a->out_stride % 8 == 0;
-  if (p.splits > 1) {
-    p.out = a->workspace;
+  const bool parts = p.splits > 1;
+  if (parts) {
+    p.out = room;
     p.os = a->n;
-    p.split_stride = a->rows * a->n;
-    if (const int rc = a->transpose_w ? tcg::go<float, tcg::kForwardT>(p, sms, st, me) : tcg::go<float, tcg::kForward>(p, sms, st, me)) return rc;
-    return fmt ? sum_parts(p, (__nv_bfloat16*)a->out, a->rows, a->n, a->out_stride, 1, 0, sms, st, me)
-               : sum_parts(p, (__half*)a->out, a->rows, a->n, a->out_stride, 1, 0, sms, st, me);
+    p.split_stride = plan.result;
   }
-  if (a->transpose_w) return fmt ? tcg::go<__nv_bfloat16, tcg::kForwardT>(p, sms, st, me) : tcg::go<__half, tcg::kForwardT>(p, sms, st, me);
-  return fmt ? tcg::go<__nv_bfloat16, tcg::kForward>(p, sms, st, me) : tcg::go<__half, tcg::kForward>(p, sms, st, me);
+  if (parts || a->dtype == CCB_F32) {
+    if (const int rc = a->transpose_w ? tcg::go<float, tcg::kForwardT>(p, sms, st, me) : tcg::go<float, tcg::kForward>(p, sms, st, me)) return rc;
+    if (!parts) return CCB_OK;
+    if (a->dtype == CCB_F32) return sum_parts(p, (float*)a->out, a->rows, a->n, a->out_stride, 1, 0, sms, st, me);
+    return p.format ? sum_parts(p, (__nv_bfloat16*)a->out, a->rows, a->n, a->out_stride, 1, 0, sms, st, me)
+                    : sum_parts(p, (__half*)a->out, a->rows, a->n, a->out_stride, 1, 0, sms, st, me);
+  }
+  if (a->transpose_w) return p.format ? tcg::go<__nv_bfloat16, tcg::kForwardT>(p, sms, st, me) : tcg::go<__half, tcg::kForwardT>(p, sms, st, me);
+  return p.format ? tcg::go<__nv_bfloat16, tcg::kForward>(p, sms, st, me) : tcg::go<__half, tcg::kForward>(p, sms, st, me);
 }
 
-int tensor_dw(const ccb_nn_grouped_matmul_dw_t* a, int sms, cudaStream_t st, const char* me) {
-  tcg::P p = {};
-  const int fmt = a->dtype == CCB_BF16;
-  if (!encode_mn(&p.tb, fmt, a->x, a->k, a->rows, 1, a->x_stride, 8, &p.b2) || !encode_mn(&p.ta, fmt, a->dy, a->n, a->rows, 1, a->dy_stride, 8, &p.a2))
+int tensor_dw(const ccb_nn_grouped_matmul_dw_t* a, Plan plan, int sms, cudaStream_t st, const char* me) {
+  tcg::P p = tensor_params(plan, a->offsets, a->err, a->dtype, a->rows, a->experts, a->k, a->n);
+  char* room = static_cast<char*>(a->workspace);
+  if (const int rc = settle(&plan.w, a->dtype, &room, sms, st, me)) return rc;
+  if (const int rc = settle(&plan.x, a->dtype, &room, sms, st, me)) return rc;
+  if (!encode_mn(&p.tb, p.format, plan.x.p, a->k, a->rows, plan.x.planes, plan.x.row_stride, a->rows * plan.x.row_stride, &p.b2) ||
+      !encode_mn(&p.ta, p.format, plan.w.p, a->n, a->rows, plan.w.planes, plan.w.row_stride, a->rows * plan.w.row_stride, &p.a2))
     return fail(CCB_ERR_DRIVER, me, "cuTensorMapEncodeTiled refused x or dy");
-  p.off = a->offsets;
   p.out = a->out;
-  p.err = a->err;
   p.os = a->out_row_stride;
   p.oe = a->out_stride;
-  p.rows = (int)a->rows;
-  p.experts = (int)a->experts;
-  p.n = (int)a->n;
-  p.k = (int)a->k;
-  p.splits = parts_of(a);
-  p.format = fmt;
   p.vec = aligned(a->out, 16) && a->out_row_stride % 8 == 0 && (a->experts == 1 || a->out_stride % 8 == 0);
-  if (p.splits > 1) {
-    p.out = a->workspace;
+  const bool parts = p.splits > 1;
+  if (parts) {
+    p.out = room;
     p.os = a->n;
     p.oe = a->k * a->n;
-    p.split_stride = a->experts * p.oe;
-    if (const int rc = tcg::go<float, tcg::kDw>(p, sms, st, me)) return rc;
-    if (a->out_dtype == CCB_F32) return sum_parts(p, (float*)a->out, a->k, a->n, a->out_row_stride, a->experts, a->out_stride, sms, st, me);
-    return fmt ? sum_parts(p, (__nv_bfloat16*)a->out, a->k, a->n, a->out_row_stride, a->experts, a->out_stride, sms, st, me)
-               : sum_parts(p, (__half*)a->out, a->k, a->n, a->out_row_stride, a->experts, a->out_stride, sms, st, me);
+    p.split_stride = plan.result;
   }
-  if (a->out_dtype == CCB_F32) return tcg::go<float, tcg::kDw>(p, sms, st, me);
-  return fmt ? tcg::go<__nv_bfloat16, tcg::kDw>(p, sms, st, me) : tcg::go<__half, tcg::kDw>(p, sms, st, me);
+  if (parts || a->out_dtype == CCB_F32) {
+    if (const int rc = tcg::go<float, tcg::kDw>(p, sms, st, me)) return rc;
+    if (!parts) return CCB_OK;
+    if (a->out_dtype == CCB_F32) return sum_parts(p, (float*)a->out, a->k, a->n, a->out_row_stride, a->experts, a->out_stride, sms, st, me);
+    return p.format ? sum_parts(p, (__nv_bfloat16*)a->out, a->k, a->n, a->out_row_stride, a->experts, a->out_stride, sms, st, me)
+                    : sum_parts(p, (__half*)a->out, a->k, a->n, a->out_row_stride, a->experts, a->out_stride, sms, st, me);
+  }
+  return p.format ? tcg::go<__nv_bfloat16, tcg::kDw>(p, sms, st, me) : tcg::go<__half, tcg::kDw>(p, sms, st, me);
 }
 
 }  // namespace
@@ -930,7 +1044,7 @@ extern "C" int ccb_nn_grouped_matmul_workspace(const ccb_nn_grouped_matmul_t* a,
     if (!a || !bytes) return fail(CCB_ERR_INVALID, me, "null pointer");
     const std::string bad = check_grouped(a);
     if (!bad.empty()) return fail(CCB_ERR_INVALID, me, bad);
-    *bytes = workspace_of(a);
+    *bytes = plan_of(a).bytes();
     return CCB_OK;
   })
 }
@@ -941,7 +1055,7 @@ extern "C" int ccb_nn_grouped_matmul_dw_workspace(const ccb_nn_grouped_matmul_dw
     if (!a || !bytes) return fail(CCB_ERR_INVALID, me, "null pointer");
     const std::string bad = check_dw(a);
     if (!bad.empty()) return fail(CCB_ERR_INVALID, me, bad);
-    *bytes = workspace_of(a);
+    *bytes = plan_of(a).bytes();
     return CCB_OK;
   })
 }
@@ -955,12 +1069,13 @@ extern "C" int ccb_nn_grouped_matmul(const ccb_nn_grouped_matmul_t* a, void* str
     if (a->rows == 0 || a->n == 0) return CCB_OK;
     if (!a->offsets || !a->out || (a->k > 0 && (!a->x || !a->w))) return fail(CCB_ERR_INVALID, me, "null pointer");
     if (!aligned(a->offsets, 4) || !aligned(a->err, 4)) return fail(CCB_ERR_INVALID, me, "offsets or err is not aligned to 4 bytes");
-    const std::string small = check_workspace(a);
+    const Plan plan = plan_of(a);
+    const std::string small = check_workspace(a, plan);
     if (!small.empty()) return fail(CCB_ERR_INVALID, me, small);
     int sms = 0;
     if (const int rc = sm_count(me, &sms)) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (on_tensor_cores(a)) return tensor_forward(a, sms, st, me);
+    if (plan.tensor) return tensor_forward(a, plan, sms, st, me);
     const GroupP p = {a->x, a->w, a->offsets, a->out, a->err, a->k, a->n, a->x_stride, a->w_stride, a->w_row_stride, a->out_stride, (int)a->rows, (int)a->experts};
     if (a->dtype == CCB_F32)
       any<float>(p, a->transpose_w, sms, st);
@@ -981,12 +1096,13 @@ extern "C" int ccb_nn_grouped_matmul_dw(const ccb_nn_grouped_matmul_dw_t* a, voi
     if (a->k == 0 || a->n == 0) return CCB_OK;
     if (!a->offsets || !a->out || (a->rows > 0 && (!a->x || !a->dy))) return fail(CCB_ERR_INVALID, me, "null pointer");
     if (!aligned(a->offsets, 4) || !aligned(a->err, 4)) return fail(CCB_ERR_INVALID, me, "offsets or err is not aligned to 4 bytes");
-    const std::string small = check_workspace(a);
+    const Plan plan = plan_of(a);
+    const std::string small = check_workspace(a, plan);
     if (!small.empty()) return fail(CCB_ERR_INVALID, me, small);
     int sms = 0;
     if (const int rc = sm_count(me, &sms)) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (on_tensor_cores(a)) return tensor_dw(a, sms, st, me);
+    if (plan.tensor) return tensor_dw(a, plan, sms, st, me);
     const GroupDwP p = {a->x, a->dy, a->offsets, a->out, a->err, a->k, a->n, a->x_stride, a->dy_stride, a->out_stride, a->out_row_stride, (int)a->rows, (int)a->experts};
     if (a->dtype == CCB_F32)
       any_dw<float, float>(p, sms, st);
