@@ -191,6 +191,142 @@ __global__ void __launch_bounds__(256) grouped_dw_any(const __grid_constant__ Gr
   }
 }
 
+// ------------------------------------- CUDA cores, few rows an expert, any alignment
+// Bound by reading the matrices of the experts that have rows: a block takes up
+// to 8 rows of one expert, a block of output columns and a part of the
+// contraction, keeps the rows' values in shared memory and reads every weight
+// once, in order. Parts are summed by add_parts, so that the SMs are filled
+// whatever the shape.
+constexpr int kFewRows = 8, kFewCols = 512, kFewColsT = 64, kFewK = 1024, kFewThreads = 128;
+
+struct FewP {
+  GroupP g;
+  int splits;
+  i64 split_stride, part;  // elements between parts' results, of the contraction in a part
+};
+
+template <class T, class TO, bool WT>
+__global__ void __launch_bounds__(kFewThreads) grouped_few(const __grid_constant__ FewP q) {
+  __shared__ Segments g;
+  __shared__ __align__(16) float xs[kFewRows * kFewK];  // [k][row], or [row][k] for a transposed w
+  const GroupP& p = q.g;
+  lay_out(g, p.off, p.experts, p.rows, kFewRows, p.err);
+  const int segs = p.experts + 2;
+  const i64 nc = (p.n + (WT ? kFewColsT : kFewCols) - 1) / (WT ? kFewColsT : kFewCols), total = nc * q.splits * g.tile[segs];
+  const T* x = static_cast<const T*>(p.x);
+  for (i64 t = blockIdx.x; t < total; t += gridDim.x) {
+    const int split = (int)(t / nc % q.splits), mt = (int)(t / nc / q.splits), s = segment_of(g, segs, mt);
+    const int r0 = g.row[s] + (mt - g.tile[s]) * kFewRows, rows = min(g.row[s + 1] - r0, kFewRows);
+    const bool real = s >= 1 && s <= p.experts;
+    const i64 n0 = (t % nc) * (WT ? kFewColsT : kFewCols), k0 = split * q.part, k1 = real ? min(p.k, k0 + q.part) : k0;
+    const T* w = static_cast<const T*>(p.w) + (real ? (s - 1) * p.we : 0);
+    TO* out = static_cast<TO*>(p.out) + split * q.split_stride;
+    float acc[4][kFewRows] = {};
+    // the rows' values, and 0 to the end of the last step
+    const int kn = (int)(k1 - k0), kz = WT ? (kn + 255) & ~255 : (kn + 7) & ~7;
+    __syncthreads();
+#pragma unroll 8
+    for (int i = threadIdx.x; i < kFewRows * kz; i += kFewThreads) {
+      const int r = i / kz, k = i - r * kz;
+      xs[WT ? r * kFewK + k : k * kFewRows + r] = r < rows && k < kn ? to_f<T>(x[(i64)(r0 + r) * p.xs + k0 + k]) : 0.0f;
+    }
+    __syncthreads();
+    // 16 weights in hand and the next 16 on their way; of 16-bit ones twice as many
+    constexpr int kStep = sizeof(T) == 4 ? 4 : 8;
+    float v[kStep][4], u[kStep][4];
+    if constexpr (!WT) {
+      bool on[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) on[j] = n0 + threadIdx.x + j * kFewThreads < p.n;
+      const T* at = w + k0 * p.ws + n0 + threadIdx.x;
+      auto fetch = [&](float (*to)[4], int k) {
+#pragma unroll
+        for (int i = 0; i < kStep; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) to[i][j] = on[j] && k + i < kn ? to_f<T>(at[(k + i) * p.ws + j * kFewThreads]) : 0.0f;
+      };
+      fetch(u, 0);
+      for (int k = 0; k < kn; k += kStep) {
+#pragma unroll
+        for (int i = 0; i < 4 * kStep; ++i) v[i >> 2][i & 3] = u[i >> 2][i & 3];
+        fetch(u, k + kStep);
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) {
+          const float4 a = *reinterpret_cast<const float4*>(xs + (k + i) * kFewRows), b = *reinterpret_cast<const float4*>(xs + (k + i) * kFewRows + 4);
+          const float xv[kFewRows] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < kFewRows; ++r) acc[j][r] = fmaf(xv[r], v[i][j], acc[j][r]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const i64 c = n0 + threadIdx.x + j * kFewThreads;
+        if (c >= p.n) continue;
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r)
+          if (r < rows) out[(i64)(r0 + r) * p.os + c] = from_f<TO>(acc[j][r]);
+      }
+    } else {
+      const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+      for (int c0 = warp * 4; c0 < kFewColsT && n0 + c0 < p.n; c0 += kFewThreads / 32 * 4) {
+        const T* at[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          at[j] = w + min(n0 + c0 + j, p.n - 1) * p.ws + k0;  // a column too many repeats the last
+#pragma unroll
+          for (int r = 0; r < kFewRows; ++r) acc[j][r] = 0.0f;
+        }
+        auto fetch = [&](float (*to)[4], int k) {
+#pragma unroll
+          for (int i = 0; i < kStep; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[i][j] = k + 32 * i < kn ? to_f<T>(at[j][k + 32 * i]) : 0.0f;
+        };
+        fetch(u, lane);
+        for (int k = lane; k < kz; k += 32 * kStep) {
+#pragma unroll
+          for (int i = 0; i < 4 * kStep; ++i) v[i >> 2][i & 3] = u[i >> 2][i & 3];
+          fetch(u, k + 32 * kStep);
+#pragma unroll
+          for (int i = 0; i < kStep; ++i) {
+            float xv[kFewRows];
+#pragma unroll
+            for (int r = 0; r < kFewRows; ++r) xv[r] = xs[r * kFewK + k + 32 * i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int r = 0; r < kFewRows; ++r) acc[j][r] = fmaf(xv[r], v[i][j], acc[j][r]);
+          }
+        }
+        // the warp's 32 sums, halved from step to step: lane 8 j + r ends with column j of row r
+        float* a = &acc[0][0];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+          for (int i = 0; i < o; ++i) {
+            const float give = lane & o ? a[i] : a[i + o], keep = lane & o ? a[i + o] : a[i];
+            a[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+          }
+        const int r = lane & 7;
+        const i64 c = n0 + c0 + (lane >> 3);
+        if (r < rows && c < p.n) out[(i64)(r0 + r) * p.os + c] = from_f<TO>(a[0]);
+      }
+    }
+  }
+}
+
+template <class T, class TO>
+void few(const FewP& q, bool wt, int sms, cudaStream_t st) {
+  const i64 cols = wt ? kFewColsT : kFewCols, tiles = (q.g.rows / kFewRows + q.g.experts + 2) * ((q.g.n + cols - 1) / cols) * q.splits, most = (i64)sms * 5;
+  const unsigned grid = (unsigned)(tiles < most ? tiles : most);
+  if (wt)
+    grouped_few<T, TO, true><<<grid, kFewThreads, 0, st>>>(q);
+  else
+    grouped_few<T, TO, false><<<grid, kFewThreads, 0, st>>>(q);
+}
+
 template <class T>
 void any(const GroupP& p, bool wt, int sms, cudaStream_t st) {
   const i64 tiles = ((p.rows + kB - 1) / kB + p.experts + 1) * ((p.n + kB - 1) / kB), most = (i64)sms * 4;
@@ -360,33 +496,37 @@ __device__ __forceinline__ void drain16(unsigned taddr, bool zero, unsigned buf,
                  "r"(h[8 + 2 * j]), "r"(h[8 + 2 * j + 1])
                  : "memory");
   __syncwarp();
-  // token 8 j + lane / 4, piece lane % 4
-  const unsigned get = buf + (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
-  uint4 w[4];
+  if (vec && feats >= 8) {
+    // token 8 j + lane / 4, piece lane % 4
+    const unsigned get = buf + (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
+    uint4 w[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[j].x), "=r"(w[j].y), "=r"(w[j].z), "=r"(w[j].w) : "r"(get + j * 512) : "memory");
-  __syncwarp();
-  const int f = (lane & 3) * 8, tok = lane >> 2;
-  TO* dst = out + tok * os + f;
-  if (vec && tokens >= 32 && feats >= 32) {
+    for (int j = 0; j < 4; ++j)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[j].x), "=r"(w[j].y), "=r"(w[j].z), "=r"(w[j].w) : "r"(get + j * 512) : "memory");
+    const int f = (lane & 3) * 8, tok = lane >> 2;
+    TO* dst = out + tok * os + f;
+    if (tokens >= 32 && feats >= 32) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + 8 * j * os) = w[j];
-  } else {
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + 8 * j * os) = w[j];
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (8 * j + tok >= tokens || f >= feats) continue;
-      TO* at = dst + 8 * j * os;
-      if (vec && f + 8 <= feats) {
-        *reinterpret_cast<uint4*>(at) = w[j];
-      } else {
-        const unsigned u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (f + i < feats) reinterpret_cast<unsigned short*>(at)[i] = (unsigned short)(u[i >> 1] >> (16 * (i & 1)));
-      }
+      for (int j = 0; j < 4; ++j)
+        if (8 * j + tok < tokens && f + 8 <= feats) *reinterpret_cast<uint4*>(dst + 8 * j * os) = w[j];
     }
   }
+  // what is left of unaligned rows and of the last features: lane by lane
+  const int done = vec ? feats & ~7 : 0;
+  if (done < feats && done < 32) {
+    const bool on = lane >= done && lane < feats;
+    TO* dst = out + lane;
+#pragma unroll 8
+    for (int t = 0; t < 32; ++t) {
+      unsigned short h;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(buf + t * 64 + (((lane >> 3) ^ ((t >> 1) & 3)) << 4) + (lane & 7) * 2) : "memory");
+      if (on && t < tokens) *reinterpret_cast<unsigned short*>(dst + t * os) = h;
+    }
+  }
+  __syncwarp();
 }
 // The same in 32 bits: lanes are features, a store is one token's 128 bytes.
 __device__ __forceinline__ void drain32(unsigned taddr, bool zero, float* out, i64 os, int tokens, int feats, int lane) {
@@ -891,11 +1031,11 @@ int parts_of(i64 tiles, i64 steps, i64 result) {
 
 // What a call does, by its sizes, types, strides and alignment alone.
 struct Plan {
-  bool tensor;     // on the tensor cores
+  bool tensor;     // on the tensor cores; else rows are few
   Operand w, x;    // M side, N side
   int parts;       // of the contraction
   i64 result;      // elements of one part's
-  size_t bytes() const { return tensor ? w.bytes() + x.bytes() + (parts > 1 ? (size_t)parts * result * sizeof(float) : 0) : 0; }
+  size_t bytes() const { return (tensor ? w.bytes() + x.bytes() : 0) + (parts > 1 ? (size_t)parts * result * sizeof(float) : 0); }
 };
 Plan plan_of(const ccb_nn_grouped_matmul_t* a) {
   Plan p = {};
@@ -906,6 +1046,12 @@ Plan plan_of(const ccb_nn_grouped_matmul_t* a) {
   // Packing reads and writes every expert's matrix: it pays from some rows an expert on.
   p.tensor = !p.w.packs || a->rows >= 16 * some;
   p.result = a->rows * a->n;
+  if (!p.tensor) {  // two tiles for each of five blocks an SM, and no part above what shared memory takes
+    const i64 tiles = ceil_div(a->n, a->transpose_w ? kFewColsT : kFewCols) * (some + a->rows / kFewRows), most = ceil_div(a->k, a->transpose_w ? 512 : 64), least = ceil_div(a->k, kFewK);
+    const i64 want = ceil_div(10 * 148, tiles);
+    p.parts = (int)(want < least ? least : want > most ? most : want);
+    return p;
+  }
   p.parts = parts_of(ceil_div(a->n, tcg::kFeat) * (some + a->rows / tcg::kTok), ceil_div(a->k, tcg::kBK) * (p.w.planes == 3 ? 6 : 1), p.result);
   return p;
 }
@@ -1004,6 +1150,30 @@ int tensor_forward(const ccb_nn_grouped_matmul_t* a, Plan plan, int sms, cudaStr
   return p.format ? tcg::go<__nv_bfloat16, tcg::kForward>(p, sms, st, me) : tcg::go<__half, tcg::kForward>(p, sms, st, me);
 }
 
+template <class T>
+int few_of(FewP* q, const ccb_nn_grouped_matmul_t* a, int sms, cudaStream_t st, const char* me) {
+  if (q->splits == 1) {
+    few<T, T>(*q, a->transpose_w, sms, st);
+    return launched(me);
+  }
+  q->g.out = a->workspace;
+  q->g.os = a->n;
+  q->split_stride = a->rows * a->n;
+  few<T, float>(*q, a->transpose_w, sms, st);
+  if (const int rc = launched(me)) return rc;
+  tcg::P p = {};
+  p.out = a->workspace;
+  p.splits = q->splits;
+  p.split_stride = q->split_stride;
+  return sum_parts(p, static_cast<T*>(a->out), a->rows, a->n, a->out_stride, 1, 0, sms, st, me);
+}
+int few_forward(const ccb_nn_grouped_matmul_t* a, const Plan& plan, int sms, cudaStream_t st, const char* me) {
+  FewP q = {{a->x, a->w, a->offsets, a->out, a->err, a->k, a->n, a->x_stride, a->w_stride, a->w_row_stride, a->out_stride, (int)a->rows, (int)a->experts},
+            plan.parts, 0, ceil_div(a->k, plan.parts)};
+  if (a->dtype == CCB_F32) return few_of<float>(&q, a, sms, st, me);
+  return a->dtype == CCB_BF16 ? few_of<__nv_bfloat16>(&q, a, sms, st, me) : few_of<__half>(&q, a, sms, st, me);
+}
+
 int tensor_dw(const ccb_nn_grouped_matmul_dw_t* a, Plan plan, int sms, cudaStream_t st, const char* me) {
   tcg::P p = tensor_params(plan, a->offsets, a->err, a->dtype, a->rows, a->experts, a->k, a->n);
   char* room = static_cast<char*>(a->workspace);
@@ -1076,6 +1246,7 @@ extern "C" int ccb_nn_grouped_matmul(const ccb_nn_grouped_matmul_t* a, void* str
     if (const int rc = sm_count(me, &sms)) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (plan.tensor) return tensor_forward(a, plan, sms, st, me);
+    if (plan.parts > 0) return few_forward(a, plan, sms, st, me);
     const GroupP p = {a->x, a->w, a->offsets, a->out, a->err, a->k, a->n, a->x_stride, a->w_stride, a->w_row_stride, a->out_stride, (int)a->rows, (int)a->experts};
     if (a->dtype == CCB_F32)
       any<float>(p, a->transpose_w, sms, st);

@@ -69,7 +69,7 @@ def _dense(shape):
 def _see(x, what):
     """(pointer, type code, shape, strides) of an argument in device memory."""
     try:
-        ptr, dtype, shape, strides = x.data_ptr, x.dtype, x.shape, x.stride
+        ptr, dtype, shape, strides, here = x.data_ptr, x.dtype, x.shape, x.stride, x.is_cuda
     except AttributeError:
         if isinstance(x, Array):
             shape = tuple(x.shape)
@@ -77,20 +77,28 @@ def _see(x, what):
         if isinstance(x, Resident):
             return x.buf.ptr or 0, _code(x.dtype, what), tuple(x.shape), _dense(x.shape)
         raise ValueError(f"{what} is a {type(x).__name__}: an array in device memory is needed") from None
-    if not getattr(x, "is_cuda", True):
+    if not here:
         raise ValueError(f"{what} is not in device memory")
-    return ptr(), _code(dtype, what), shape, strides()
+    code = _BY_TYPE.get(dtype)
+    return ptr(), _code(dtype, what) if code is None else code, shape, strides()
 
 
 def _mat(x, what):
     """(pointer, type code, rows, cols, row stride)."""
+    try:  # the common case in few steps: a dense matrix of another library
+        if x.is_contiguous() and x.is_cuda:
+            rows, cols = x.shape
+            return x.data_ptr(), _BY_TYPE[x.dtype], rows, cols, cols
+    except (AttributeError, ValueError, KeyError):
+        pass
     ptr, code, shape, strides = _see(x, what)
     rank = len(shape)
     if rank == 2:
         rows, cols = shape
-        if cols > 1 and strides[1] != 1:
-            raise ValueError(f"{what} has stride {strides[1]} along its rows: 1 is needed")
-        return ptr, code, rows, cols, strides[0] if rows > 1 else cols
+        stride, along = strides
+        if along != 1 and cols > 1:
+            raise ValueError(f"{what} has stride {along} along its rows: 1 is needed")
+        return ptr, code, rows, cols, stride if rows > 1 else cols
     if rank == 0:
         return ptr, code, 1, 1, 1
     cols = shape[-1]
@@ -122,6 +130,11 @@ def _vector(x, cols, what):
     """(pointer, type code) of a dense vector of `cols`, or (0, None)."""
     if x is None:
         return 0, None
+    try:
+        if x.is_contiguous() and x.is_cuda and x.shape == (cols,):
+            return x.data_ptr(), _BY_TYPE[x.dtype]
+    except (AttributeError, KeyError):
+        pass
     ptr, code, rows, n, _ = _mat(x, what)
     if rows != 1 or n != cols:
         raise ValueError(f"{what} has {rows * n} elements, expected {cols}")
@@ -144,13 +157,9 @@ def _floats(code, what):
 
 
 def _word(v, what):
-    if not 0 <= v < 1 << 64:
+    if not 0 <= v <= 0xFFFFFFFFFFFFFFFF:
         raise ValueError(f"{what} = {v} is outside [0, 2^64)")
     return v
-
-
-def _handle(stream):
-    return stream.h if isinstance(stream, R.Stream) else stream
 
 
 def _space(ws):
@@ -171,7 +180,7 @@ def _space(ws):
 
 
 def _call(name, args, stream):
-    rc = getattr(R._LIB or R.lib(), name)(args, _handle(stream))
+    rc = getattr(R._LIB or R.lib(), name)(args, stream.h if isinstance(stream, R.Stream) else stream)
     if rc:
         R.check(rc)
 
@@ -227,8 +236,10 @@ def _like(x, rows, cols, code, what):
     if x is None:
         return 0, 0
     ptr, c, r, n, s = _mat(x, what)
-    _same((r, n), (rows, cols), what)
-    _typed(c, code, what)
+    if r != rows or n != cols:
+        _same((r, n), (rows, cols), what)
+    if c != code:
+        _typed(c, code, what)
     return ptr, s
 
 
@@ -259,12 +270,15 @@ def _weights(cols, *named):
     """The pointers of the optional vectors, and their common type code."""
     code, out = None, []
     for name, v in named:
-        ptr, c = _vector(v, cols, f"nn.block_norm: {name}")
-        if c is not None:
-            _floats(c, f"nn.block_norm: {name}")
-            if code is not None and c != code:
-                raise ValueError("nn.block_norm: weights and biases have different element types")
-            code = c
+        if v is None:
+            out.append(0)
+            continue
+        ptr, c = _vector(v, cols, name)
+        if c == 2:
+            _floats(c, name)
+        if code is not None and c != code:
+            raise ValueError("nn.block_norm: weights and biases have different element types")
+        code = c
         out.append(ptr)
     return out, code or 0
 
@@ -298,7 +312,7 @@ def block_norm(x, y=None, h=None, *, kind="rms", eps=1e-6, branch=None, post_nor
     yp, ys = _like(y, rows, cols, xc, "nn.block_norm: y")
     hp, hs = _like(h, rows, cols, code, "nn.block_norm: h")
     gp, gs, gc = _gate(gate, rows, cols, code)
-    (w1, c1, w2, c2), wc = _weights(cols, ("pre_weight", pre_weight), ("pre_bias", pre_bias), ("post_weight", post_weight), ("post_bias", post_bias))
+    (w1, c1, w2, c2), wc = _weights(cols, ("nn.block_norm: pre_weight", pre_weight), ("nn.block_norm: pre_bias", pre_bias), ("nn.block_norm: post_weight", post_weight), ("nn.block_norm: post_bias", post_bias))
     _call("ccb_nn_block_norm", _NORM.pack(xp, bp, gp, w1, c1, w2, c2, yp, hp, rows, cols, xs, bs, gs, ys, hs, _word(seed, "nn.block_norm: seed"),
                                           _word(offset, "nn.block_norm: offset"), _word(base, "nn.block_norm: base"), p, eps, scale, code, xc, gc, wc,
                                           _pick(KINDS, kind, "kind"), _pick(ACTS, gate_act, "gate_act"), 1 if post_norm else 0), stream)
@@ -345,12 +359,12 @@ def block_norm_backward(y, *, dy=None, dh=None, dx=None, dbranch=None, dgate=Non
         else:
             dgp, dgs = _like(dgate, rows, cols, gc, "nn.block_norm: dgate")
     # biases have no part in the gradient but for the gate's, through u
-    (w1, w2, c2), wc = _weights(cols, ("pre_weight", pre_weight), ("post_weight", post_weight), ("post_bias", post_bias))
+    (w1, w2, c2), wc = _weights(cols, ("nn.block_norm: pre_weight", pre_weight), ("nn.block_norm: post_weight", post_weight), ("nn.block_norm: post_bias", post_bias))
     sums = []
-    for name, v in (("dpre_weight", dpre_weight), ("dpre_bias", dpre_bias), ("dpost_weight", dpost_weight), ("dpost_bias", dpost_bias)):
-        ptr, c = _vector(v, cols, f"nn.block_norm: {name}")
-        if c is not None:
-            _typed(c, 0, f"nn.block_norm: {name}")
+    for name, v in (("nn.block_norm: dpre_weight", dpre_weight), ("nn.block_norm: dpre_bias", dpre_bias), ("nn.block_norm: dpost_weight", dpost_weight), ("nn.block_norm: dpost_bias", dpost_bias)):
+        ptr, c = _vector(v, cols, name)
+        if c:
+            _typed(c, 0, name)
         sums.append(ptr)
     wp, wn = _space(workspace)
     _call("ccb_nn_block_norm_backward",
