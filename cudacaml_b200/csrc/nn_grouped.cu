@@ -384,7 +384,6 @@ struct P {
   i64 os, oe;           // strides of out: a row, an expert's matrix (dw)
   i64 split_stride;     // elements from one part's result to the next
   int rows, experts, n, k, splits, format;
-  int terms;            // products of planes that make up one of the operands: 1, or 6 for f32
   int a2, b2;           // whether one copy takes two 64-wide blocks of an MN-major operand
   int box;              // rows of a copy of tokens
   int vec;              // out takes 16-byte stores
@@ -528,6 +527,19 @@ __device__ __forceinline__ void drain16(unsigned taddr, bool zero, unsigned buf,
   }
   __syncwarp();
 }
+template <class TO>
+__device__ __forceinline__ void store32(const float* v, TO* out, i64 os, int tokens, int feats, int lane) {
+  if (lane >= feats) return;
+  TO* dst = out + lane;
+  if (tokens >= 32) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) dst[i * os] = v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < tokens) dst[i * os] = v[i];
+  }
+}
 // The same in 32 bits: lanes are features, a store is one token's 128 bytes.
 __device__ __forceinline__ void drain32(unsigned taddr, bool zero, float* out, i64 os, int tokens, int feats, int lane) {
   float v[32];
@@ -537,17 +549,7 @@ __device__ __forceinline__ void drain32(unsigned taddr, bool zero, float* out, i
   } else {
     ccb::tc::ld32(taddr, v);
   }
-  if (lane < feats) {
-    float* dst = out + lane;
-    if (tokens >= 32) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) dst[i * os] = v[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < tokens) dst[i * os] = v[i];
-    }
-  }
+  store32(v, out, os, tokens, feats, lane);
 }
 
 // One thread of a converged warp. The loops that issue copies and MMAs are run
@@ -566,28 +568,26 @@ struct Tile {
   int r0, r1;      // rows: of the result (forward), of the contraction (dw)
   int f0, c0;      // first feature; first column of x (dw)
   int nn;          // N of the MMA
-  int kt;          // steps of the contraction of one term
-  int b0, b1;      // steps of all terms
+  int b0, b1;      // steps of the contraction
   int split;
 };
-// Step b of a tile: `kb`-th of the contraction in term `term`.
-struct Step {
-  int kb, term;
-  __device__ __forceinline__ explicit Step(const Tile& o) : kb(o.kt ? o.b0 % o.kt : 0), term(o.kt ? o.b0 / o.kt : 0) {}
-  __device__ __forceinline__ void next(const Tile& o) {
-    if (++kb == o.kt) {
-      kb = 0;
-      ++term;
-    }
-  }
-};
-// The planes of a term: f32 operands are sums hi + mid + lo of three 16-bit
-// planes, and the six products down to 2^-16 of the largest are added up from
-// the smallest, so that the accumulator's rounding is that of the last term's
-// steps.
-__device__ __forceinline__ int plane_m(int terms, int term) { return terms == 1 ? 0 : (0x001102 >> (4 * term)) & 15; }
-__device__ __forceinline__ int plane_n(int terms, int term) { return terms == 1 ? 0 : (0x010120 >> (4 * term)) & 15; }
-
+// f32 operands are sums hi + mid + lo of three 16-bit planes (WIDE), and a
+// product is the six of their products down to 2^-16 of the largest, added up
+// from the smallest. The accumulator truncates: over a long contraction that
+// is a bias of some 2^-25 of it for each MMA, so a tile's contraction is cut
+// into chunks of kChunk steps, each summed from 0 in its six terms, and the
+// draining warps add the chunks up in registers, rounding to nearest (the
+// error against 64 bits at K = 1024: 1.0e-6 in one go, see below by chunks).
+constexpr int kChunk = 4;
+template <bool WIDE>
+__device__ __forceinline__ int chunk_end(int a, int b1) { return WIDE ? min(a + kChunk, b1) : b1; }
+template <bool WIDE>
+__device__ __forceinline__ constexpr int terms() { return WIDE ? 6 : 1; }
+// The planes of a term.
+template <bool WIDE>
+__device__ __forceinline__ int plane_m(int term) { return WIDE ? (0x001102 >> (4 * term)) & 15 : 0; }
+template <bool WIDE>
+__device__ __forceinline__ int plane_n(int term) { return WIDE ? (0x010120 >> (4 * term)) & 15 : 0; }
 enum { kForward = 0, kForwardT = 1, kDw = 2 };
 
 template <int MODE>
@@ -606,6 +606,7 @@ __device__ __forceinline__ Tile tile_at(const P& p, const Segments& g, unsigned 
   t /= nf;
   o.split = (int)(t % (unsigned)p.splits);
   t /= (unsigned)p.splits;
+  int steps;
   if (MODE == kDw) {
     const unsigned nc = (p.k + kTok - 1) / kTok;
     o.c0 = (int)(t % nc) * kTok;
@@ -613,7 +614,7 @@ __device__ __forceinline__ Tile tile_at(const P& p, const Segments& g, unsigned 
     o.r0 = g.row[o.expert + 1];
     o.r1 = g.row[o.expert + 2];
     o.nn = p.k - o.c0 > kTok / 2 ? kTok : kTok / 2;
-    o.kt = (o.r1 - o.r0 + kBK - 1) / kBK;
+    steps = (o.r1 - o.r0 + kBK - 1) / kBK;
   } else {
     const int s = segment_of(g, p.experts + 2, (int)t);
     const int first = g.row[s], rows = g.row[s + 1] - first, parts = g.tile[s + 1] - g.tile[s], i = (int)t - g.tile[s];
@@ -623,20 +624,19 @@ __device__ __forceinline__ Tile tile_at(const P& p, const Segments& g, unsigned 
     o.r1 = first + min((i + 1) * each, rows);
     o.c0 = 0;
     o.nn = max((o.r1 - o.r0 + 31) & ~31, 32);
-    o.kt = o.expert < 0 ? 0 : (p.k + kBK - 1) / kBK;
+    steps = o.expert < 0 ? 0 : (p.k + kBK - 1) / kBK;
   }
-  const int steps = o.kt * p.terms;
   o.b0 = (int)((i64)steps * o.split / p.splits);
   o.b1 = (int)((i64)steps * (o.split + 1) / p.splits);
   return o;
 }
 // Whether a step of a dw tile reaches past its expert's rows.
 template <int MODE>
-__device__ __forceinline__ bool clears(const Tile& o, const Step& at) {
-  return MODE == kDw && o.r1 - o.r0 - at.kb * kBK < kBK;
+__device__ __forceinline__ bool clears(const Tile& o, int kb) {
+  return MODE == kDw && o.r1 - o.r0 - kb * kBK < kBK;
 }
 
-template <class TO, int MODE>
+template <class TO, int MODE, bool WIDE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped_tc(const __grid_constant__ P p) {
   using namespace ccb;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -682,62 +682,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
       const int half = o.nn >> 1, f = o.f0 + (int)rank * 128, c = o.c0 + (int)rank * half, tok = o.r0 + (int)rank * half;
       const int boxes = MODE == kDw ? (p.b2 ? 1 : half / 64) : (half + p.box - 1) / p.box;
       const unsigned box = MODE == kDw ? (p.b2 ? 16384u : 8192u) : (unsigned)p.box * 128u, bytes = kABytes + boxes * box;
-      Step in(o);
-      for (int b = o.b0; b < o.b1; ++b, in.next(o)) {
-        wait(empty + st, phase);
-        if (one) {
-          unsigned bar = lead_full + st;
-          const int pm = plane_m(p.terms, in.term), pn = plane_n(p.terms, in.term);
-          if (clears<MODE>(o, in)) {
-            bar = part + st;
-            expect(bar, bytes);
-          } else if (rank == 0) {
-            expect(full + st, 2u * bytes);
-          } else {
-            arrive_relaxed(bar);
+      int a = o.b0;
+      do {
+        const int z = chunk_end<WIDE>(a, o.b1);
+        for (int term = 0; term < terms<WIDE>(); ++term)
+          for (int kb = a; kb < z; ++kb) {
+            wait(empty + st, phase);
+            if (one) {
+              unsigned bar = lead_full + st;
+              const int pm = plane_m<WIDE>(term), pn = plane_n<WIDE>(term);
+              if (clears<MODE>(o, kb)) {
+                bar = part + st;
+                expect(bar, bytes);
+              } else if (rank == 0) {
+                expect(full + st, 2u * bytes);
+              } else {
+                arrive_relaxed(bar);
+              }
+              const int k0 = kb * kBK;
+              unsigned sb = at + kABytes;
+              if (MODE == kDw) {
+                const int r = o.r0 + k0;
+                if (p.a2) {
+                  load4(at, &p.ta, 0, r, f >> 6, pm, bar);
+                } else {
+                  load4(at, &p.ta, f, r, pm, 0, bar);
+                  load4(at + 8192u, &p.ta, f + 64, r, pm, 0, bar);
+                }
+                if (p.b2) {
+                  load4(sb, &p.tb, 0, r, c >> 6, pn, bar);
+                } else {
+                  load4(sb, &p.tb, c, r, pn, 0, bar);
+                  if (boxes > 1) load4(sb + 8192u, &p.tb, c + 64, r, pn, 0, bar);
+                }
+              } else {
+                const int e = pm * p.experts + o.expert;
+                if (MODE == kForwardT) {
+                  load4(at, &p.ta, k0, f, e, 0, bar);
+                } else if (p.a2) {
+                  load4(at, &p.ta, 0, k0, f >> 6, e, bar);
+                } else {
+                  load4(at, &p.ta, f, k0, e, 0, bar);
+                  load4(at + 8192u, &p.ta, f + 64, k0, e, 0, bar);
+                }
+                load4(sb, &p.tb, k0, tok, pn, 0, bar);
+                for (int i = 1; i < boxes; ++i) {
+                  sb += box;
+                  load4(sb, &p.tb, k0, tok + i * p.box, pn, 0, bar);
+                }
+              }
+            }
+            __syncwarp();
+            st += 8;
+            at += kStageBytes;
+            if (st == 8 * kStages) {
+              st = 0;
+              at = ring;
+              phase ^= 1u;
+            }
           }
-          const int k0 = in.kb * kBK;
-          unsigned sb = at + kABytes;
-          if (MODE == kDw) {
-            const int r = o.r0 + k0;
-            if (p.a2) {
-              load4(at, &p.ta, 0, r, f >> 6, pm, bar);
-            } else {
-              load4(at, &p.ta, f, r, pm, 0, bar);
-              load4(at + 8192u, &p.ta, f + 64, r, pm, 0, bar);
-            }
-            if (p.b2) {
-              load4(sb, &p.tb, 0, r, c >> 6, pn, bar);
-            } else {
-              load4(sb, &p.tb, c, r, pn, 0, bar);
-              if (boxes > 1) load4(sb + 8192u, &p.tb, c + 64, r, pn, 0, bar);
-            }
-          } else {
-            const int e = pm * p.experts + o.expert;
-            if (MODE == kForwardT) {
-              load4(at, &p.ta, k0, f, e, 0, bar);
-            } else if (p.a2) {
-              load4(at, &p.ta, 0, k0, f >> 6, e, bar);
-            } else {
-              load4(at, &p.ta, f, k0, e, 0, bar);
-              load4(at + 8192u, &p.ta, f + 64, k0, e, 0, bar);
-            }
-            load4(sb, &p.tb, k0, tok, pn, 0, bar);
-            for (int i = 1; i < boxes; ++i) {
-              sb += box;
-              load4(sb, &p.tb, k0, tok + i * p.box, pn, 0, bar);
-            }
-          }
-        }
-        __syncwarp();
-        st += 8;
-        at += kStageBytes;
-        if (st == 8 * kStages) {
-          st = 0;
-          at = ring;
-          phase ^= 1u;
-        }
-      }
+        a = z;
+      } while (a < o.b1);
     }
   } else if (warp == 1) {
     if (rank == 0) {
@@ -749,92 +754,144 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
       const unsigned accf0 = tc2::peer_addr(&s.accf[0], 0), accf1 = tc2::peer_addr(&s.accf[0], 1);
       unsigned st = 0, phase = 0, it = 0;
       u64 a = a0, bd = b0;
-      for (unsigned t = pair; t < tiles; t += pairs, ++it) {
+      for (unsigned t = pair; t < tiles; t += pairs) {
         const Tile o = tile_at<MODE>(p, s.g, t);
-        const unsigned ab = it & 1u, d = tmem + ab * kTok;
         const unsigned idesc = base | ((unsigned)(o.nn >> 3) << 17);
-        wait(acce + 8 * ab, ((it >> 1) & 1u) ^ 1u);
-        tc::fence_after();
-        Step in(o);
-        for (int b = o.b0; b < o.b1; ++b, in.next(o)) {
-          wait(full + st, phase);
+        int from = o.b0;
+        do {
+          const int to = chunk_end<WIDE>(from, o.b1);
+          const unsigned ab = it & 1u, d = tmem + ab * kTok;
+          wait(acce + 8 * ab, ((it >> 1) & 1u) ^ 1u);
           tc::fence_after();
-          if (one) {
-            if (clears<MODE>(o, in)) {
-              const int kks = (o.r1 - o.r0 - in.kb * kBK + 15) / 16;
-              for (int kk = 0; kk < kks; ++kk) mma(d, a + kk * desc_step<amn>(), bd + kk * desc_step<bmn>(), idesc, b > o.b0 || kk > 0 ? 1u : 0u);
-            } else {
+          for (int term = 0; term < terms<WIDE>(); ++term)
+            for (int kb = from; kb < to; ++kb) {
+              const unsigned more = term > 0 || kb > from ? 1u : 0u;
+              wait(full + st, phase);
+              tc::fence_after();
+              if (one) {
+                if (clears<MODE>(o, kb)) {
+                  const int kks = (o.r1 - o.r0 - kb * kBK + 15) / 16;
+                  for (int kk = 0; kk < kks; ++kk) mma(d, a + kk * desc_step<amn>(), bd + kk * desc_step<bmn>(), idesc, kk > 0 ? 1u : more);
+                } else {
 #pragma unroll
-              for (int kk = 0; kk < kBK / 16; ++kk) mma(d, a + kk * desc_step<amn>(), bd + kk * desc_step<bmn>(), idesc, b > o.b0 || kk > 0 ? 1u : 0u);
+                  for (int kk = 0; kk < kBK / 16; ++kk) mma(d, a + kk * desc_step<amn>(), bd + kk * desc_step<bmn>(), idesc, kk > 0 ? 1u : more);
+                }
+                commit(empty0 + st);
+                commit(empty1 + st);
+              }
+              __syncwarp();
+              st += 8;
+              a += kStageBytes >> 4;
+              bd += kStageBytes >> 4;
+              if (st == 8 * kStages) {
+                st = 0;
+                a = a0;
+                bd = b0;
+                phase ^= 1u;
+              }
             }
-            commit(empty0 + st);
-            commit(empty1 + st);
+          if (one) {
+            commit(accf0 + 8 * ab);
+            commit(accf1 + 8 * ab);
           }
           __syncwarp();
-          st += 8;
-          a += kStageBytes >> 4;
-          bd += kStageBytes >> 4;
-          if (st == 8 * kStages) {
-            st = 0;
-            a = a0;
-            bd = b0;
-            phase ^= 1u;
-          }
-        }
-        if (one) {
-          commit(accf0 + 8 * ab);
-          commit(accf1 + 8 * ab);
-        }
-        __syncwarp();
+          ++it;
+          from = to;
+        } while (from < o.b1);
       }
     }
   } else if (warp < 2 + kDrain) {
     const int q = warp & 3, other = (warp - 2) >> 2;  // its quarter of the lanes; every other 32 columns
     unsigned it = 0;
-    for (unsigned t = pair; t < tiles; t += pairs, ++it) {
+    for (unsigned t = pair; t < tiles; t += pairs) {
       const Tile o = tile_at<MODE>(p, s.g, t);
-      const unsigned ab = it & 1u, aph = (it >> 1) & 1u;
       const int f = o.f0 + (int)rank * 128 + q * 32;
       const int count = MODE == kDw ? min(p.k - o.c0, o.nn) : o.r1 - o.r0;
       TO* out = static_cast<TO*>(p.out) + o.split * p.split_stride + f + (MODE == kDw ? o.expert * p.oe + (i64)o.c0 * p.os : (i64)o.r0 * p.os);
-      const unsigned buf = smem_u32(s.out[warp - 2]);
-      const unsigned acc = tmem + ((unsigned)(q * 32) << 16) + ab * kTok;
-      wait(accf + 8 * ab, aph);
-      __syncwarp();
-      tc::fence_after();
-      if (f < p.n) {
-        for (int c = 32 * other; c < count; c += 32 * (kDrain / 4)) {
-          if constexpr (sizeof(TO) == 2)
-            drain16<TO>(acc + c, o.b0 >= o.b1, buf, out + c * p.os, p.os, count - c, p.n - f, p.vec, lane);
-          else
-            drain32(acc + c, o.b0 >= o.b1, out + c * p.os, p.os, count - c, p.n - f, lane);
+      const unsigned acc0 = tmem + ((unsigned)(q * 32) << 16);
+      if constexpr (WIDE) {
+        float sum[kTok / 64][32];
+#pragma unroll
+        for (int g = 0; g < kTok / 64; ++g)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sum[g][i] = 0.0f;
+        int a = o.b0;
+        do {
+          const unsigned ab = it & 1u;
+          wait(accf + 8 * ab, (it >> 1) & 1u);
           __syncwarp();
+          tc::fence_after();
+          if (f < p.n && a < o.b1) {
+#pragma unroll
+            for (int g = 0; g < kTok / 64; ++g) {
+              const int c = 32 * other + 64 * g;
+              if (c < count) {
+                float v[32];
+                __syncwarp();
+                tc::ld32(acc0 + ab * kTok + c, v);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) sum[g][i] += v[i];
+              }
+            }
+          }
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_relaxed(lead_acce + 8 * ab);
+          ++it;
+          a = chunk_end<WIDE>(a, o.b1);
+        } while (a < o.b1);
+        if (f < p.n) {
+#pragma unroll
+          for (int g = 0; g < kTok / 64; ++g) {
+            const int c = 32 * other + 64 * g;
+            if (c < count) store32(sum[g], out + c * p.os, p.os, count - c, p.n - f, lane);
+          }
         }
+      } else {
+        const unsigned ab = it & 1u;
+        wait(accf + 8 * ab, (it >> 1) & 1u);
+        __syncwarp();
+        tc::fence_after();
+        if (f < p.n) {
+          for (int c = 32 * other; c < count; c += 32 * (kDrain / 4)) {
+            if constexpr (sizeof(TO) == 2)
+              drain16<TO>(acc0 + ab * kTok + c, o.b0 >= o.b1, smem_u32(s.out[warp - 2]), out + c * p.os, p.os, count - c, p.n - f, p.vec, lane);
+            else
+              drain32(acc0 + ab * kTok + c, o.b0 >= o.b1, out + c * p.os, p.os, count - c, p.n - f, lane);
+            __syncwarp();
+          }
+        }
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_relaxed(lead_acce + 8 * ab);
+        ++it;
       }
-      tc::fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_relaxed(lead_acce + 8 * ab);
     }
   } else if (MODE == kDw) {
     // a lane has one 16-byte piece of each row: two 64-wide blocks of the M side, then the N side's
     unsigned stage = 0, phases = 0;  // bit i: parity of part[i]
     for (unsigned t = pair; t < tiles; t += pairs) {
       const Tile o = tile_at<MODE>(p, s.g, t);
-      Step in(o);
-      for (int b = o.b0; b < o.b1; ++b, in.next(o)) {
-        if (clears<MODE>(o, in)) {
-          wait(part + 8 * stage, (phases >> stage) & 1u);
-          __syncwarp();
-          phases ^= 1u << stage;
-          const int left = o.r1 - o.r0 - in.kb * kBK, to = (left + 15) & ~15;
-          uint4* at = reinterpret_cast<uint4*>(smem + pad + stage * kStageBytes + (lane >> 3) * 8192 + (lane & 7) * 16);
-          for (int r = left; r < to; ++r) at[r * 8] = make_uint4(0, 0, 0, 0);
-          asm volatile("fence.proxy.async;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) arrive(lead_full + 8 * stage);
-        }
-        stage = stage + 1 == kStages ? 0 : stage + 1;
-      }
+      int a = o.b0;
+      do {
+        const int z = chunk_end<WIDE>(a, o.b1);
+        for (int term = 0; term < terms<WIDE>(); ++term)
+          for (int kb = a; kb < z; ++kb) {
+            if (clears<MODE>(o, kb)) {
+              wait(part + 8 * stage, (phases >> stage) & 1u);
+              __syncwarp();
+              phases ^= 1u << stage;
+              const int left = o.r1 - o.r0 - kb * kBK, to = (left + 15) & ~15;
+              uint4* at = reinterpret_cast<uint4*>(smem + pad + stage * kStageBytes + (lane >> 3) * 8192 + (lane & 7) * 16);
+              for (int r = left; r < to; ++r) at[r * 8] = make_uint4(0, 0, 0, 0);
+              asm volatile("fence.proxy.async;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) arrive(lead_full + 8 * stage);
+            }
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+          }
+        a = z;
+      } while (a < o.b1);
     }
   }
   tc::fence_before();
@@ -879,17 +936,17 @@ bool encode(ccb::TmaDesc* out, int format, const void* base, int rank, const i64
                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class TO, int MODE>
+template <class TO, int MODE, bool WIDE = false>
 int go(const P& p, int sms, cudaStream_t st, const char* me) {
   static bool ready[64];  // the kernel's shared-memory limit was raised on the device
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !__atomic_load_n(&ready[dev], __ATOMIC_RELAXED)) {
-    const cudaError_t e = cudaFuncSetAttribute(grouped_tc<TO, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(grouped_tc<TO, MODE, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return fail(CCB_ERR_DRIVER, me, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) __atomic_store_n(&ready[dev], true, __ATOMIC_RELAXED);
   }
-  grouped_tc<TO, MODE><<<(unsigned)(sms & ~1), kThreads, kSmem, st>>>(p);
+  grouped_tc<TO, MODE, WIDE><<<(unsigned)(sms & ~1), kThreads, kSmem, st>>>(p);
   return launched(me);
 }
 }  // namespace tcg
@@ -1106,7 +1163,6 @@ tcg::P tensor_params(const Plan& plan, const int* off, unsigned* err, int dtype,
   p.k = (int)k;
   p.splits = plan.parts;
   p.format = dtype != CCB_F16;
-  p.terms = dtype == CCB_F32 ? 6 : 1;
   return p;
 }
 
@@ -1139,10 +1195,12 @@ int tensor_forward(const ccb_nn_grouped_matmul_t* a, Plan plan, int sms, cudaStr
     p.os = a->n;
     p.split_stride = plan.result;
   }
-  if (parts || a->dtype == CCB_F32) {
+  if (a->dtype == CCB_F32) {
+    if (const int rc = a->transpose_w ? tcg::go<float, tcg::kForwardT, true>(p, sms, st, me) : tcg::go<float, tcg::kForward, true>(p, sms, st, me)) return rc;
+    return parts ? sum_parts(p, (float*)a->out, a->rows, a->n, a->out_stride, 1, 0, sms, st, me) : CCB_OK;
+  }
+  if (parts) {
     if (const int rc = a->transpose_w ? tcg::go<float, tcg::kForwardT>(p, sms, st, me) : tcg::go<float, tcg::kForward>(p, sms, st, me)) return rc;
-    if (!parts) return CCB_OK;
-    if (a->dtype == CCB_F32) return sum_parts(p, (float*)a->out, a->rows, a->n, a->out_stride, 1, 0, sms, st, me);
     return p.format ? sum_parts(p, (__nv_bfloat16*)a->out, a->rows, a->n, a->out_stride, 1, 0, sms, st, me)
                     : sum_parts(p, (__half*)a->out, a->rows, a->n, a->out_stride, 1, 0, sms, st, me);
   }
@@ -1194,7 +1252,7 @@ int tensor_dw(const ccb_nn_grouped_matmul_dw_t* a, Plan plan, int sms, cudaStrea
     p.split_stride = plan.result;
   }
   if (parts || a->out_dtype == CCB_F32) {
-    if (const int rc = tcg::go<float, tcg::kDw>(p, sms, st, me)) return rc;
+    if (const int rc = a->dtype == CCB_F32 ? tcg::go<float, tcg::kDw, true>(p, sms, st, me) : tcg::go<float, tcg::kDw>(p, sms, st, me)) return rc;
     if (!parts) return CCB_OK;
     if (a->out_dtype == CCB_F32) return sum_parts(p, (float*)a->out, a->k, a->n, a->out_row_stride, a->experts, a->out_stride, sms, st, me);
     return p.format ? sum_parts(p, (__nv_bfloat16*)a->out, a->k, a->n, a->out_row_stride, a->experts, a->out_stride, sms, st, me)
