@@ -164,36 +164,44 @@ __device__ __forceinline__ void philox_round(const Drop& d, int i, unsigned& c0,
   c2 = (unsigned)(a >> 32) ^ c3 ^ d.key[2 * i + 1];
   c3 = (unsigned)a;
 }
-__device__ __forceinline__ void philox4(const Drop& d, u64 q, unsigned* w) {
-  unsigned c0, c1, c2, c3;
+// N blocks from q on, round by round: their products do not wait for one another.
+template <int N>
+__device__ __forceinline__ void philox(const Drop& d, u64 q, unsigned* w) {
+  unsigned c[N][4];
   if (d.same) {
-    const u64 a = (u64)0xD2511F53u * (unsigned)q;
-    const u64 b = (u64)0xCD9E8D57u * ((unsigned)(a >> 32) ^ d.c2);
-    c0 = (unsigned)(b >> 32) ^ d.c0;
-    c1 = (unsigned)b;
-    c2 = (unsigned)a ^ d.hi;
-    c3 = d.c3;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const u64 a = (u64)0xD2511F53u * (unsigned)(q + n);
+      const u64 b = (u64)0xCD9E8D57u * ((unsigned)(a >> 32) ^ d.c2);
+      c[n][0] = (unsigned)(b >> 32) ^ d.c0;
+      c[n][1] = (unsigned)b;
+      c[n][2] = (unsigned)a ^ d.hi;
+      c[n][3] = d.c3;
+    }
   } else {
-    c0 = (unsigned)q;
-    c1 = (unsigned)(q >> 32);
-    c2 = (unsigned)d.offset;
-    c3 = (unsigned)(d.offset >> 32);
-    philox_round(d, 0, c0, c1, c2, c3);
-    philox_round(d, 1, c0, c1, c2, c3);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      c[n][0] = (unsigned)(q + n);
+      c[n][1] = (unsigned)((q + n) >> 32);
+      c[n][2] = (unsigned)d.offset;
+      c[n][3] = (unsigned)(d.offset >> 32);
+      philox_round(d, 0, c[n][0], c[n][1], c[n][2], c[n][3]);
+      philox_round(d, 1, c[n][0], c[n][1], c[n][2], c[n][3]);
+    }
   }
 #pragma unroll
-  for (int i = 2; i < 10; ++i) philox_round(d, i, c0, c1, c2, c3);
-  w[0] = c0;
-  w[1] = c1;
-  w[2] = c2;
-  w[3] = c3;
+  for (int i = 2; i < 10; ++i)
+#pragma unroll
+    for (int n = 0; n < N; ++n) philox_round(d, i, c[n][0], c[n][1], c[n][2], c[n][3]);
+#pragma unroll
+  for (int i = 0; i < 4 * N; ++i) w[i] = c[i >> 2][i & 3];
 }
+__device__ __forceinline__ void philox4(const Drop& d, u64 q, unsigned* w) { philox<1>(d, q, w); }
 // The words of the 8 elements from e0 on: two blocks, or three where the index
 // is no multiple of 4.
 __device__ __forceinline__ void philox8(const Drop& d, u64 e0, unsigned* w) {
   const u64 q = e0 >> 2;
-  philox4(d, q, w);
-  philox4(d, q + 1, w + 4);
+  philox<2>(d, q, w);
   const int shift = (int)(e0 & 3);
   if (shift) {
     unsigned x[4];
