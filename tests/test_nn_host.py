@@ -163,3 +163,11 @@ def test_empty_tensors_need_no_device():
     nn.grouped_matmul(A(0, 8), A(3, 8, 5), A(4, dtype="i32"), A(0, 5))
     nn.grouped_matmul_dw(A(6, 0), A(6, 5), A(4, dtype="i32"), A(3, 0, 5))
     assert struct.calcsize("P") == 8
+
+
+def test_expert_block_graphs_lower_to_one_launch_each():
+    from cudacaml_b200 import backend_cuda as B
+    from cudacaml_b200 import expert_block as E
+
+    for g in (E.activation((24, 40)), E.activation_grad((24, 40)), E.squared_error((24, 16)), E.descent((3, 16, 40), 0.1)):
+        assert B.lower_info(g)["launches"] == 1
