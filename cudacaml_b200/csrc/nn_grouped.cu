@@ -22,14 +22,6 @@ struct GroupP {
   i64 k, n, xs, we, ws, os;
   int rows, experts;
 };
-struct GroupDwP {
-  const void *x, *dy;
-  const int* off;
-  void* out;
-  unsigned* err;
-  i64 k, n, xs, ys, oe, os;
-  int rows, experts;
-};
 
 // Row ranges and their tiles of `bm` rows. Segment s in [1, experts] is
 // expert s - 1; segments 0 and experts + 1 are the rows that belong to none.
@@ -100,95 +92,27 @@ __device__ __forceinline__ int segment_of(const Segments& g, int segs, int t) {
   return lo;
 }
 
-// ------------------------------------------------- CUDA cores, any alignment
-// 64 x 64 tiles, 16 of the contraction at a time, 4 x 4 results a thread.
-constexpr int kB = 64, kK = 16;
-
-__device__ __forceinline__ void simt_step(const float (*a)[kB + 4], const float (*b)[kB + 4], float acc[4][4], int tx, int ty) {
-#pragma unroll
-  for (int k = 0; k < kK; ++k) {
-    float av[4], bv[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) av[i] = a[k][ty * 4 + i];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) bv[j] = b[k][tx * 4 + j];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
+// ------------------------------------------------- nothing to contract over
+// Zeros, and the offsets' check.
+template <class T>
+__global__ void __launch_bounds__(256) clear_out(T* out, i64 mats, i64 rows, i64 cols, i64 oe, i64 os, const int* off, int experts, int tokens, unsigned* err) {
+  __shared__ Segments g;
+  if (blockIdx.x == 0) lay_out(g, off, experts, tokens, 256, err);
+  const i64 each = rows * cols;
+  for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < mats * each; i += (i64)gridDim.x * 256) {
+    const i64 m = i / each, r = (i - m * each) / cols;
+    out[m * oe + r * os + (i - m * each - r * cols)] = from_f<T>(0.0f);
   }
 }
-
-template <class T, bool WT>
-__global__ void __launch_bounds__(256) grouped_any(const __grid_constant__ GroupP p) {
-  __shared__ Segments g;
-  __shared__ float sa[kK][kB + 4], sb[kK][kB + 4];
-  lay_out(g, p.off, p.experts, p.rows, kB, p.err);
-  const int segs = p.experts + 2, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const i64 nt = (p.n + kB - 1) / kB, total = nt * g.tile[segs];
-  const T* x = static_cast<const T*>(p.x);
-  for (i64 t = blockIdx.x; t < total; t += gridDim.x) {
-    const int mt = (int)(t / nt);
-    const i64 n0 = (t % nt) * kB;
-    const int s = segment_of(g, segs, mt);
-    const int r0 = g.row[s] + (mt - g.tile[s]) * kB, r1 = min(g.row[s + 1], r0 + kB);
-    float acc[4][4] = {};
-    if (s >= 1 && s <= p.experts) {
-      const T* w = static_cast<const T*>(p.w) + (s - 1) * p.we;
-      for (i64 k0 = 0; k0 < p.k; k0 += kK) {
-        for (int i = threadIdx.x; i < kB * kK; i += 256) {
-          const int m = i / kK, k = i % kK;
-          sa[k][m] = r0 + m < r1 && k0 + k < p.k ? to_f<T>(x[(i64)(r0 + m) * p.xs + k0 + k]) : 0.0f;
-        }
-        for (int i = threadIdx.x; i < kB * kK; i += 256) {
-          const int k = WT ? i % kK : i / kB, n = WT ? i / kK : i % kB;
-          sb[k][n] = n0 + n < p.n && k0 + k < p.k ? to_f<T>(w[WT ? (n0 + n) * p.ws + k0 + k : (k0 + k) * p.ws + n0 + n]) : 0.0f;
-        }
-        __syncthreads();
-        simt_step(sa, sb, acc, tx, ty);
-        __syncthreads();
-      }
-    }
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j) {
-        const i64 r = r0 + ty * 4 + i, c = n0 + tx * 4 + j;
-        if (r < r1 && c < p.n) static_cast<T*>(p.out)[r * p.os + c] = from_f<T>(acc[i][j]);
-      }
-  }
-}
-
-template <class T, class TO>
-__global__ void __launch_bounds__(256) grouped_dw_any(const __grid_constant__ GroupDwP p) {
-  __shared__ Segments g;
-  __shared__ float sa[kK][kB + 4], sb[kK][kB + 4];
-  lay_out(g, p.off, p.experts, p.rows, kB, p.err);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const i64 kt = (p.k + kB - 1) / kB, nt = (p.n + kB - 1) / kB, total = kt * nt * p.experts;
-  const T* x = static_cast<const T*>(p.x);
-  const T* dy = static_cast<const T*>(p.dy);
-  for (i64 t = blockIdx.x; t < total; t += gridDim.x) {
-    const int e = (int)(t / (kt * nt));
-    const i64 m0 = (t / nt % kt) * kB, n0 = (t % nt) * kB;
-    const int r1 = g.row[e + 2];
-    float acc[4][4] = {};
-    for (i64 r0 = g.row[e + 1]; r0 < r1; r0 += kK) {
-      for (int i = threadIdx.x; i < kB * kK; i += 256) {
-        const int k = i / kB, c = i % kB;
-        const bool in = r0 + k < r1;
-        sa[k][c] = in && m0 + c < p.k ? to_f<T>(x[(r0 + k) * p.xs + m0 + c]) : 0.0f;
-        sb[k][c] = in && n0 + c < p.n ? to_f<T>(dy[(r0 + k) * p.ys + n0 + c]) : 0.0f;
-      }
-      __syncthreads();
-      simt_step(sa, sb, acc, tx, ty);
-      __syncthreads();
-    }
-    TO* out = static_cast<TO*>(p.out) + e * p.oe;
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j) {
-        const i64 r = m0 + ty * 4 + i, c = n0 + tx * 4 + j;
-        if (r < p.k && c < p.n) out[r * p.os + c] = from_f<TO>(acc[i][j]);
-      }
-  }
+int clear(int dtype, void* out, i64 mats, i64 rows, i64 cols, i64 oe, i64 os, const int* off, i64 experts, i64 tokens, unsigned* err, int sms, cudaStream_t st,
+          const char* me) {
+  const i64 work = (mats * rows * cols + 255) / 256, most = (i64)sms * 8;
+  const unsigned grid = (unsigned)(work < most ? work : most);
+  if (dtype == CCB_F32)
+    clear_out<<<grid, 256, 0, st>>>(static_cast<float*>(out), mats, rows, cols, oe, os, off, (int)experts, (int)tokens, err);
+  else  // the two 16-bit zeros are the same
+    clear_out<<<grid, 256, 0, st>>>(static_cast<__half*>(out), mats, rows, cols, oe, os, off, (int)experts, (int)tokens, err);
+  return launched(me);
 }
 
 // ------------------------------------- CUDA cores, few rows an expert, any alignment
@@ -325,21 +249,6 @@ void few(const FewP& q, bool wt, int sms, cudaStream_t st) {
     grouped_few<T, TO, true><<<grid, kFewThreads, 0, st>>>(q);
   else
     grouped_few<T, TO, false><<<grid, kFewThreads, 0, st>>>(q);
-}
-
-template <class T>
-void any(const GroupP& p, bool wt, int sms, cudaStream_t st) {
-  const i64 tiles = ((p.rows + kB - 1) / kB + p.experts + 1) * ((p.n + kB - 1) / kB), most = (i64)sms * 4;
-  const unsigned grid = (unsigned)(tiles < most ? tiles : most);
-  if (wt)
-    grouped_any<T, true><<<grid, 256, 0, st>>>(p);
-  else
-    grouped_any<T, false><<<grid, 256, 0, st>>>(p);
-}
-template <class T, class TO>
-void any_dw(const GroupDwP& p, int sms, cudaStream_t st) {
-  const i64 tiles = ((p.k + kB - 1) / kB) * ((p.n + kB - 1) / kB) * p.experts, most = (i64)sms * 4;
-  grouped_dw_any<T, TO><<<(unsigned)(tiles < most ? tiles : most), 256, 0, st>>>(p);
 }
 
 // ------------------------------------------------------------ tensor cores
@@ -894,6 +803,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
       } while (a < o.b1);
     }
   }
+  if (wait.limit < MBAR_SPIN_LIMIT)  // a wait ran out: copies may be on their way yet
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  __syncwarp();
   tc::fence_before();
   __syncthreads();
   tc2::cluster_sync();
@@ -902,15 +814,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-// The sum of the parts of a divided contraction, in order.
-template <class TO>
-__global__ void __launch_bounds__(256) add_parts(const float* part, i64 stride, int parts, TO* out, i64 rows_, i64 cols, i64 os, i64 mats, i64 oe) {
-  const i64 each = rows_ * cols, total = mats * each;
+// The sum of the parts of a divided contraction, in order: four results a
+// thread, of one row of `out` (cols a multiple of 4, or one at a time).
+template <class TO, int N>
+__global__ void __launch_bounds__(256) add_parts(const float* part, i64 stride, int parts, TO* out, i64 rows, i64 cols, i64 os, i64 mats, i64 oe) {
+  const i64 each = rows * cols, total = mats * each / N;
   for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < total; i += (i64)gridDim.x * 256) {
-    float v = 0.0f;
-    for (int s = 0; s < parts; ++s) v += part[s * stride + i];
-    const i64 m = i / each, r = (i - m * each) / cols, c = i - m * each - r * cols;
-    out[m * oe + r * os + c] = from_f<TO>(v);
+    float v[N] = {};
+    const float* at = part + i * N;
+    for (int s = 0; s < parts; ++s, at += stride) {
+      if constexpr (N == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(at);
+        v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w;
+      } else {
+        v[0] += *at;
+      }
+    }
+    const i64 e = i * N;
+    i64 to = e;
+    if (os != cols || (mats > 1 && oe != each)) {
+      const i64 m = e / each, r = (e - m * each) / cols;
+      to = m * oe + r * os + (e - m * each - r * cols);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[to + j] = from_f<TO>(v[j]);
   }
 }
 
@@ -952,7 +879,7 @@ int go(const P& p, int sms, cudaStream_t st, const char* me) {
 }  // namespace tcg
 
 std::string check_sizes(i64 rows, i64 experts, i64 k, i64 n, int dtype) {
-  if (rows < 0 || rows > INT_MAX) return "rows must be in [0, 2^31)";
+  if (rows < 0 || rows > INT_MAX - 1024) return "rows must be in [0, 2^31 - 1025]";
   if (experts < 1 || experts > kMaxExperts) return "experts must be in [1, " + std::to_string(kMaxExperts) + "]";
   if (k < 0 || n < 0 || k > INT_MAX || n > INT_MAX) return "k and n must be in [0, 2^31)";
   if (!float_type(dtype)) return "dtype code " + std::to_string(dtype) + " (0 f32, 4 bf16, 5 f16)";
@@ -997,20 +924,30 @@ std::string check_dw(const ccb_nn_grouped_matmul_dw_t* a) {
 // the number itself and no plane rounds up past the largest), and 16-bit ones
 // whose rows are not aligned, copied. Rows of a plane are dense but for the
 // last 16 bytes. A number that is not finite is its first plane alone.
+struct PackP {
+  const void* in;
+  unsigned short* out;
+  i64 stride, row_stride, mats, rows;
+  unsigned cols, ld;
+};
+struct PackBoth {
+  PackP p[2];
+};
 template <class T>
-__global__ void __launch_bounds__(256) pack_planes(const T* in, i64 stride, i64 row_stride, unsigned short* out, i64 mats, i64 rows, unsigned cols, unsigned ld) {
-  const unsigned pieces = ld / 8;
-  const i64 total = mats * rows * pieces, plane = mats * rows * ld;
+__global__ void __launch_bounds__(256) pack_planes(const __grid_constant__ PackBoth both) {
+  const PackP& q = both.p[blockIdx.y];
+  const unsigned pieces = q.ld / 8;
+  const i64 total = q.mats * q.rows * pieces, plane = q.mats * q.rows * q.ld;
   for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < total; i += (i64)gridDim.x * 256) {
-    const i64 row = i / pieces, m = row / rows;
+    const i64 row = i / pieces, m = q.mats == 1 ? 0 : row / q.rows;
     const unsigned c = (unsigned)(i - row * pieces) * 8;
-    const T* p = in + m * stride + (row - m * rows) * row_stride + c;
-    unsigned short* o = out + row * ld + c;
+    const T* p = static_cast<const T*>(q.in) + m * q.stride + (row - m * q.rows) * q.row_stride + c;
+    unsigned short* o = q.out + row * q.ld + c;
     if constexpr (sizeof(T) == 4) {
-      unsigned short v[3][8];
+      alignas(16) unsigned short v[3][8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float x = c + j < cols ? (float)p[j] : 0.0f;
+        const float x = c + j < q.cols ? (float)p[j] : 0.0f;
         const float hi = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
         const bool fine = (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u;
         const float r = fine ? x - hi : 0.0f, mid = __uint_as_float(__float_as_uint(r) & 0xFFFF0000u), lo = r - mid;
@@ -1022,9 +959,9 @@ __global__ void __launch_bounds__(256) pack_planes(const T* in, i64 stride, i64 
 #pragma unroll
       for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(o + k * plane) = *reinterpret_cast<const uint4*>(v[k]);
     } else {
-      unsigned short v[8];
+      alignas(16) unsigned short v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? reinterpret_cast<const unsigned short*>(p)[j] : (unsigned short)0;
+      for (int j = 0; j < 8; ++j) v[j] = c + j < q.cols ? reinterpret_cast<const unsigned short*>(p)[j] : (unsigned short)0;
       *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(v);
     }
   }
@@ -1049,20 +986,30 @@ Operand operand(int dtype, const void* p, i64 mats, i64 rows, i64 cols, i64 stri
   o.packs = dtype == CCB_F32 || !lies_well(p, mats, rows, stride, row_stride);
   return o;
 }
-// Packs the operand into `room` if it has to be (and moves `room` on).
-int settle(Operand* o, int dtype, char** room, int sms, cudaStream_t st, const char* me) {
-  if (!o->packs) return CCB_OK;
-  const i64 ld = o->ld(), work = ceil_div(o->mats * o->rows * (ld / 8), 256), most = (i64)sms * 16;
-  const unsigned grid = (unsigned)(work < most ? work : most);
-  unsigned short* out = reinterpret_cast<unsigned short*>(*room);
+// Packs the operands that have to be into `room` (and moves it on), in one launch.
+int settle(Operand* a, Operand* b, int dtype, char** room, int sms, cudaStream_t st, const char* me) {
+  PackBoth both = {};
+  int n = 0;
+  i64 work = 0;
+  for (Operand* o : {a, b}) {
+    if (!o->packs) continue;
+    const i64 ld = o->ld();
+    PackP& q = both.p[n++];
+    q = {o->p, reinterpret_cast<unsigned short*>(*room), o->stride, o->row_stride, o->mats, o->rows, (unsigned)o->cols, (unsigned)ld};
+    const i64 w = ceil_div(o->mats * o->rows * (ld / 8), 256);
+    work = w > work ? w : work;
+    *room += o->bytes();
+    o->p = q.out;
+    o->row_stride = ld;
+    o->stride = o->rows * ld;
+  }
+  if (n == 0) return CCB_OK;
+  const i64 most = (i64)sms * 16;
+  const dim3 grid((unsigned)(work < most ? work : most), (unsigned)n);
   if (dtype == CCB_F32)
-    pack_planes<float><<<grid, 256, 0, st>>>(static_cast<const float*>(o->p), o->stride, o->row_stride, out, o->mats, o->rows, (unsigned)o->cols, (unsigned)ld);
+    pack_planes<float><<<grid, 256, 0, st>>>(both);
   else
-    pack_planes<__half><<<grid, 256, 0, st>>>(static_cast<const __half*>(o->p), o->stride, o->row_stride, out, o->mats, o->rows, (unsigned)o->cols, (unsigned)ld);
-  *room += o->bytes();
-  o->p = out;
-  o->row_stride = ld;
-  o->stride = o->rows * ld;
+    pack_planes<__half><<<grid, 256, 0, st>>>(both);
   return launched(me);
 }
 
@@ -1104,7 +1051,7 @@ Plan plan_of(const ccb_nn_grouped_matmul_t* a) {
   p.tensor = !p.w.packs || a->rows >= 16 * some;
   p.result = a->rows * a->n;
   if (!p.tensor) {  // two tiles for each of five blocks an SM, and no part above what shared memory takes
-    const i64 tiles = ceil_div(a->n, a->transpose_w ? kFewColsT : kFewCols) * (some + a->rows / kFewRows), most = ceil_div(a->k, a->transpose_w ? 512 : 64), least = ceil_div(a->k, kFewK);
+    const i64 tiles = ceil_div(a->n, a->transpose_w ? kFewColsT : kFewCols) * (some + a->rows / kFewRows), most = ceil_div(a->k, a->transpose_w ? 512 : 256 / type_bytes(a->dtype)), least = ceil_div(a->k, kFewK);
     const i64 want = ceil_div(10 * 148, tiles);
     p.parts = (int)(want < least ? least : want > most ? most : want);
     return p;
@@ -1132,8 +1079,14 @@ std::string check_workspace(const A* a, const Plan& p) {
 
 template <class TO>
 int sum_parts(const tcg::P& p, TO* out, i64 rows, i64 cols, i64 os, i64 mats, i64 oe, int sms, cudaStream_t st, const char* me) {
-  const i64 blocks = ceil_div(rows * cols * mats, 256), most = (i64)sms * 8;
-  tcg::add_parts<TO><<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(static_cast<const float*>(p.out), p.split_stride, p.splits, out, rows, cols, os, mats, oe);
+  const bool four = cols % 4 == 0 && p.split_stride % 4 == 0;
+  const i64 blocks = ceil_div(rows * cols * mats, four ? 1024 : 256), most = (i64)sms * 8;
+  const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+  const float* part = static_cast<const float*>(p.out);
+  if (four)
+    tcg::add_parts<TO, 4><<<grid, 256, 0, st>>>(part, p.split_stride, p.splits, out, rows, cols, os, mats, oe);
+  else
+    tcg::add_parts<TO, 1><<<grid, 256, 0, st>>>(part, p.split_stride, p.splits, out, rows, cols, os, mats, oe);
   return launched(me);
 }
 
@@ -1169,8 +1122,7 @@ tcg::P tensor_params(const Plan& plan, const int* off, unsigned* err, int dtype,
 int tensor_forward(const ccb_nn_grouped_matmul_t* a, Plan plan, int sms, cudaStream_t st, const char* me) {
   tcg::P p = tensor_params(plan, a->offsets, a->err, a->dtype, a->rows, a->experts, a->k, a->n);
   char* room = static_cast<char*>(a->workspace);
-  if (const int rc = settle(&plan.w, a->dtype, &room, sms, st, me)) return rc;
-  if (const int rc = settle(&plan.x, a->dtype, &room, sms, st, me)) return rc;
+  if (const int rc = settle(&plan.w, &plan.x, a->dtype, &room, sms, st, me)) return rc;
   // tokens come in boxes of about half of what an expert has on average: a
   // box is one copy, and a larger one than needed is read in vain
   const i64 mean = a->rows / (a->experts < a->rows ? a->experts : a->rows);
@@ -1235,8 +1187,7 @@ int few_forward(const ccb_nn_grouped_matmul_t* a, const Plan& plan, int sms, cud
 int tensor_dw(const ccb_nn_grouped_matmul_dw_t* a, Plan plan, int sms, cudaStream_t st, const char* me) {
   tcg::P p = tensor_params(plan, a->offsets, a->err, a->dtype, a->rows, a->experts, a->k, a->n);
   char* room = static_cast<char*>(a->workspace);
-  if (const int rc = settle(&plan.w, a->dtype, &room, sms, st, me)) return rc;
-  if (const int rc = settle(&plan.x, a->dtype, &room, sms, st, me)) return rc;
+  if (const int rc = settle(&plan.w, &plan.x, a->dtype, &room, sms, st, me)) return rc;
   if (!encode_mn(&p.tb, p.format, plan.x.p, a->k, a->rows, plan.x.planes, plan.x.row_stride, a->rows * plan.x.row_stride, &p.b2) ||
       !encode_mn(&p.ta, p.format, plan.w.p, a->n, a->rows, plan.w.planes, plan.w.row_stride, a->rows * plan.w.row_stride, &p.a2))
     return fail(CCB_ERR_DRIVER, me, "cuTensorMapEncodeTiled refused x or dy");
@@ -1305,14 +1256,7 @@ extern "C" int ccb_nn_grouped_matmul(const ccb_nn_grouped_matmul_t* a, void* str
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (plan.tensor) return tensor_forward(a, plan, sms, st, me);
     if (plan.parts > 0) return few_forward(a, plan, sms, st, me);
-    const GroupP p = {a->x, a->w, a->offsets, a->out, a->err, a->k, a->n, a->x_stride, a->w_stride, a->w_row_stride, a->out_stride, (int)a->rows, (int)a->experts};
-    if (a->dtype == CCB_F32)
-      any<float>(p, a->transpose_w, sms, st);
-    else if (a->dtype == CCB_BF16)
-      any<__nv_bfloat16>(p, a->transpose_w, sms, st);
-    else
-      any<__half>(p, a->transpose_w, sms, st);
-    return launched(me);
+    return clear(a->dtype, a->out, 1, a->rows, a->n, 0, a->out_stride, a->offsets, a->experts, a->rows, a->err, sms, st, me);
   })
 }
 
@@ -1332,17 +1276,6 @@ extern "C" int ccb_nn_grouped_matmul_dw(const ccb_nn_grouped_matmul_dw_t* a, voi
     if (const int rc = sm_count(me, &sms)) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (plan.tensor) return tensor_dw(a, plan, sms, st, me);
-    const GroupDwP p = {a->x, a->dy, a->offsets, a->out, a->err, a->k, a->n, a->x_stride, a->dy_stride, a->out_stride, a->out_row_stride, (int)a->rows, (int)a->experts};
-    if (a->dtype == CCB_F32)
-      any_dw<float, float>(p, sms, st);
-    else if (a->dtype == CCB_BF16 && a->out_dtype == CCB_F32)
-      any_dw<__nv_bfloat16, float>(p, sms, st);
-    else if (a->dtype == CCB_BF16)
-      any_dw<__nv_bfloat16, __nv_bfloat16>(p, sms, st);
-    else if (a->out_dtype == CCB_F32)
-      any_dw<__half, float>(p, sms, st);
-    else
-      any_dw<__half, __half>(p, sms, st);
-    return launched(me);
+    return clear(a->out_dtype, a->out, a->experts, a->k, a->n, a->out_stride, a->out_row_stride, a->offsets, a->experts, a->rows, a->err, sms, st, me);
   })
 }

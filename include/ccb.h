@@ -318,7 +318,10 @@ int ccb_nn_block_norm_backward_workspace(long long rows, long long cols, size_t*
  * experts + 1 i32 words in device memory, ascending, in [0, rows]: the host
  * never learns them. Words out of order or range are clamped and raise bit 64
  * of *err; a wait that ran out raises bit 16 (err may be NULL). Matrix e of w
- * starts w_stride * e elements in, its rows w_row_stride apart. The gradient
+ * starts w_stride * e elements in, its rows w_row_stride apart. At most 1024
+ * experts and 2^31 - 1025 rows. f32 products are sums of 16-bit products on the
+ * tensor cores, as exact as f32 arithmetic, but an infinite operand may give
+ * NaN where f32 arithmetic gives an infinity. The gradient
  * of x is the same call on dy with transpose_w flipped. Sums are in 32 bits,
  * the same bits in every run. workspace: at least
  * ccb_nn_grouped_matmul_workspace bytes, 16-byte aligned, uninitialised. */
