@@ -165,10 +165,11 @@ __device__ __forceinline__ void philox_round(const Drop& d, int i, unsigned& c0,
   c3 = (unsigned)a;
 }
 // N blocks from q on, round by round: their products do not wait for one another.
-template <int N>
+// SAME: d.same is known to hold.
+template <int N, bool SAME>
 __device__ __forceinline__ void philox(const Drop& d, u64 q, unsigned* w) {
   unsigned c[N][4];
-  if (d.same) {
+  if (SAME || d.same) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const u64 a = (u64)0xD2511F53u * (unsigned)(q + n);
@@ -196,16 +197,16 @@ __device__ __forceinline__ void philox(const Drop& d, u64 q, unsigned* w) {
 #pragma unroll
   for (int i = 0; i < 4 * N; ++i) w[i] = c[i >> 2][i & 3];
 }
-__device__ __forceinline__ void philox4(const Drop& d, u64 q, unsigned* w) { philox<1>(d, q, w); }
-// The words of the 8 elements from e0 on: two blocks, or three where the index
-// is no multiple of 4.
+__device__ __forceinline__ void philox4(const Drop& d, u64 q, unsigned* w) { philox<1, false>(d, q, w); }
+// The words of the 8 elements from e0 on, d.same: two blocks, or three where
+// the index is no multiple of 4.
 __device__ __forceinline__ void philox8(const Drop& d, u64 e0, unsigned* w) {
   const u64 q = e0 >> 2;
-  philox<2>(d, q, w);
+  philox<2, true>(d, q, w);
   const int shift = (int)(e0 & 3);
   if (shift) {
     unsigned x[4];
-    philox4(d, q + 2, x);
+    philox<1, true>(d, q + 2, x);
     for (int k = 0; k < shift; ++k) {
 #pragma unroll
       for (int i = 0; i < 7; ++i) w[i] = w[i + 1];

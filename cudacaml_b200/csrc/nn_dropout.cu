@@ -113,7 +113,7 @@ template <class T>
 void go(const DropoutP& p, int sms, cudaStream_t st) {
   const u64 n = (u64)p.rows * (u64)p.cols;
   const bool lines = p.rows == 1 || (p.cols % 8 == 0 && p.xs % 8 == 0 && p.os % 8 == 0 && (!p.res || p.rs % 8 == 0) && n / 8 < (1ull << 32));
-  if (lines && aligned(p.x, 16) && aligned(p.out, 16) && aligned(p.res, 16)) {
+  if (lines && (p.d.same || !p.d.on) && aligned(p.x, 16) && aligned(p.out, 16) && aligned(p.res, 16)) {
     const u64 total = n / 8, want = total / 256 + 1, most = (u64)sms * 16;
     dropout_wide<T><<<(unsigned)(want < most ? want : most), 256, 0, st>>>(p, (unsigned)(p.cols / 8), total);
     return;

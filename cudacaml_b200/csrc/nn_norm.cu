@@ -246,8 +246,8 @@ struct Forward {
     return true;
   }
   static bool by_width(const NormP& p, int sms, cudaStream_t st) {
-    if (!near({p.xs, p.bs, p.gs, p.ys, p.hs})) return false;
-    if (!wide(p.cols, {p.x, p.b, p.gate, p.y, p.h}, {p.xs, p.bs, p.gs, p.ys, p.hs})) return rows<false, 1>(p, sms, st);
+    if (!near({p.xs, p.bs, p.gs, p.ys, p.hs}) || (p.d.on && !p.d.same)) return false;
+    if ((p.d.base & 3) || !wide(p.cols, {p.x, p.b, p.gate, p.y, p.h}, {p.xs, p.bs, p.gs, p.ys, p.hs})) return rows<false, 1>(p, sms, st);
     // What a thread does once a row (its sums, addresses, copies) is some 300
     // instructions: 16 elements share them, fewer where a warp holds the row (32
     // would spill at the registers that three rows of 4096 leave). The shape goes

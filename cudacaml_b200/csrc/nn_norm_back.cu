@@ -410,8 +410,8 @@ struct Backward {
   // registers), so that a row's results do not either.
   template <bool MORE>
   static int by_width(const BackP& p, int sms, cudaStream_t st) {
-    if (!near({p.ys, p.dys, p.dhs, p.bs, p.gs, p.dxs, p.dbs, p.dgs})) return 0;
-    if (!wide(p.cols, {p.y, p.dy, p.dh, p.b, p.gate, p.dx, p.db, p.dgate}, {p.ys, p.dys, p.dhs, p.bs, p.gs, p.dxs, p.dbs, p.dgs}))
+    if (!near({p.ys, p.dys, p.dhs, p.bs, p.gs, p.dxs, p.dbs, p.dgs}) || (p.d.on && !p.d.same)) return 0;
+    if ((p.d.base & 3) || !wide(p.cols, {p.y, p.dy, p.dh, p.b, p.gate, p.dx, p.db, p.dgate}, {p.ys, p.dys, p.dhs, p.bs, p.gs, p.dxs, p.dbs, p.dgs}))
       return rows<false, 1, MORE>(p, sms, st);
     if (p.cols <= 256 || (sizeof(TX) == 4 && p.cols <= 4096)) return rows<true, 1, MORE>(p, sms, st);
     return rows<true, 2, MORE>(p, sms, st);

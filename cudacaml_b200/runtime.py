@@ -37,7 +37,7 @@ class CcbInvalid(CcbError, ValueError):
 def build(force: bool = False) -> str:
     """Compile libccb.so in place with the committed Makefile."""
     csrc = os.path.join(_HERE, "csrc")
-    args = ["make", "-s", "-C", csrc]
+    args = ["make", "-s", "-j4", "-C", csrc]
     if force:
         subprocess.run(args + ["clean"], check=True)
     subprocess.run(args, check=True)
