@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
   unsigned here = all;
   for (unsigned r = first; r < rows; r += step) {
     turn_ring<VEC>(g, ahead, fetch);
-    float y[PIECES][kE], t[1];
+    float y[PIECES][kE], t[2];
     float m2 = 0.0f, r2 = 1.0f;
     const T* brow = row_at<T>(p.b, r, p.bs);
     if (p.b && p.post) {
@@ -131,17 +131,18 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
         g.sum<1>(t);
         m2 = t[0] / (float)p.cols;
       }
-      t[0] = 0.0f;
+      t[0] = t[1] = 0.0f;
 #pragma unroll
       for (int k = 0; k < PIECES; ++k) {
         float b[kE];
         PT::get(b, here + ob, brow, w0, k);
+        if (KIND == 1) {
 #pragma unroll
-        for (int i = 0; i < kE; ++i) {
-          if (KIND == 1) b[i] = w0.piece(k).on(i) ? b[i] - m2 : 0.0f;
-          t[0] += b[i] * b[i];
+          for (int i = 0; i < kE; ++i) b[i] = w0.piece(k).on(i) ? b[i] - m2 : 0.0f;
         }
+        dot8(t, b, b);
       }
+      t[0] += t[1];
       g.sum<1>(t);
       r2 = rsqrtf(t[0] * inv + p.eps);
     }
@@ -156,8 +157,8 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
 #pragma unroll
           for (int i = 0; i < kE; ++i) b[i] -= m2;
         }
-#pragma unroll
-        for (int i = 0; i < kE; ++i) b[i] = b[i] * r2 * v[i];
+        mul8(b, b, r2);
+        mul8(b, b, v);
         if (p.c2) {
           kept.get(k * slots + 2, v);
 #pragma unroll
@@ -173,19 +174,16 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
               vec8(v, gate_row(p.gate, p.gdt, p.gs, r), p.gdt, 0.0f, w);
             act8(p.act, v);
           }
-#pragma unroll
-          for (int i = 0; i < kE; ++i) b[i] *= v[i];
+          mul8(b, b, v);
         }
         PX::get(y[k], here + ox, row_at<TX>(p.x, r, p.xs), w0, k);
         if (p.d.on) {
           unsigned u[kE];
           words8<VEC>(u, p.d, p.d.base + (u64)r * (unsigned)p.cols, w, places + hold.words);
 #pragma unroll
-          for (int i = 0; i < kE; ++i) y[k][i] += u[i] > p.d.last ? f * b[i] : 0.0f;
-        } else {
-#pragma unroll
-          for (int i = 0; i < kE; ++i) y[k][i] += f * b[i];
+          for (int i = 0; i < kE; ++i) b[i] = u[i] > p.d.last ? b[i] : 0.0f;
         }
+        fma8(y[k], b, f, y[k]);
       } else {
         PX::get(y[k], here + ox, row_at<TX>(p.x, r, p.xs), w0, k);
       }
@@ -204,22 +202,24 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
       g.sum<1>(t);
       m1 = t[0] / (float)p.cols;
     }
-    t[0] = 0.0f;
+    t[0] = t[1] = 0.0f;
 #pragma unroll
-    for (int k = 0; k < PIECES; ++k)
+    for (int k = 0; k < PIECES; ++k) {  // columns that there are not: x and b are 0, but not b - mean or a bias
+      if (KIND == 1 || p.c2) {
 #pragma unroll
-      for (int i = 0; i < kE; ++i) {
-        if (KIND == 1) y[k][i] -= m1;
-        if (w0.piece(k).on(i)) t[0] += y[k][i] * y[k][i];
+        for (int i = 0; i < kE; ++i) y[k][i] = w0.piece(k).on(i) ? y[k][i] - m1 : 0.0f;
       }
+      dot8(t, y[k], y[k]);
+    }
+    t[0] += t[1];
     g.sum<1>(t);
     const float r1 = rsqrtf(t[0] * inv + p.eps);
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
       float v[kE];
       kept.get(k * slots + 1, v);
-#pragma unroll
-      for (int i = 0; i < kE; ++i) y[k][i] = y[k][i] * r1 * v[i];
+      mul8(y[k], y[k], r1);
+      mul8(y[k], y[k], v);
       if (p.c1) {
         kept.get(k * slots + c1_at, v);
 #pragma unroll

@@ -198,6 +198,40 @@ struct Kept {
       asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[4 * h]), "=f"(v[4 * h + 1]), "=f"(v[4 * h + 2]), "=f"(v[4 * h + 3]) : "r"(at + (2 * slot + h) * plane));
   }
 };
+// Eight elements at a time by the packed F32 instructions: two results for the
+// issue slot of one, and issue slots are what bounds these loops.
+__device__ __forceinline__ void fma2(float* o, float a0, float a1, float b0, float b1, float c0, float c1) {
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(o[0]), "=f"(o[1])
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mul2(float* o, float a0, float a1, float b0, float b1) {
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(o[0]), "=f"(o[1])
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+// o = a * b, a * s, a * b + c, a * s + c, and s += a . b in two halves
+__device__ __forceinline__ void mul8(float* o, const float* a, const float* b) {
+#pragma unroll
+  for (int i = 0; i < kE; i += 2) mul2(o + i, a[i], a[i + 1], b[i], b[i + 1]);
+}
+__device__ __forceinline__ void mul8(float* o, const float* a, float s) {
+#pragma unroll
+  for (int i = 0; i < kE; i += 2) mul2(o + i, a[i], a[i + 1], s, s);
+}
+__device__ __forceinline__ void fma8(float* o, const float* a, const float* b, const float* c) {
+#pragma unroll
+  for (int i = 0; i < kE; i += 2) fma2(o + i, a[i], a[i + 1], b[i], b[i + 1], c[i], c[i + 1]);
+}
+__device__ __forceinline__ void fma8(float* o, const float* a, float s, const float* c) {
+#pragma unroll
+  for (int i = 0; i < kE; i += 2) fma2(o + i, a[i], a[i + 1], s, s, c[i], c[i + 1]);
+}
+__device__ __forceinline__ void dot8(float* s, const float* a, const float* b) {
+#pragma unroll
+  for (int i = 0; i < kE; i += 2) fma2(s, a[i], a[i + 1], b[i], b[i + 1], s[0], s[1]);
+}
+
 // How a launch holds its rows: threads of a row, slots of the ring and their
 // bytes, where the vectors are kept and where the generator's words go.
 struct Hold {
@@ -306,13 +340,16 @@ __device__ __forceinline__ void act8(int act, float* g) {
 }
 // act'(g) times v, from a = act(g)
 __device__ __forceinline__ void slope8(int act, const float* a, float* v) {
-  if (act == 1) {
+  if (act == 0) return;
+  float t[kE];
 #pragma unroll
-    for (int i = 0; i < kE; ++i) v[i] *= a[i] * (1.0f - a[i]);
-  } else if (act == 2) {
-#pragma unroll
-    for (int i = 0; i < kE; ++i) v[i] *= 1.0f - a[i] * a[i];
+  for (int i = 0; i < kE; i += 2) {
+    if (act == 1)
+      fma2(t + i, -a[i], -a[i + 1], a[i], a[i + 1], a[i], a[i + 1]);
+    else
+      fma2(t + i, -a[i], -a[i + 1], a[i], a[i + 1], 1.0f, 1.0f);
   }
+  mul8(v, v, t);
 }
 // The gate's row where it is not a matrix of T: one for all, or in f32.
 __device__ __forceinline__ const void* gate_row(const void* gate, int gdt, i64 gs, i64 r) {

@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
       f1 = t[1] * inv;
       m2 = t[2] / (float)p.cols;
     }
-    float q[3] = {0.0f, 0.0f, 0.0f};
+    float q0[2] = {}, q1[2] = {}, q2[2] = {};
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
       const Place<VEC> w = w0.piece(k);
@@ -207,25 +207,27 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
         get_y(a, k);
         get_dh(b, k);
         kept.get(k * slots, c);
+        if (KIND == 1) {
 #pragma unroll
-        for (int i = 0; i < kE; ++i) {
-          if (KIND == 1) a[i] = w.on(i) ? a[i] - m1 : 0.0f;
-          q[0] += a[i] * a[i];
-          q[1] += b[i] * c[i] * a[i];
+          for (int i = 0; i < kE; ++i) a[i] = w.on(i) ? a[i] - m1 : 0.0f;
         }
+        dot8(q0, a, a);
+        mul8(b, b, c);
+        dot8(q1, b, a);
       }
       if (norm2) {
         get_b(a, k);
+        if (KIND == 1) {
 #pragma unroll
-        for (int i = 0; i < kE; ++i) {
-          if (KIND == 1) a[i] = w.on(i) ? a[i] - m2 : 0.0f;
-          q[2] += a[i] * a[i];
+          for (int i = 0; i < kE; ++i) a[i] = w.on(i) ? a[i] - m2 : 0.0f;
         }
+        dot8(q2, a, a);
       }
     }
+    float q[3] = {q0[0] + q0[1], q1[0] + q1[1], q2[0] + q2[1]};
     g.sum<3>(q);
     const float r1 = rsqrtf(q[0] * inv + p.eps), a1 = q[1] * inv * r1, r2 = norm2 ? rsqrtf(q[2] * inv + p.eps) : 1.0f;
-    float g2[PIECES][kE], t[2] = {0.0f, 0.0f};
+    float g2[PIECES][kE], t[2] = {0.0f, 0.0f}, t0[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
       const Place<VEC> w = w0.piece(k);
@@ -243,13 +245,19 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
 #pragma unroll
           for (int i = 0; i < kE; ++i) a[i] = w.on(i) ? a[i] - m1 : 0.0f;
         }
+        mul8(a, a, r1);  // hat
+        fma8(acc[0] + k * kE, b, a, acc[0] + k * kE);
+        if (MORE) {
 #pragma unroll
-        for (int i = 0; i < kE; ++i) {
-          const float hat = a[i] * r1;
-          d[i] += r1 * (b[i] * c[i] - hat * a1 - f1);
-          acc[0][k * kE + i] += b[i] * hat;
-          if (MORE) acc[2][k * kE + i] += b[i];
+          for (int i = 0; i < kE; ++i) acc[2][k * kE + i] += b[i];
         }
+        mul8(b, b, c);
+        fma8(b, a, -a1, b);
+        if (KIND == 1) {
+#pragma unroll
+          for (int i = 0; i < kE; ++i) b[i] -= f1;
+        }
+        fma8(d, b, r1, d);
       }
       if (p.dx) store8<TX>(row_at<TX>(p.dx, r, p.dxs), d, w);
       if (!p.b) continue;
@@ -257,11 +265,9 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
         unsigned u[kE];
         words8<VEC>(u, p.d, p.d.base + (u64)r * (unsigned)p.cols, w, places + hold.words);
 #pragma unroll
-        for (int i = 0; i < kE; ++i) d[i] = u[i] > p.d.last ? f * d[i] : 0.0f;  // dz
-      } else {
-#pragma unroll
-        for (int i = 0; i < kE; ++i) d[i] *= f;
+        for (int i = 0; i < kE; ++i) d[i] = u[i] > p.d.last ? d[i] : 0.0f;
       }
+      mul8(d, d, f);  // dz
       get_b(b, k);
       kept.get(k * slots + 1, c);
       if (KIND == 1) {  // 0 - mean is not 0
@@ -271,8 +277,7 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
           if (!w.on(i)) b[i] = d[i] = 0.0f;
         }
       }
-#pragma unroll
-      for (int i = 0; i < kE; ++i) b[i] *= r2;  // hat
+      mul8(b, b, r2);  // hat
       if (p.gate) {
         if (channel) {
           kept.get(k * slots + gate_at, a);
@@ -286,18 +291,17 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
         float u[kE];
         if (p.c2) {
           kept.get(k * slots + 2, u);
-#pragma unroll
-          for (int i = 0; i < kE; ++i) u[i] = d[i] * (b[i] * c[i] + u[i]);
+          fma8(u, b, c, u);
         } else {
-#pragma unroll
-          for (int i = 0; i < kE; ++i) u[i] = d[i] * b[i] * c[i];
+          mul8(u, b, c);
         }
+        mul8(u, u, d);
         slope8(p.act, a, u);
+        if (MORE) {
 #pragma unroll
-        for (int i = 0; i < kE; ++i) {
-          if (MORE) acc[4][k * kE + i] += u[i];
-          d[i] *= a[i];  // du
+          for (int i = 0; i < kE; ++i) acc[4][k * kE + i] += u[i];
         }
+        mul8(d, d, a);  // du
         if (p.dgate) {
           if (p.gdt == CCB_F32)
             store8<float>(row_at<float>(p.dgate, r, p.dgs), u, w);
@@ -305,15 +309,19 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
             store8<T>(row_at<T>(p.dgate, r, p.dgs), u, w);
         }
       }
+      fma8(acc[1] + k * kE, d, b, acc[1] + k * kE);
+      if (MORE) {
 #pragma unroll
-      for (int i = 0; i < kE; ++i) {
-        acc[1][k * kE + i] += d[i] * b[i];
-        if (MORE) acc[3][k * kE + i] += d[i];
-        g2[k][i] = d[i] * c[i];
-        t[0] += g2[k][i] * b[i];
-        if (KIND == 1) t[1] += g2[k][i];
+        for (int i = 0; i < kE; ++i) acc[3][k * kE + i] += d[i];
+      }
+      mul8(g2[k], d, c);
+      dot8(t0, g2[k], b);
+      if (KIND == 1) {
+#pragma unroll
+        for (int i = 0; i < kE; ++i) t[1] += g2[k][i];
       }
     }
+    t[0] = t0[0] + t0[1];
     if (p.db) {
       float a2 = 0.0f, f2 = 0.0f;
       if (p.post) {
@@ -329,8 +337,16 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
         if (p.post) {
           float b[kE];
           get_b(b, k);
+          if (KIND == 1) {
 #pragma unroll
-          for (int i = 0; i < kE; ++i) g2[k][i] = r2 * g2[k][i] - (b[i] - m2) * a2 - f2;
+            for (int i = 0; i < kE; ++i) b[i] -= m2;
+          }
+          mul8(g2[k], g2[k], r2);
+          fma8(g2[k], b, -a2, g2[k]);
+          if (KIND == 1) {
+#pragma unroll
+            for (int i = 0; i < kE; ++i) g2[k][i] -= f2;
+          }
         }
         store8<T>(row_at<T>(p.db, r, p.dbs), g2[k], w0.piece(k));
       }
