@@ -59,44 +59,56 @@ __global__ void __launch_bounds__(256) dropout_any(const __grid_constant__ Dropo
 
 // 8 consecutive elements of a row by 16-byte accesses: pointers and strides of
 // 16 bytes, and rows of whole pieces of 8 (dense rows are one long row, whose
-// last elements the first threads take).
+// last elements the first threads take). The generator takes half as long as
+// the memory, so they have to overlap: a thread has 32 bytes (64 with a
+// residual) on their way whatever the type, two pieces of a 16-bit one (one
+// alone left 16384 x 4096 of them at 75 us without a residual).
 template <class T>
 __global__ void __launch_bounds__(256) dropout_wide(const __grid_constant__ DropoutP p, unsigned pieces, u64 total) {
+  constexpr int kWords = sizeof(T) / 2, kOnce = 4 / (int)sizeof(T);  // 16-byte words of a piece, pieces at once
   const u64 step = (u64)gridDim.x * blockDim.x, first = (u64)blockIdx.x * blockDim.x + threadIdx.x;
-  for (u64 v = first; v < total; v += step) {
-    u64 r = 0, c = v;
-    if (p.rows > 1) {  // total is below 2^32
-      r = (unsigned)v / pieces;
-      c = (unsigned)v - (unsigned)r * pieces;
-    }
-    c *= 8;
-    const T* x = static_cast<const T*>(p.x) + r * p.xs + c;
-    const T* res = static_cast<const T*>(p.res) + r * p.rs + c;
-    T* out = static_cast<T*>(p.out) + r * p.os + c;
-    constexpr int kWords = 2 * sizeof(T);
-    uint4 a[kWords / 4], b[kWords / 4] = {};
+  for (u64 v0 = first; v0 < total; v0 += kOnce * step) {
+    uint4 a[kOnce][kWords], b[kOnce][kWords];
+    u64 row[kOnce], col[kOnce];
 #pragma unroll
-    for (int i = 0; i < kWords / 4; ++i) a[i] = reinterpret_cast<const uint4*>(x)[i];
-    if (p.res)
+    for (int k = 0; k < kOnce; ++k) {
+      const u64 v = v0 + k * step;
+      row[k] = 0;
+      col[k] = v;
+      if (p.rows > 1) {  // total is below 2^32
+        row[k] = (unsigned)v / pieces;
+        col[k] = (unsigned)v - (unsigned)row[k] * pieces;
+      }
+      col[k] *= 8;
+      if (v >= total) continue;
+      const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + row[k] * p.xs + col[k]);
+      const uint4* res = reinterpret_cast<const uint4*>(static_cast<const T*>(p.res) + row[k] * p.rs + col[k]);
 #pragma unroll
-      for (int i = 0; i < kWords / 4; ++i) b[i] = reinterpret_cast<const uint4*>(res)[i];
-    unsigned w[8];
-    if (p.d.on) philox8(p.d, p.d.base + r * (u64)p.cols + c, w);
-    float y[8];
+      for (int i = 0; i < kWords; ++i) a[k][i] = x[i];
+      if (p.res)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      y[i] = element<T>(a, i) * p.d.factor;
-      if (p.d.on && w[i] <= p.d.last) y[i] = 0.0f;
-      if (p.res) y[i] += element<T>(b, i);
+        for (int i = 0; i < kWords; ++i) b[k][i] = res[i];
     }
 #pragma unroll
-    for (int i = 0; i < kWords / 4; ++i) {
-      uint4 o;
-      if constexpr (sizeof(T) == 4)
-        o = make_uint4(__float_as_uint(y[4 * i]), __float_as_uint(y[4 * i + 1]), __float_as_uint(y[4 * i + 2]), __float_as_uint(y[4 * i + 3]));
-      else
-        o = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
-      reinterpret_cast<uint4*>(out)[i] = o;
+    for (int k = 0; k < kOnce; ++k) {
+      if (v0 + k * step >= total) break;
+      unsigned w[8];
+      if (p.d.on) philox8(p.d, p.d.base + row[k] * (u64)p.cols + col[k], w);
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[i] = element<T>(a[k], i) * p.d.factor;
+        if (p.d.on && w[i] <= p.d.last) y[i] = 0.0f;
+        if (p.res) y[i] += element<T>(b[k], i);
+      }
+      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row[k] * p.os + col[k]);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        if constexpr (sizeof(T) == 4)
+          out[i] = make_uint4(__float_as_uint(y[4 * i]), __float_as_uint(y[4 * i + 1]), __float_as_uint(y[4 * i + 2]), __float_as_uint(y[4 * i + 3]));
+        else
+          out[i] = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
+      }
     }
   }
   if (p.rows == 1) {
