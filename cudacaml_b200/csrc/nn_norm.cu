@@ -16,8 +16,9 @@ struct NormP {
   Drop d;
 };
 
-// Rows of any length and alignment: a block walks a row once for each
-// statistic and once for the results, reading it again each time.
+// Rows of any length, alignment and stride, for what norm_rows does not take: a
+// block walks a row once for each statistic and once for the results, reading
+// it again each time (8192 x 4096 bf16 with gate and mask: 565 us).
 template <class T, class TX, int KIND>
 __global__ void __launch_bounds__(kBlock) norm_any(const __grid_constant__ NormP p) {
   __shared__ float s[kBlock / 32];
@@ -53,6 +54,9 @@ __global__ void __launch_bounds__(kBlock) norm_any(const __grid_constant__ NormP
   }
 }
 
+// The join of rows that a group holds. Bound by instruction issue: at 8192 x 4096
+// bf16 with a sigmoid gate and a mask 78 us (4.3 TB/s, 60 % of the issue slots;
+// the generator is 19 us of it), 49 us without both (5.5 TB/s).
 template <class T, class TX, int KIND, bool VEC, int PIECES>
 __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__ NormP p, const Hold hold) {
   __shared__ __align__(16) float s[kRowThreads / 32 * 8];

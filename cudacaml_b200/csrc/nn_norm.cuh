@@ -65,7 +65,9 @@ __device__ __forceinline__ void stats(i64 cols, float eps, float* s, float& mean
 // (cols a multiple of 8; pointers and strides of 16 bytes): a thread's elements
 // are consecutive, and it copies and reads its own alone, so that there is no
 // barrier. Otherwise they are tpr apart, and the group copies the 16-byte
-// pieces of memory that hold the row between its threads. A block holds
+// pieces of memory that hold the row between its threads (the bytes before a
+// row's first element in its first piece are read, inside the aligned 16 bytes
+// that hold it, and not used; none are read past its last). A block holds
 // blockDim.x / tpr rows at a time and takes every grid-th set.
 constexpr int kE = 8;
 

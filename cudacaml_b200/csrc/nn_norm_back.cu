@@ -18,7 +18,8 @@ struct BackP {
   Drop d;
 };
 
-// The gradient for any length and alignment. A block takes every grid-th row
+// The gradient for any length, alignment and stride, for what norm_back_rows
+// does not take (8192 x 4096 bf16: 1767 us). A block takes every grid-th row
 // and keeps its own partial sums over rows in the workspace; a thread always
 // handles the same columns of it.
 template <class T, class TX, int KIND>
@@ -99,7 +100,10 @@ __global__ void __launch_bounds__(kBlock) norm_back_any(const __grid_constant__ 
 // gradient. A row takes two sums over it (the statistics and the first norm's
 // terms; the second norm's terms), three for the layer norm; between them the
 // row is read again from the ring, piece by piece, which leaves registers for
-// the sums over rows: they stay in them for all of a thread's rows.
+// the sums over rows: they stay in them for all of a thread's rows. Bound by
+// instruction issue and latency at two rows of 4096 an SM: 8192 x 4096 bf16 with
+// gate and mask 135 us (4.0 TB/s), 241 us with the layer norm's biases and a
+// channel gate, whose five sums spill registers.
 template <class T, class TX, int KIND, bool VEC, int PIECES, bool MORE>
 __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ BackP p, const Hold hold) {
   __shared__ __align__(16) float s[16 * 8];
@@ -383,7 +387,8 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
 }
 
 // Column sums of the blocks' partials: a warp's 32 columns, 8 warps that each
-// take every eighth block, their results added in order.
+// take every eighth block, their results added in order (3 us for 148 blocks of
+// 4096 columns and two sums).
 __global__ void __launch_bounds__(kBlock) norm_back_sum(const __grid_constant__ BackP p, int blocks) {
   __shared__ float s[kBlock];
   float* out = p.vec[blockIdx.y];

@@ -183,3 +183,12 @@ def test_residents_and_arrays():
     assert np.array_equal(cuda.download(x).data.reshape(-1), got.cpu().numpy().reshape(-1))
     cuda.free_resident(x)
     cuda.free_resident(out)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("base", [(1 << 34) - 21, (1 << 34) - 4000])
+def test_counters_whose_high_word_changes_on_the_way(dtype, base):
+    x = rand((40, 200), TYPES[dtype], 13)
+    out = torch.empty_like(x)
+    nn.dropout(x, 0.3, 5, out, base=base, offset=(1 << 33) + 7)
+    check(x, out, 0.3, 5, (1 << 33) + 7, base)

@@ -252,3 +252,33 @@ def test_capture_with_offsets_that_change():
         close(dw, e, slack(m, 300), "captured dw")
     g.destroy()
     st.destroy()
+
+
+@pytest.mark.parametrize("rows,k,n", [(96, 200, 72), (6, 200, 72)])
+@pytest.mark.parametrize("wt", [False, True])
+def test_f32_holds_over_the_whole_range(rows, k, n, wt):
+    # numbers of very different size, down to where the lowest of three planes vanishes, each row and matrix of one size
+    offsets = [0, rows // 3, rows // 3, rows]
+    scale = torch.tensor([2.0**e for e in (-60, -20, 0, 30, 90)], device=DEV)
+    x = rand((rows, k), torch.float32, 30) * scale[torch.arange(rows, device=DEV) % 5][:, None]
+    w = rand((3, n, k) if wt else (3, k, n), torch.float32, 31)
+    forward(x, w, offsets, wt)
+
+
+def test_f32_nan_reaches_its_row_alone():
+    x, w = rand((64, 96), torch.float32, 32), rand((2, 96, 40), torch.float32, 33)
+    x[5, 7] = float("nan")
+    for offsets in ([0, 32, 64], [0, 5, 6]):
+        y = forward(x, w, offsets, False, check=False)
+        bad = torch.isnan(y).any(1)
+        assert bool(bad[5]) and int(bad.sum()) == 1 and bool(torch.isnan(y[5]).all())
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_a_long_contraction_over_one_expert(dtype):
+    t = TYPES[dtype]
+    x, dy = rand((5000, 24), t, 34), rand((5000, 40), t, 35)
+    backward_w(x, dy, [0, 4990])
+    backward_w(x, dy, [0, 10, 4000, 5000])
+    forward(rand((3, 9000), t, 36), rand((2, 9000, 40), t, 37, 0.01), [0, 1, 3], False)
+    forward(rand((3, 9000), t, 36), rand((2, 40, 9000), t, 37, 0.01), [0, 1, 3], True)

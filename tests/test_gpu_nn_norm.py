@@ -283,3 +283,36 @@ def test_another_stream_and_capture():
         assert torch.equal(y, y2) and torch.equal(h, h2) and torch.equal(dx, g0["dx"]) and torch.equal(dw, g0["dpost_weight"])
     g.destroy()
     st.destroy()
+
+
+@pytest.mark.parametrize("base", [3, (1 << 34) - 700, (1 << 34) - 702, (1 << 63) + 8])
+@pytest.mark.parametrize("t,cols", [("bf16", 256), ("f32", 130)])
+def test_masks_of_any_first_index(base, t, cols):
+    # a first index that is no multiple of the generator's four, and one whose counters' high word changes on the way
+    c = Case(9, cols, TYPES[t], TYPES[t], p=0.3)
+    c.base = c.how["base"] = base
+    c.plain["mask"] = keep(base, (9, cols), 0.3, c.seed, c.offset, DEV).double() / 0.7
+    y, _ = c.forward()
+    c.backward(y, c.dy, c.dh)
+
+
+@pytest.mark.parametrize("t", ["bf16", "f32"])
+def test_f32_gate_of_every_element(t):
+    rows, cols = 19, 264
+    c = Case(rows, cols, TYPES[t], torch.float32, act="tanh")
+    c.gate = rand((rows, cols), torch.float32, 31, 0.4)
+    c.how["gate"], c.plain["gate"] = c.gate, c.gate
+    y, _ = c.forward()
+    dgate = torch.empty_like(c.gate)
+    nn.block_norm_backward(y, dy=c.dy, dh=c.dh, dgate=dgate, **c.how)
+    e, m = block_grad(y, c.branch, c.dy, c.dh, **c.plain)["dgate"]
+    close(dgate, e, slack(m, cols), "dgate")
+
+
+def test_tanh_gate_near_zero_keeps_its_relative_error():
+    g = torch.cat([torch.logspace(-30, 0.7, 2000), -torch.logspace(-30, 0.7, 2000), torch.tensor([0.0, 0.5499, 0.5501, float("inf"), -float("inf")])]).to(DEV)
+    cols = g.numel()
+    x, y = torch.zeros((1, cols), device=DEV), torch.empty((1, cols), device=DEV)
+    nn.block_norm(x, y, branch=torch.ones_like(x), post_norm=False, gate=g.reshape(1, -1), gate_act="tanh")
+    # series, exponential and reciprocal: eight units in the last place
+    close(y, torch.tanh(g.double()).reshape(1, -1), 8 * U * torch.tanh(g.double()).abs().reshape(1, -1), "tanh")
