@@ -1059,7 +1059,13 @@ Plan plan_of(const ccb_nn_grouped_matmul_t* a) {
   const i64 some = a->experts < a->rows ? a->experts : a->rows;
   p.w = operand(a->dtype, a->w, a->experts, a->transpose_w ? a->n : a->k, a->transpose_w ? a->k : a->n, a->w_stride, a->w_row_stride);
   p.x = operand(a->dtype, a->x, 1, a->rows, a->k, 0, a->x_stride);
-  // Packing reads and writes every expert's matrix: it pays from some rows an expert on.
+  // Packing reads and writes every expert's matrix: it pays from some rows an
+  // expert on. In us, CUDA cores against packing and tensor cores: F32, 32 rows
+  // of 12 experts, 2048 x 1024: 38 / 110; 128 rows of 16, 256 x 512: 11 / 17;
+  // 700 rows of 20, 1024 x 1024: 76 / 84, transposed 113 / 82; 1003 rows of 6,
+  // 515 x 129: 29 / 19; 200 rows of 2, 2000 x 2000: 68 / 38. BF16, 100 rows of
+  // 5, 333 x 777: 46 / 11; 32 rows of 12, 2047 x 1023: 56 / 44, transposed
+  // 34 / 45.
   p.tensor = !p.w.packs || a->rows >= 16 * some;
   p.result = a->rows * a->n;
   if (!p.tensor) {  // two tiles for each of five blocks an SM, and no part above what shared memory takes
