@@ -119,7 +119,8 @@ int clear(int dtype, void* out, i64 mats, i64 rows, i64 cols, i64 oe, i64 os, co
 // Bound by reading the matrices of the experts that have rows (64 rows over 50
 // of 64 experts of 1024 x 2048 f32: 96 us, 4.4 TB/s; transposed 127 us, 3.3
 // TB/s; 64 x 64 tiles before it left most SMs idle: 445 us for 32 rows over 12
-// experts of 2048 x 1024, 38 us now): a block takes up
+// experts of 2048 x 1024, 38 us now; 64 rows over 50 of 64 of 1023 x 2047 bf16
+// 82 us, 2.6 TB/s by single elements): a block takes up
 // to 8 rows of one expert, a block of output columns and a part of the
 // contraction, keeps the rows' values in shared memory and reads every weight
 // once, in order. Parts are summed by add_parts, so that the SMs are filled
@@ -160,22 +161,24 @@ __global__ void __launch_bounds__(kFewThreads) grouped_few(const __grid_constant
     __syncthreads();
     // 16 weights in hand and the next 16 on their way; of 16-bit ones twice as many
     constexpr int kStep = sizeof(T) == 4 ? 4 : 8;
-    float v[kStep][4], u[kStep][4];
+    float v[kStep][4];
+    T u[kStep][4];  // as read: a conversion in the fetch would wait for its load
+    const T none = from_f<T>(0.0f);
     if constexpr (!WT) {
       bool on[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) on[j] = n0 + threadIdx.x + j * kFewThreads < p.n;
       const T* at = w + k0 * p.ws + n0 + threadIdx.x;
-      auto fetch = [&](float (*to)[4], int k) {
+      auto fetch = [&](T (*to)[4], int k) {
 #pragma unroll
         for (int i = 0; i < kStep; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) to[i][j] = on[j] && k + i < kn ? to_f<T>(at[(k + i) * p.ws + j * kFewThreads]) : 0.0f;
+          for (int j = 0; j < 4; ++j) to[i][j] = on[j] && k + i < kn ? at[(k + i) * p.ws + j * kFewThreads] : none;
       };
       fetch(u, 0);
       for (int k = 0; k < kn; k += kStep) {
 #pragma unroll
-        for (int i = 0; i < 4 * kStep; ++i) v[i >> 2][i & 3] = u[i >> 2][i & 3];
+        for (int i = 0; i < 4 * kStep; ++i) v[i >> 2][i & 3] = to_f<T>(u[i >> 2][i & 3]);
         fetch(u, k + kStep);
 #pragma unroll
         for (int i = 0; i < kStep; ++i) {
@@ -205,16 +208,16 @@ __global__ void __launch_bounds__(kFewThreads) grouped_few(const __grid_constant
 #pragma unroll
           for (int r = 0; r < kFewRows; ++r) acc[j][r] = 0.0f;
         }
-        auto fetch = [&](float (*to)[4], int k) {
+        auto fetch = [&](T (*to)[4], int k) {
 #pragma unroll
           for (int i = 0; i < kStep; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) to[i][j] = k + 32 * i < kn ? to_f<T>(at[j][k + 32 * i]) : 0.0f;
+            for (int j = 0; j < 4; ++j) to[i][j] = k + 32 * i < kn ? at[j][k + 32 * i] : none;
         };
         fetch(u, lane);
         for (int k = lane; k < kz; k += 32 * kStep) {
 #pragma unroll
-          for (int i = 0; i < 4 * kStep; ++i) v[i >> 2][i & 3] = u[i >> 2][i & 3];
+          for (int i = 0; i < 4 * kStep; ++i) v[i >> 2][i & 3] = to_f<T>(u[i >> 2][i & 3]);
           fetch(u, k + 32 * kStep);
 #pragma unroll
           for (int i = 0; i < kStep; ++i) {
@@ -1063,9 +1066,8 @@ Plan plan_of(const ccb_nn_grouped_matmul_t* a) {
   // expert on. In us, CUDA cores against packing and tensor cores: F32, 32 rows
   // of 12 experts, 2048 x 1024: 38 / 110; 128 rows of 16, 256 x 512: 11 / 17;
   // 700 rows of 20, 1024 x 1024: 76 / 84, transposed 113 / 82; 1003 rows of 6,
-  // 515 x 129: 29 / 19; 200 rows of 2, 2000 x 2000: 68 / 38. BF16, 100 rows of
-  // 5, 333 x 777: 46 / 11; 32 rows of 12, 2047 x 1023: 56 / 44, transposed
-  // 34 / 45.
+  // 515 x 129: 29 / 19; 200 rows of 2, 2000 x 2000: 68 / 38. BF16, 32 rows of
+  // 12, 2047 x 1023: 27 / 44, transposed 33 / 45.
   p.tensor = !p.w.packs || a->rows >= 16 * some;
   p.result = a->rows * a->n;
   if (!p.tensor) {  // two tiles for each of five blocks an SM, and no part above what shared memory takes
