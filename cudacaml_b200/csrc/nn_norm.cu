@@ -54,10 +54,14 @@ __global__ void __launch_bounds__(kBlock) norm_any(const __grid_constant__ NormP
   }
 }
 
-// The join of rows that a group holds. Bound by instruction issue: at 8192 x 4096
-// bf16 with a sigmoid gate and a mask 78 us (4.3 TB/s, 60 % of the issue slots;
-// the generator is 19 us of it), 49 us without both (5.5 TB/s).
-template <class T, class TX, int KIND, bool VEC, int PIECES>
+// The join of rows that a group holds. HAS: 0 any arguments; else a normed
+// branch without biases and both results, with (2) a gate as a matrix of T or
+// without one (1): what a training step of an rms norm asks for, whose loops
+// have no branches left to end the compiler's schedule. Bound by instruction
+// issue: at 8192 x 4096 bf16 with a sigmoid gate and a mask 72 us (4.7 TB/s; 78
+// by HAS = 0; the generator is 17 us of it), a mask alone 62 us (70), neither 53
+// us (52; 512 columns 15 against 16).
+template <class T, class TX, int KIND, bool VEC, int PIECES, int HAS>
 __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__ NormP p, const Hold hold) {
   __shared__ __align__(16) float s[kRowThreads / 32 * 8];
   extern __shared__ __align__(16) unsigned char places[];
@@ -68,7 +72,8 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
   const Place<VEC> w0 = {(int)threadIdx.x - g.id * tpr, tpr, (int)p.cols};
   // a mean is divided, so that a constant row's is its value
   const float inv = 1.0f / (float)p.cols, f = p.scale * p.d.factor;
-  const bool channel = p.gate && p.gs == 0, full = p.gate && !channel && p.gdt != CCB_F32;
+  const bool gate = HAS ? HAS == 2 : p.gate != nullptr, channel = !HAS && gate && p.gs == 0, full = HAS ? gate : gate && !channel && p.gdt != CCB_F32;
+  const bool has_b = HAS || p.b, post = HAS || p.post, c1 = !HAS && p.c1, c2 = !HAS && p.c2;
   const unsigned sets = blockDim.x / tpr, first = blockIdx.x * sets + g.id, step = gridDim.x * sets, rows = (unsigned)p.rows;
   const unsigned all = (unsigned)__cvta_generic_to_shared(places);
   const unsigned ox = VEC ? threadIdx.x * 16 : g.id * (part_bytes<TX, VEC, PIECES>(p.cols, blockDim.x, tpr) / sets);
@@ -76,7 +81,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
   const unsigned og = ob + part_bytes<T, VEC, PIECES>(p.cols, blockDim.x, tpr), end = all + ahead * hold.slot;
   // kept, for each piece: w2, w1, then c2, c1 and a channel gate's act, as far as there are any
   const Kept kept = {all + hold.kept + w0.t * 16, (unsigned)tpr * 16};
-  const int c1_at = 2 + (p.c2 != nullptr), gate_at = c1_at + (p.c1 != nullptr), slots = gate_at + channel;
+  const int c1_at = 2 + c2, gate_at = c1_at + c1, slots = gate_at + channel;
   if (g.id == 0) {
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
@@ -86,11 +91,11 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
       kept.put(k * slots, v);
       vec8(v, p.w1, p.wdt, 1.0f, w);
       kept.put(k * slots + 1, v);
-      if (p.c2) {
+      if (c2) {
         vec8(v, p.c2, p.wdt, 0.0f, w);
         kept.put(k * slots + 2, v);
       }
-      if (p.c1) {
+      if (c1) {
         vec8(v, p.c1, p.wdt, 0.0f, w);
         kept.put(k * slots + c1_at, v);
       }
@@ -105,7 +110,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
   auto fetch = [&]() {
     if (coming < rows) {
       PX::fetch(to + ox, row_at<TX>(p.x, coming, p.xs), w0);
-      if (p.b) PT::fetch(to + ob, row_at<T>(p.b, coming, p.bs), w0);
+      if (has_b) PT::fetch(to + ob, row_at<T>(p.b, coming, p.bs), w0);
       if (full) PT::fetch(to + og, row_at<T>(p.gate, coming, p.gs), w0);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -122,7 +127,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
     float y[PIECES][kE], t[2];
     float m2 = 0.0f, r2 = 1.0f;
     const T* brow = row_at<T>(p.b, r, p.bs);
-    if (p.b && p.post) {
+    if (has_b && post) {
       if (KIND == 1) {
         t[0] = 0.0f;
 #pragma unroll
@@ -153,7 +158,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
       const Place<VEC> w = w0.piece(k);
-      if (p.b) {
+      if (has_b) {
         float b[kE], v[kE];
         PT::get(b, here + ob, brow, w0, k);
         kept.get(k * slots, v);
@@ -163,12 +168,12 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
         }
         mul8(b, b, r2);
         mul8(b, b, v);
-        if (p.c2) {
+        if (c2) {
           kept.get(k * slots + 2, v);
 #pragma unroll
           for (int i = 0; i < kE; ++i) b[i] += v[i];
         }
-        if (p.gate) {
+        if (gate) {
           if (channel) {
             kept.get(k * slots + gate_at, v);
           } else {
@@ -191,10 +196,10 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
       } else {
         PX::get(y[k], here + ox, row_at<TX>(p.x, r, p.xs), w0, k);
       }
-      if (p.y) store8<TX>(row_at<TX>(p.y, r, p.ys), y[k], w);
+      if (HAS || p.y) store8<TX>(row_at<TX>(p.y, r, p.ys), y[k], w);
     }
     here = here + hold.slot == end ? all : here + hold.slot;
-    if (!p.h) continue;
+    if (!HAS && !p.h) continue;
     float m1 = 0.0f;
     if (KIND == 1) {
       t[0] = 0.0f;
@@ -209,7 +214,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
     t[0] = t[1] = 0.0f;
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {  // columns that there are not: x and b are 0, but not b - mean or a bias
-      if (KIND == 1 || p.c2) {
+      if (KIND == 1 || c2) {
 #pragma unroll
         for (int i = 0; i < kE; ++i) y[k][i] = w0.piece(k).on(i) ? y[k][i] - m1 : 0.0f;
       }
@@ -224,7 +229,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
       kept.get(k * slots + 1, v);
       mul8(y[k], y[k], r1);
       mul8(y[k], y[k], v);
-      if (p.c1) {
+      if (c1) {
         kept.get(k * slots + c1_at, v);
 #pragma unroll
         for (int i = 0; i < kE; ++i) y[k][i] += v[i];
@@ -237,26 +242,31 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
 
 template <class T, class TX, int KIND>
 struct Forward {
-  template <bool VEC, int PIECES>
+  template <bool VEC, int PIECES, int HAS>
   static bool rows(const NormP& p, int sms, cudaStream_t st) {
     static bool ready[64];
-    const int matrices = (p.b != nullptr) + (p.gate && p.gs != 0 && p.gdt != CCB_F32);
+    const int matrices = (p.b != nullptr) + (HAS ? HAS == 2 : p.gate && p.gs != 0 && p.gdt != CCB_F32);
     const Shape f = shape_of(p.cols, PIECES, kRowThreads, VEC, 2 + (p.c1 != nullptr) + (p.c2 != nullptr) + (p.gate && p.gs == 0), 0, [&](int block, int tpr) {
       return part_bytes<TX, VEC, PIECES>(p.cols, block, tpr) + matrices * part_bytes<T, VEC, PIECES>(p.cols, block, tpr);
     });
-    if (!f.block || !room_for(norm_rows<T, TX, KIND, VEC, PIECES>, ready)) return false;
+    if (!f.block || !room_for(norm_rows<T, TX, KIND, VEC, PIECES, HAS>, ready)) return false;
     const i64 groups = f.block / f.hold.tpr, sets = (p.rows + groups - 1) / groups;
-    norm_rows<T, TX, KIND, VEC, PIECES><<<(unsigned)(sets < sms ? sets : sms), f.block, f.smem, st>>>(p, f.hold);
+    norm_rows<T, TX, KIND, VEC, PIECES, HAS><<<(unsigned)(sets < sms ? sets : sms), f.block, f.smem, st>>>(p, f.hold);
     return true;
   }
   static bool by_width(const NormP& p, int sms, cudaStream_t st) {
     if (!near({p.xs, p.bs, p.gs, p.ys, p.hs}) || (p.d.on && !p.d.same)) return false;
-    if ((p.d.base & 3) || !wide(p.cols, {p.x, p.b, p.gate, p.y, p.h}, {p.xs, p.bs, p.gs, p.ys, p.hs})) return rows<false, 1>(p, sms, st);
+    if ((p.d.base & 3) || !wide(p.cols, {p.x, p.b, p.gate, p.y, p.h}, {p.xs, p.bs, p.gs, p.ys, p.hs})) return rows<false, 1, 0>(p, sms, st);
     // What a thread does once a row (its sums, addresses, copies) is some 300
     // instructions: 16 elements share them, fewer where a warp holds the row (32
     // would spill at the registers that three rows of 4096 leave). The shape goes
     // by the columns alone: a row's result does not depend on the rows beside it.
-    return p.cols <= 256 ? rows<true, 1>(p, sms, st) : rows<true, 2>(p, sms, st);
+    const bool one = p.cols <= 256;
+    if (p.b && p.post && p.y && p.h && !p.c1 && !p.c2) {
+      if (!p.gate) return one ? rows<true, 1, 1>(p, sms, st) : rows<true, 2, 1>(p, sms, st);
+      if (p.gs && p.gdt == code_of<T>) return one ? rows<true, 1, 2>(p, sms, st) : rows<true, 2, 2>(p, sms, st);
+    }
+    return one ? rows<true, 1, 0>(p, sms, st) : rows<true, 2, 0>(p, sms, st);
   }
   static void run(const NormP& p, int sms, cudaStream_t st) {
     if (by_width(p, sms, st)) return;
@@ -297,7 +307,11 @@ extern "C" int ccb_nn_block_norm(const ccb_nn_block_norm_t* a, void* stream) {
     const NormP p = {a->x, a->branch, a->gate, a->pre_weight, a->pre_bias, a->post_weight, a->post_bias, a->y, a->h, a->rows, a->cols,
                      a->x_stride, a->branch_stride, a->gate_stride, a->y_stride, a->h_stride, (float)a->eps, (float)a->scale, a->gate_dtype,
                      a->weight_dtype, a->act, a->post_norm, make_drop(a->p, a->seed, a->offset, a->base, (u64)a->rows * (u64)a->cols)};
-    by_type<Forward>(a->dtype, a->x_dtype, a->kind, p, sms, static_cast<cudaStream_t>(stream));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->dtype == CCB_F16)
+      by_f16<Forward>(a->dtype, a->x_dtype, a->kind, p, sms, st);
+    else
+      by_type_but_f16<Forward>(a->dtype, a->x_dtype, a->kind, p, sms, st);
     return launched(me);
   })
 }

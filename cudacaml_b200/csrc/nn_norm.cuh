@@ -71,6 +71,9 @@ __device__ __forceinline__ void stats(i64 cols, float eps, float* s, float& mean
 // blockDim.x / tpr rows at a time and takes every grid-th set.
 constexpr int kE = 8;
 
+template <class T>
+constexpr int code_of = sizeof(T) == 4 ? CCB_F32 : std::is_same<T, __half>::value ? CCB_F16 : CCB_BF16;
+
 template <bool VEC>
 struct Place {
   int t, tpr, cols;
@@ -317,10 +320,14 @@ __device__ __forceinline__ void words8(unsigned* u, const Drop& d, u64 e0, const
 __device__ __forceinline__ void act8(int act, float* g) {
   if (act == 1) {
 #pragma unroll
-    for (int i = 0; i < kE; ++i) {
-      float e;
-      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g[i] * -1.4426950408889634f));
-      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(g[i]) : "f"(1.0f + e));
+    for (int i = 0; i < kE; i += 2) {
+      float e[2];
+      mul2(e, g[i], g[i + 1], -1.4426950408889634f, -1.4426950408889634f);
+      asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[0]));
+      asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[1]));
+      fma2(e, e[0], e[1], 1.0f, 1.0f, 1.0f, 1.0f);
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(g[i]) : "f"(e[0]));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(g[i + 1]) : "f"(e[1]));
     }
   } else if (act == 2) {  // 1 - 2 / (1 + e^2g); below 0.55, where that cancels, the series to x^13 (3e-7 at its end)
 #pragma unroll
@@ -346,10 +353,12 @@ __device__ __forceinline__ void slope8(int act, const float* a, float* v) {
   float t[kE];
 #pragma unroll
   for (int i = 0; i < kE; i += 2) {
-    if (act == 1)
-      fma2(t + i, -a[i], -a[i + 1], a[i], a[i + 1], a[i], a[i + 1]);
-    else
+    if (act == 1) {
+      fma2(t + i, a[i], a[i + 1], -1.0f, -1.0f, 1.0f, 1.0f);
+      mul2(t + i, t[i], t[i + 1], a[i], a[i + 1]);
+    } else {
       fma2(t + i, -a[i], -a[i + 1], a[i], a[i + 1], 1.0f, 1.0f);
+    }
   }
   mul8(v, v, t);
 }
@@ -396,9 +405,8 @@ __device__ __forceinline__ void turn_ring(const Group& g, int ahead, F fetch) {
   }
 }
 
-// The element types a call may have: dtype, and the residual stream in it or in f32.
-template <template <class, class, int> class Go, class... A>
-void by_type(int dtype, int x_dtype, int kind, A... a) {
+// The element types a call may have: dtype, and the residual stream in it or in
+// f32. The f16 ones by themselves, for a file of their own.
 #define CCB_NN_CASE(dt, xdt, T, TX)         \
   if (dtype == dt && x_dtype == xdt) {      \
     if (kind == 0)                          \
@@ -407,13 +415,18 @@ void by_type(int dtype, int x_dtype, int kind, A... a) {
       Go<T, TX, 1>::run(a...);              \
     return;                                 \
   }
+template <template <class, class, int> class Go, class... A>
+void by_f16(int dtype, int x_dtype, int kind, A... a) {
+  CCB_NN_CASE(CCB_F16, CCB_F16, __half, __half)
+  CCB_NN_CASE(CCB_F16, CCB_F32, __half, float)
+}
+template <template <class, class, int> class Go, class... A>
+void by_type_but_f16(int dtype, int x_dtype, int kind, A... a) {
   CCB_NN_CASE(CCB_F32, CCB_F32, float, float)
   CCB_NN_CASE(CCB_BF16, CCB_BF16, __nv_bfloat16, __nv_bfloat16)
   CCB_NN_CASE(CCB_BF16, CCB_F32, __nv_bfloat16, float)
-  CCB_NN_CASE(CCB_F16, CCB_F16, __half, __half)
-  CCB_NN_CASE(CCB_F16, CCB_F32, __half, float)
-#undef CCB_NN_CASE
 }
+#undef CCB_NN_CASE
 
 // How rows are held, the block's threads (0: rows are too long) and its shared
 // memory. `part(block, tpr)`: bytes of a slot of the ring; `vectors`: kept ones;

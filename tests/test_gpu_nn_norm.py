@@ -195,6 +195,28 @@ def test_rows_do_not_depend_on_their_neighbours_and_runs_repeat():
     assert torch.equal(y1[0], y[600]) and torch.equal(h1[0], h[600])
 
 
+@pytest.mark.parametrize("t,xt", T)
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("gate,p", [("full", 0.2), ("full", 0.0), (None, 0.2), (None, 0.0)])
+@pytest.mark.parametrize("rows,cols", [(1, 8), (70, 96), (33, 1000), (301, 1024), (9, 4096), (3, 8192)])
+def test_rows_do_not_depend_on_the_results_asked_for(t, xt, kind, gate, p, rows, cols):
+    c = Case(rows, cols, TYPES[t], TYPES[xt], kind=kind, gate=gate, act="sigmoid" if gate else "none", p=p)
+    y, h = c.forward()
+    alone = torch.empty_like(y), torch.empty_like(h)
+    nn.block_norm(c.x, alone[0], **{**c.how, "pre_weight": None})
+    nn.block_norm(c.x, h=alone[1], **c.how)
+    assert torch.equal(alone[0], y) and torch.equal(alone[1], h)
+    every = c.backward(y, c.dy, c.dh)
+    names = [n for n in every if n not in ("dpre_bias", "dpost_bias")]
+    some = {n: torch.empty_like(every[n]) for n in names}
+    ws = torch.full((nn.block_norm_backward_workspace(rows, cols),), 255, dtype=torch.uint8, device=DEV)
+    nn.block_norm_backward(y, dy=c.dy, dh=c.dh, workspace=ws, **some, **c.how)
+    assert all(torch.equal(some[n], every[n]) for n in names)
+    dx = torch.empty_like(some["dx"])
+    nn.block_norm_backward(y, dy=c.dy, dh=c.dh, dx=dx, **c.how)
+    assert torch.equal(dx, every["dx"])
+
+
 @pytest.mark.parametrize("rows,cols", [(0, 64), (2000, 64), (3000, 136), (1000, 31)])
 def test_many_or_no_rows(rows, cols):
     c = Case(rows, cols, torch.bfloat16, torch.bfloat16, gate="channel", act="tanh", bias=True)
