@@ -256,7 +256,10 @@ struct Forward {
   }
   static bool by_width(const NormP& p, int sms, cudaStream_t st) {
     if (!near({p.xs, p.bs, p.gs, p.ys, p.hs}) || (p.d.on && !p.d.same)) return false;
-    if ((p.d.base & 3) || !wide(p.cols, {p.x, p.b, p.gate, p.y, p.h}, {p.xs, p.bs, p.gs, p.ys, p.hs})) return rows<false, 1, 0>(p, sms, st);
+    // rows that share no 16-byte piece: 16 elements a thread only where 8 do not reach
+    // (4096 x 6499 bf16: 205 us, 439 by norm_any)
+    if ((p.d.base & 3) || !wide(p.cols, {p.x, p.b, p.gate, p.y, p.h}, {p.xs, p.bs, p.gs, p.ys, p.hs}))
+      return p.cols <= kRowThreads * kE ? rows<false, 1, 0>(p, sms, st) : rows<false, 2, 0>(p, sms, st);
     // What a thread does once a row (its sums, addresses, copies) is some 300
     // instructions: 16 elements share them, fewer where a warp holds the row (32
     // would spill at the registers that three rows of 4096 leave). The shape goes

@@ -92,6 +92,15 @@ def test_values_and_gradients(t, xt, kind, rows, cols):
     c.backward(y, c.dy, c.dh)
 
 
+@pytest.mark.parametrize("t,xt", T)
+@pytest.mark.parametrize("kind,gate,bias", [("rms", "full", False), ("layer", "channel", True)])
+@pytest.mark.parametrize("rows,cols", [(300, 4097), (5, 6147), (161, 6499), (4, 8191), (3, 12287)])
+def test_long_rows_of_odd_length(t, xt, kind, gate, bias, rows, cols):
+    c = Case(rows, cols, TYPES[t], TYPES[xt], kind=kind, gate=gate, act="tanh", p=0.2, bias=bias)
+    y, _ = c.forward()
+    c.backward(y, c.dy, c.dh)
+
+
 @pytest.mark.parametrize("gate,act", [(None, "none"), ("full", "none"), ("full", "tanh"), ("channel", "sigmoid"), ("channel", "none"), ("channel", "tanh")])
 @pytest.mark.parametrize("t,rows,cols", [("bf16", 65, 1024), ("f32", 17, 257), ("f16", 300, 96)])
 def test_gates(gate, act, t, rows, cols):
