@@ -289,8 +289,10 @@ constexpr int kDrain = 8, kThreads = 32 * (3 + kDrain);  // draining warps; all
 constexpr unsigned kErrWait = 16u;
 
 struct Tail {  // after the ring
-  ccb::u64 full[kStages], empty[kStages], part[kStages], accf[2], acce[2];
+  ccb::u64 full[kStages], empty[kStages], part[kStages], accf[2], acce[2], done;
   unsigned tmem;
+  unsigned stop;         // a wait ran out in either CTA: nothing more is issued
+  unsigned issued;       // stages that the producer has filled or begun to
   alignas(128) unsigned char out[kDrain][2048];  // a draining warp's 32 tokens x 32 features
   Segments g;
 };
@@ -308,6 +310,7 @@ struct P {
   int a2, b2;           // whether one copy takes two 64-wide blocks of an MN-major operand
   int box;              // rows of a copy of tokens
   int vec;              // out takes 16-byte stores
+  unsigned polls;       // of a wait, before it gives up
 };
 
 // Barriers and tiles are addressed by 32-bit shared addresses throughout: one
@@ -322,32 +325,54 @@ __device__ __forceinline__ bool try_wait(unsigned bar, unsigned parity) {
                : "memory");
   return ok != 0;
 }
-// Bounded; once a wait has run out the thread's later ones hardly poll, so
-// that the kernel ends (with the error bit raised and `out` undefined).
+// A wait of a whole warp: true once the phase is over. It is bounded: when it
+// has run out it raises the error bit and both CTAs' stop flags, which every
+// wait of either CTA looks at while it polls, and from then on each role ends at
+// its next wait that is not already over, without another copy, MMA, commit or
+// arrival; what is on its way by then is waited for at the kernel's end. A false
+// return is the same for all lanes.
 struct Waiter {
-  unsigned limit = ccb::MBAR_SPIN_LIMIT;
+  unsigned stop, peer_stop, polls;  // shared addresses of the flags
   unsigned* err;
-  __device__ __forceinline__ explicit Waiter(unsigned* e) : err(e) {}
-  __device__ __forceinline__ void operator()(unsigned bar, unsigned parity) {
-    if (try_wait(bar, parity)) return;
-    for (unsigned it = 0; it < limit; ++it)
-      if (try_wait(bar, parity)) return;
-    if (err) atomicOr(err, kErrWait);
-    limit = 64;
+  __device__ __forceinline__ bool operator()(unsigned bar, unsigned parity) const {
+    if (__all_sync(0xffffffffu, try_wait(bar, parity))) return true;
+    for (unsigned it = 0; it < polls; ++it) {
+      if (__all_sync(0xffffffffu, try_wait(bar, parity))) return true;
+      unsigned flag;
+      asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(flag) : "r"(stop) : "memory");
+      if (__any_sync(0xffffffffu, flag != 0)) return false;
+    }
+    if ((threadIdx.x & 31) == 0) {
+      if (err) atomicOr(err, kErrWait);
+      asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(stop), "r"(1) : "memory");
+      asm volatile("st.relaxed.cluster.shared::cluster.u32 [%0], %1;" ::"r"(peer_stop), "r"(1) : "memory");
+    }
+    __syncwarp();
+    return false;
   }
 };
+// The same after a stop, for what was issued before it and ends by itself.
+__device__ __forceinline__ void wait_out(unsigned bar, unsigned parity) {
+  for (unsigned it = 0; it < ccb::MBAR_SPIN_LIMIT; ++it)
+    if (try_wait(bar, parity)) return;
+}
 __device__ __forceinline__ void expect(unsigned bar, unsigned bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 // Arrivals on a barrier of either CTA. A release at cluster scope waits until
 // every earlier store of the thread, those to `out` too, has been performed,
 // some 3 us under load, so none is asked for where nothing in memory is handed
-// over: the other CTA's producer says that its copies are issued (their bytes
-// are counted by the barrier itself), a draining warp that its loads from the
-// accumulator are done (they are: tcgen05.wait::ld). The clearing warp hands
-// over shared memory that its proxy fence has already made visible.
+// over: the other CTA's producer says how many bytes its copies bring (which the
+// barrier counts itself), a draining warp that its loads from the accumulator are
+// done (they are: tcgen05.wait::ld). The clearing warp hands over its own CTA's
+// shared memory, to the CTA's own tensor core, and its proxy fence has already
+// made that visible (a release at cluster scope there: the gradient of 30
+// experts' 4096 x 1024 from 8192 rows 113 us instead of 95).
 __device__ __forceinline__ void arrive(unsigned bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void expect_relaxed(unsigned bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void arrive_relaxed(unsigned bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -365,6 +390,12 @@ __device__ __forceinline__ void mma(unsigned d, ccb::u64 a, ccb::u64 b, unsigned
   asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
                "r"(accumulate)
                : "memory");
+}
+// A word of the other CTA's shared memory.
+__device__ __forceinline__ unsigned peer_word(const unsigned* local, unsigned rank) {
+  unsigned v;
+  asm volatile("ld.volatile.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(ccb::tc2::peer_addr(local, rank)) : "memory");
+  return v;
 }
 // Operand descriptors of 16-bit tiles with the 128-byte swizzle. K-major:
 // 128-byte rows of 64 along the contraction, 8-row groups 1024 bytes apart, 16
@@ -579,6 +610,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
       mbar_init(&s.accf[i], 1);
       mbar_init(&s.acce[i], 2 * kDrain);  // the draining warps of both CTAs
     }
+    mbar_init(&s.done, 1);
+    s.stop = 0;
     mbar_fence_init();
   }
   if (warp == 0) {
@@ -590,90 +623,97 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
   tc::fence_after();
   const unsigned tmem = s.tmem;
   const unsigned tiles = tiles_of<MODE>(p, s.g);
-  Waiter wait(p.err);
+  const Waiter wait = {smem_u32(&s.stop), tc2::peer_addr(&s.stop, rank ^ 1u), p.polls, p.err};
+  const bool one = elect_one();
   const unsigned full = smem_u32(&s.full[0]), empty = smem_u32(&s.empty[0]), part = smem_u32(&s.part[0]), accf = smem_u32(&s.accf[0]),
                  acce = smem_u32(&s.acce[0]);
   const unsigned lead_full = tc2::peer_addr(&s.full[0], 0), lead_acce = tc2::peer_addr(&s.acce[0], 0);
 
+  // each role returns at its end, or when a wait says that the kernel is to stop
   if (warp == 0) {
-    const bool one = elect_one();
-    unsigned st = 0, at = ring, phase = 1;  // 8 * stage, its address
-    for (unsigned t = pair; t < tiles; t += pairs) {
-      const Tile o = tile_at<MODE>(p, s.g, t);
-      const int half = o.nn >> 1, f = o.f0 + (int)rank * 128, c = o.c0 + (int)rank * half, tok = o.r0 + (int)rank * half;
-      const int boxes = MODE == kDw ? (p.b2 ? 1 : half / 64) : (half + p.box - 1) / p.box;
-      const unsigned box = MODE == kDw ? (p.b2 ? 16384u : 8192u) : (unsigned)p.box * 128u, bytes = kABytes + boxes * box;
-      int a = o.b0;
-      do {
-        const int z = chunk_end<WIDE>(a, o.b1);
-        for (int term = 0; term < terms<WIDE>(); ++term)
-          for (int kb = a; kb < z; ++kb) {
-            wait(empty + st, phase);
-            if (one) {
-              unsigned bar = lead_full + st;
-              const int pm = plane_m<WIDE>(term), pn = plane_n<WIDE>(term);
-              if (clears<MODE>(o, kb)) {
-                bar = part + st;
-                expect(bar, bytes);
-              } else if (rank == 0) {
-                expect(full + st, 2u * bytes);
-              } else {
-                arrive_relaxed(bar);
+    unsigned st, turn;  // 8 * stage, turns of the ring
+    auto produce = [&]() {
+      unsigned at = ring, phase = 1;  // the stage's address
+      st = turn = 0;
+      for (unsigned t = pair; t < tiles; t += pairs) {
+        const Tile o = tile_at<MODE>(p, s.g, t);
+        const int half = o.nn >> 1, f = o.f0 + (int)rank * 128, c = o.c0 + (int)rank * half, tok = o.r0 + (int)rank * half;
+        const int boxes = MODE == kDw ? (p.b2 ? 1 : half / 64) : (half + p.box - 1) / p.box;
+        const unsigned box = MODE == kDw ? (p.b2 ? 16384u : 8192u) : (unsigned)p.box * 128u, bytes = kABytes + boxes * box;
+        int a = o.b0;
+        do {
+          const int z = chunk_end<WIDE>(a, o.b1);
+          for (int term = 0; term < terms<WIDE>(); ++term)
+            for (int kb = a; kb < z; ++kb) {
+              if (!wait(empty + st, phase)) return;
+              if (one) {
+                unsigned bar = lead_full + st;
+                const int pm = plane_m<WIDE>(term), pn = plane_n<WIDE>(term);
+                if (clears<MODE>(o, kb)) {
+                  bar = part + st;
+                  expect(bar, bytes);
+                } else if (rank == 0) {
+                  expect(full + st, bytes);
+                } else {
+                  expect_relaxed(bar, bytes);
+                }
+                const int k0 = kb * kBK;
+                unsigned sb = at + kABytes;
+                if (MODE == kDw) {
+                  const int r = o.r0 + k0;
+                  if (p.a2) {
+                    load4(at, &p.ta, 0, r, f >> 6, pm, bar);
+                  } else {
+                    load4(at, &p.ta, f, r, pm, 0, bar);
+                    load4(at + 8192u, &p.ta, f + 64, r, pm, 0, bar);
+                  }
+                  if (p.b2) {
+                    load4(sb, &p.tb, 0, r, c >> 6, pn, bar);
+                  } else {
+                    load4(sb, &p.tb, c, r, pn, 0, bar);
+                    if (boxes > 1) load4(sb + 8192u, &p.tb, c + 64, r, pn, 0, bar);
+                  }
+                } else {
+                  const int e = pm * p.experts + o.expert;
+                  if (MODE == kForwardT) {
+                    load4(at, &p.ta, k0, f, e, 0, bar);
+                  } else if (p.a2) {
+                    load4(at, &p.ta, 0, k0, f >> 6, e, bar);
+                  } else {
+                    load4(at, &p.ta, f, k0, e, 0, bar);
+                    load4(at + 8192u, &p.ta, f + 64, k0, e, 0, bar);
+                  }
+                  load4(sb, &p.tb, k0, tok, pn, 0, bar);
+                  for (int i = 1; i < boxes; ++i) {
+                    sb += box;
+                    load4(sb, &p.tb, k0, tok + i * p.box, pn, 0, bar);
+                  }
+                }
               }
-              const int k0 = kb * kBK;
-              unsigned sb = at + kABytes;
-              if (MODE == kDw) {
-                const int r = o.r0 + k0;
-                if (p.a2) {
-                  load4(at, &p.ta, 0, r, f >> 6, pm, bar);
-                } else {
-                  load4(at, &p.ta, f, r, pm, 0, bar);
-                  load4(at + 8192u, &p.ta, f + 64, r, pm, 0, bar);
-                }
-                if (p.b2) {
-                  load4(sb, &p.tb, 0, r, c >> 6, pn, bar);
-                } else {
-                  load4(sb, &p.tb, c, r, pn, 0, bar);
-                  if (boxes > 1) load4(sb + 8192u, &p.tb, c + 64, r, pn, 0, bar);
-                }
-              } else {
-                const int e = pm * p.experts + o.expert;
-                if (MODE == kForwardT) {
-                  load4(at, &p.ta, k0, f, e, 0, bar);
-                } else if (p.a2) {
-                  load4(at, &p.ta, 0, k0, f >> 6, e, bar);
-                } else {
-                  load4(at, &p.ta, f, k0, e, 0, bar);
-                  load4(at + 8192u, &p.ta, f + 64, k0, e, 0, bar);
-                }
-                load4(sb, &p.tb, k0, tok, pn, 0, bar);
-                for (int i = 1; i < boxes; ++i) {
-                  sb += box;
-                  load4(sb, &p.tb, k0, tok + i * p.box, pn, 0, bar);
-                }
+              __syncwarp();
+              st += 8;
+              at += kStageBytes;
+              if (st == 8 * kStages) {
+                st = 0;
+                at = ring;
+                phase ^= 1u;
+                ++turn;
               }
             }
-            __syncwarp();
-            st += 8;
-            at += kStageBytes;
-            if (st == 8 * kStages) {
-              st = 0;
-              at = ring;
-              phase ^= 1u;
-            }
-          }
-        a = z;
-      } while (a < o.b1);
-    }
+          a = z;
+        } while (a < o.b1);
+      }
+    };
+    produce();
+    if (lane == 0) s.issued = turn * kStages + (st >> 3);
   } else if (warp == 1) {
-    if (rank == 0) {
+    auto multiply = [&]() {
       constexpr bool amn = MODE != kForwardT, bmn = MODE == kDw;
-      const bool one = elect_one();
       const unsigned base = (1u << 4) | ((unsigned)p.format << 7) | ((unsigned)p.format << 10) | ((amn ? 1u : 0u) << 15) | ((bmn ? 1u : 0u) << 16) | (16u << 24);
       const u64 a0 = desc<amn>(ring), b0 = desc<bmn>(ring + kABytes);
       const unsigned empty0 = tc2::peer_addr(&s.empty[0], 0), empty1 = tc2::peer_addr(&s.empty[0], 1);
       const unsigned accf0 = tc2::peer_addr(&s.accf[0], 0), accf1 = tc2::peer_addr(&s.accf[0], 1);
-      unsigned st = 0, phase = 0, it = 0;
+      unsigned at = 0, phase = 0, it = 0;
       u64 a = a0, bd = b0;
       for (unsigned t = pair; t < tiles; t += pairs) {
         const Tile o = tile_at<MODE>(p, s.g, t);
@@ -682,12 +722,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
         do {
           const int to = chunk_end<WIDE>(from, o.b1);
           const unsigned ab = it & 1u, d = tmem + ab * kTok;
-          wait(acce + 8 * ab, ((it >> 1) & 1u) ^ 1u);
+          if (!wait(acce + 8 * ab, ((it >> 1) & 1u) ^ 1u)) return;
           tc::fence_after();
           for (int term = 0; term < terms<WIDE>(); ++term)
             for (int kb = from; kb < to; ++kb) {
               const unsigned more = term > 0 || kb > from ? 1u : 0u;
-              wait(full + st, phase);
+              if (!wait(full + at, phase)) return;
               tc::fence_after();
               if (one) {
                 if (clears<MODE>(o, kb)) {
@@ -697,15 +737,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
 #pragma unroll
                   for (int kk = 0; kk < kBK / 16; ++kk) mma(d, a + kk * desc_step<amn>(), bd + kk * desc_step<bmn>(), idesc, kk > 0 ? 1u : more);
                 }
-                commit(empty0 + st);
-                commit(empty1 + st);
+                commit(empty0 + at);
+                commit(empty1 + at);
               }
               __syncwarp();
-              st += 8;
+              at += 8;
               a += kStageBytes >> 4;
               bd += kStageBytes >> 4;
-              if (st == 8 * kStages) {
-                st = 0;
+              if (at == 8 * kStages) {
+                at = 0;
                 a = a0;
                 bd = b0;
                 phase ^= 1u;
@@ -720,108 +760,162 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
           from = to;
         } while (from < o.b1);
       }
-    }
+    };
+    if (rank == 0) multiply();
   } else if (warp < 2 + kDrain) {
-    const int q = warp & 3, other = (warp - 2) >> 2;  // its quarter of the lanes; every other 32 columns
-    unsigned it = 0;
-    for (unsigned t = pair; t < tiles; t += pairs) {
-      const Tile o = tile_at<MODE>(p, s.g, t);
-      const int f = o.f0 + (int)rank * 128 + q * 32;
-      const int count = MODE == kDw ? min(p.k - o.c0, o.nn) : o.r1 - o.r0;
-      TO* out = static_cast<TO*>(p.out) + o.split * p.split_stride + f + (MODE == kDw ? o.expert * p.oe + (i64)o.c0 * p.os : (i64)o.r0 * p.os);
-      const unsigned acc0 = tmem + ((unsigned)(q * 32) << 16);
-      if constexpr (WIDE) {
-        float sum[kTok / 64][32];
+    auto drain = [&]() {
+      const int q = warp & 3, other = (warp - 2) >> 2;  // its quarter of the lanes; every other 32 columns
+      unsigned it = 0;
+      for (unsigned t = pair; t < tiles; t += pairs) {
+        const Tile o = tile_at<MODE>(p, s.g, t);
+        const int f = o.f0 + (int)rank * 128 + q * 32;
+        const int count = MODE == kDw ? min(p.k - o.c0, o.nn) : o.r1 - o.r0;
+        TO* out = static_cast<TO*>(p.out) + o.split * p.split_stride + f + (MODE == kDw ? o.expert * p.oe + (i64)o.c0 * p.os : (i64)o.r0 * p.os);
+        const unsigned acc0 = tmem + ((unsigned)(q * 32) << 16);
+        if constexpr (WIDE) {
+          float sum[kTok / 64][32];
 #pragma unroll
-        for (int g = 0; g < kTok / 64; ++g)
+          for (int g = 0; g < kTok / 64; ++g)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) sum[g][i] = 0.0f;
-        int a = o.b0;
-        do {
-          const unsigned ab = it & 1u;
-          wait(accf + 8 * ab, (it >> 1) & 1u);
-          __syncwarp();
-          tc::fence_after();
-          if (f < p.n && a < o.b1) {
+            for (int i = 0; i < 32; ++i) sum[g][i] = 0.0f;
+          int a = o.b0;
+          do {
+            const unsigned ab = it & 1u;
+            if (!wait(accf + 8 * ab, (it >> 1) & 1u)) return;
+            tc::fence_after();
+            if (f < p.n && a < o.b1) {
+#pragma unroll
+              for (int g = 0; g < kTok / 64; ++g) {
+                const int c = 32 * other + 64 * g;
+                if (c < count) {
+                  float v[32];
+                  __syncwarp();
+                  tc::ld32(acc0 + ab * kTok + c, v);
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) sum[g][i] += v[i];
+                }
+              }
+            }
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_relaxed(lead_acce + 8 * ab);
+            ++it;
+            a = chunk_end<WIDE>(a, o.b1);
+          } while (a < o.b1);
+          if (f < p.n) {
 #pragma unroll
             for (int g = 0; g < kTok / 64; ++g) {
               const int c = 32 * other + 64 * g;
-              if (c < count) {
-                float v[32];
-                __syncwarp();
-                tc::ld32(acc0 + ab * kTok + c, v);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) sum[g][i] += v[i];
-              }
+              if (c < count) store32(sum[g], out + c * p.os, p.os, count - c, p.n - f, lane);
+            }
+          }
+        } else {
+          const unsigned ab = it & 1u;
+          if (!wait(accf + 8 * ab, (it >> 1) & 1u)) return;
+          tc::fence_after();
+          if (f < p.n) {
+            for (int c = 32 * other; c < count; c += 32 * (kDrain / 4)) {
+              if constexpr (sizeof(TO) == 2)
+                drain16<TO>(acc0 + ab * kTok + c, o.b0 >= o.b1, smem_u32(s.out[warp - 2]), out + c * p.os, p.os, count - c, p.n - f, p.vec, lane);
+              else
+                drain32(acc0 + ab * kTok + c, o.b0 >= o.b1, out + c * p.os, p.os, count - c, p.n - f, lane);
+              __syncwarp();
             }
           }
           tc::fence_before();
           __syncwarp();
           if (lane == 0) arrive_relaxed(lead_acce + 8 * ab);
           ++it;
-          a = chunk_end<WIDE>(a, o.b1);
-        } while (a < o.b1);
-        if (f < p.n) {
-#pragma unroll
-          for (int g = 0; g < kTok / 64; ++g) {
-            const int c = 32 * other + 64 * g;
-            if (c < count) store32(sum[g], out + c * p.os, p.os, count - c, p.n - f, lane);
-          }
         }
-      } else {
-        const unsigned ab = it & 1u;
-        wait(accf + 8 * ab, (it >> 1) & 1u);
-        __syncwarp();
-        tc::fence_after();
-        if (f < p.n) {
-          for (int c = 32 * other; c < count; c += 32 * (kDrain / 4)) {
-            if constexpr (sizeof(TO) == 2)
-              drain16<TO>(acc0 + ab * kTok + c, o.b0 >= o.b1, smem_u32(s.out[warp - 2]), out + c * p.os, p.os, count - c, p.n - f, p.vec, lane);
-            else
-              drain32(acc0 + ab * kTok + c, o.b0 >= o.b1, out + c * p.os, p.os, count - c, p.n - f, lane);
-            __syncwarp();
-          }
-        }
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_relaxed(lead_acce + 8 * ab);
-        ++it;
       }
-    }
+    };
+    drain();
   } else if (MODE == kDw) {
     // a lane has one 16-byte piece of each row: two 64-wide blocks of the M side, then the N side's
-    unsigned stage = 0, phases = 0;  // bit i: parity of part[i]
-    for (unsigned t = pair; t < tiles; t += pairs) {
-      const Tile o = tile_at<MODE>(p, s.g, t);
-      int a = o.b0;
-      do {
-        const int z = chunk_end<WIDE>(a, o.b1);
-        for (int term = 0; term < terms<WIDE>(); ++term)
-          for (int kb = a; kb < z; ++kb) {
-            if (clears<MODE>(o, kb)) {
-              wait(part + 8 * stage, (phases >> stage) & 1u);
-              __syncwarp();
-              phases ^= 1u << stage;
-              const int left = o.r1 - o.r0 - kb * kBK, to = (left + 15) & ~15;
-              uint4* at = reinterpret_cast<uint4*>(smem + pad + stage * kStageBytes + (lane >> 3) * 8192 + (lane & 7) * 16);
-              for (int r = left; r < to; ++r) at[r * 8] = make_uint4(0, 0, 0, 0);
-              asm volatile("fence.proxy.async;" ::: "memory");
-              __syncwarp();
-              if (lane == 0) arrive(lead_full + 8 * stage);
+    auto clear_rows = [&]() {
+      unsigned stage = 0, phases = 0;  // bit i: parity of part[i]
+      for (unsigned t = pair; t < tiles; t += pairs) {
+        const Tile o = tile_at<MODE>(p, s.g, t);
+        int a = o.b0;
+        do {
+          const int z = chunk_end<WIDE>(a, o.b1);
+          for (int term = 0; term < terms<WIDE>(); ++term)
+            for (int kb = a; kb < z; ++kb) {
+              if (clears<MODE>(o, kb)) {
+                if (!wait(part + 8 * stage, (phases >> stage) & 1u)) return;
+                phases ^= 1u << stage;
+                const int left = o.r1 - o.r0 - kb * kBK, to = (left + 15) & ~15;
+                uint4* at = reinterpret_cast<uint4*>(smem + pad + stage * kStageBytes + (lane >> 3) * 8192 + (lane & 7) * 16);
+                for (int r = left; r < to; ++r) at[r * 8] = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) arrive(lead_full + 8 * stage);
+              }
+              stage = stage + 1 == kStages ? 0 : stage + 1;
             }
-            stage = stage + 1 == kStages ? 0 : stage + 1;
-          }
-        a = z;
-      } while (a < o.b1);
-    }
+          a = z;
+        } while (a < o.b1);
+      }
+    };
+    clear_rows();
   }
-  if (wait.limit < MBAR_SPIN_LIMIT)  // a wait ran out: copies may be on their way yet
-    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
   __syncwarp();
   tc::fence_before();
   __syncthreads();
   tc2::cluster_sync();
   tc::fence_after();
+  if (s.stop) {  // in both CTAs or in neither
+    // Every role has ended. What is on its way: the MMAs, whose commit says when
+    // they are over, and the copies. Those into a stage that is cleared complete
+    // on the CTA's own barrier, the others on the even CTA's, whose phase ends
+    // with an announcement by each producer and all bytes announced; where one
+    // producer got further than the other (by at most the ring), the other
+    // announces none for the stages in between.
+    if (warp == 1) {
+      if (rank == 0 && one) {
+        commit(tc2::peer_addr(&s.done, 0));
+        commit(tc2::peer_addr(&s.done, 1));
+      }
+      __syncwarp();
+      wait_out(smem_u32(&s.done), 0);
+    }
+    if (warp == 0 && lane == 0) {
+      const unsigned mine = s.issued, other = peer_word(&s.issued, rank ^ 1u), last = mine > other ? mine : other;
+      // which of the stages' last copies are of rows that are cleared, and what each barrier `part` of this CTA has counted
+      unsigned clear = 0, armed = 0, odd = 0;
+      if (MODE == kDw) {
+        unsigned j = 0;
+        for (unsigned t = pair; t < tiles && j < last; t += pairs) {
+          const Tile o = tile_at<MODE>(p, s.g, t);
+          int a = o.b0;
+          do {
+            const int z = chunk_end<WIDE>(a, o.b1);
+            for (int term = 0; term < terms<WIDE>(); ++term)
+              for (int kb = a; kb < z && j < last; ++kb, ++j) {
+                const unsigned bit = 1u << (j % kStages);
+                clear = clears<MODE>(o, kb) ? clear | bit : clear & ~bit;
+                if (clears<MODE>(o, kb) && j < mine) {
+                  armed |= bit;
+                  odd ^= bit;
+                }
+              }
+            a = z;
+          } while (a < o.b1);
+        }
+      }
+      for (unsigned i = 0; i < kStages; ++i)
+        if ((armed >> i) & 1u) wait_out(part + 8 * i, ((odd >> i) & 1u) ^ 1u);
+      for (unsigned j = mine; j < other; ++j)
+        if (!((clear >> (j % kStages)) & 1u)) arrive(lead_full + 8 * (j % kStages));
+      if (rank == 0)
+        for (unsigned j = last > kStages ? last - kStages : 0; j < last; ++j)
+          if (!((clear >> (j % kStages)) & 1u)) wait_out(full + 8 * (j % kStages), (j / kStages) & 1u);
+    }
+    __syncwarp();
+    __syncthreads();
+    tc2::cluster_sync();
+    tc::fence_after();
+  }
   __syncwarp();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
@@ -1125,6 +1219,8 @@ bool encode_mn(ccb::TmaDesc* m, int fmt, const void* base, i64 cols, i64 rows, i
   return tcg::encode(m, fmt, base, 4, d, st, box);
 }
 
+unsigned wait_polls = ccb::MBAR_SPIN_LIMIT;  // ccb_nn_wait_polls
+
 // The parts that both directions share.
 tcg::P tensor_params(const Plan& plan, const int* off, unsigned* err, int dtype, i64 rows, i64 experts, i64 k, i64 n) {
   tcg::P p = {};
@@ -1136,6 +1232,7 @@ tcg::P tensor_params(const Plan& plan, const int* off, unsigned* err, int dtype,
   p.k = (int)k;
   p.splits = plan.parts;
   p.format = dtype != CCB_F16;
+  p.polls = __atomic_load_n(&wait_polls, __ATOMIC_RELAXED);
   return p;
 }
 
@@ -1298,4 +1395,9 @@ extern "C" int ccb_nn_grouped_matmul_dw(const ccb_nn_grouped_matmul_dw_t* a, voi
     if (plan.tensor) return tensor_dw(a, plan, sms, st, me);
     return clear(a->out_dtype, a->out, a->experts, a->k, a->n, a->out_stride, a->out_row_stride, a->offsets, a->experts, a->rows, a->err, sms, st, me);
   })
+}
+
+extern "C" int ccb_nn_wait_polls(unsigned polls) {
+  __atomic_store_n(&wait_polls, polls ? polls : ccb::MBAR_SPIN_LIMIT, __ATOMIC_RELAXED);
+  return CCB_OK;
 }

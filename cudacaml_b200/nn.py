@@ -427,7 +427,8 @@ def grouped_matmul(x, w, offsets, out, *, transpose_w=False, workspace=None, err
     (or [experts, n, k] with ``transpose_w``), out [rows, n], all of one type;
     ``offsets`` is experts + 1 ascending i32 words in device memory that the
     host does not read. Words out of order or range are clamped and raise bit
-    64 of the 32-bit word ``err``. The gradient of x is the same call on dy
+    64 of the 32-bit word ``err``; bit 16 says that a wait inside the kernel ran
+    out and ``out`` is undefined. The gradient of x is the same call on dy
     with ``transpose_w`` flipped, that of w is ``grouped_matmul_dw``."""
     _call("ccb_nn_grouped_matmul", _grouped_args(x, w, offsets, out, transpose_w, workspace, err), stream)
 
@@ -459,3 +460,12 @@ def grouped_matmul_dw(x, dy, offsets, out, *, workspace=None, err=None, stream=N
     gradient of ``grouped_matmul``'s w ([experts, k, n]; for a transposed w
     swap x and dy). out has x's type or f32."""
     _call("ccb_nn_grouped_matmul_dw", _dw_args(x, dy, offsets, out, workspace, err), stream)
+
+
+def wait_polls(polls: int = 0) -> None:
+    """How often a wait inside the grouped products polls before it gives up
+    (bit 16 of ``err``, the output undefined, the stream usable), for the calls
+    that follow; 0 is the default, 2**22."""
+    if not 0 <= polls < 1 << 32:
+        raise ValueError(f"nn.wait_polls: {polls} is outside [0, 2^32)")
+    R.check((R._LIB or R.lib()).ccb_nn_wait_polls(polls))

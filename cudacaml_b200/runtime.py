@@ -122,6 +122,7 @@ def _declare(L):
         "ccb_nn_grouped_matmul_workspace": (I, [P, c.POINTER(SZ)]),
         "ccb_nn_grouped_matmul_dw": (I, [P, P]),
         "ccb_nn_grouped_matmul_dw_workspace": (I, [P, c.POINTER(SZ)]),
+        "ccb_nn_wait_polls": (I, [c.c_uint]),
         "ccb_ipc_mem_handle": (I, [P, c.POINTER(c.c_ubyte)]),
         "ccb_ipc_mem_open": (I, [c.POINTER(c.c_ubyte), c.POINTER(P)]),
         "ccb_ipc_mem_close": (I, [P]),

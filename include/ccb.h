@@ -317,8 +317,9 @@ int ccb_nn_block_norm_backward_workspace(long long rows, long long cols, size_t*
  * Rows before offsets[0] and from offsets[experts] on give 0. `offsets` is
  * experts + 1 i32 words in device memory, ascending, in [0, rows]: the host
  * never learns them. Words out of order or range are clamped and raise bit 64
- * of *err; a wait that ran out raises bit 16 (err may be NULL). Matrix e of w
- * starts w_stride * e elements in, its rows w_row_stride apart. At most 1024
+ * of *err; a wait inside the kernel that ran out raises bit 16: the kernel
+ * then ends, out is undefined, the device and the stream stay usable (err may
+ * be NULL). Matrix e of w starts w_stride * e elements in, its rows w_row_stride apart. At most 1024
  * experts and 2^31 - 1025 rows. f32 products are sums of 16-bit products on the
  * tensor cores, as exact as f32 arithmetic, but an infinite operand may give
  * NaN where f32 arithmetic gives an infinity. The gradient
@@ -352,6 +353,10 @@ typedef struct {
 } ccb_nn_grouped_matmul_dw_t;
 int ccb_nn_grouped_matmul_dw(const ccb_nn_grouped_matmul_dw_t* a, void* stream);
 int ccb_nn_grouped_matmul_dw_workspace(const ccb_nn_grouped_matmul_dw_t* a, size_t* bytes);
+
+/* How often a wait inside the grouped products polls before it gives up, for
+ * the calls that this process issues from here on; 0: the default, 2^22. */
+int ccb_nn_wait_polls(unsigned polls);
 
 /* ---------------------------------------------------------------- peer memory and the cross-rank sum
  * New: the reference has no collective (lib/backend_cuda/multi.ml:51-109

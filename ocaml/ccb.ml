@@ -326,6 +326,8 @@ let nn_grouped_matmul_dw = fn "ccb_nn_grouped_matmul_dw" (ptr nn_grouped_matmul_
 let nn_grouped_matmul_dw_workspace =
   fn "ccb_nn_grouped_matmul_dw_workspace" (ptr nn_grouped_matmul_dw_t @-> ptr size_t @-> returning int)
 
+let nn_wait_polls = fn "ccb_nn_wait_polls" (uint @-> returning int)
+
 (* ---------------------------------------------------------------- peer memory and the cross-rank sum
    (no reference counterpart) *)
 let ipc_mem_handle = fn "ccb_ipc_mem_handle" (ptr void @-> ptr uchar @-> returning int)
