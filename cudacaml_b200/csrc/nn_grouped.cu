@@ -525,14 +525,20 @@ struct Tile {
 };
 // f32 operands are sums hi + mid + lo of three 16-bit planes (WIDE), and a
 // product is the six of their products down to 2^-16 of the largest, added up
-// from the smallest. The accumulator truncates: over a long contraction that
-// is a bias of some 2^-25 of it for each MMA, so a tile's contraction is cut
-// into chunks of kChunk steps, each summed from 0 in its six terms, and the
-// draining warps add the chunks up in registers, rounding to nearest (the
-// error against 64 bits at K = 1024: 1.0e-6 in one go, see below by chunks).
-constexpr int kChunk = 4;
-template <bool WIDE>
-__device__ __forceinline__ int chunk_end(int a, int b1) { return WIDE ? min(a + kChunk, b1) : b1; }
+// from the smallest.
+//
+// The accumulator truncates. Over a contraction of one sign that is a bias, of
+// about 2^-23.4 of the sum so far for each MMA of bf16 and 2^-22.2 of f16: 8e-5
+// and 1e-4 after 16384. Where the result is F32 and a contraction may be long
+// (w's gradient; f32 operands), it is cut into chunks, each summed from 0 (in
+// its six terms), and the draining warps add the chunks up in registers,
+// rounding to nearest. Reading an accumulator takes some 370 cycles from the
+// MMAs (their operands and it share tensor memory): one expert's 4096 x 4096 from
+// 16384 rows takes 368 us in one go, 387 by chunks of 8 steps (512 rows), 412 of
+// 4; the six terms of an f32 step make a chunk long enough at 4.
+enum { kWhole = 0, kChunk = 8, kChunkWide = 4 };
+template <int CHUNK>
+__device__ __forceinline__ int chunk_end(int a, int b1) { return CHUNK ? min(a + CHUNK, b1) : b1; }
 template <bool WIDE>
 __device__ __forceinline__ constexpr int terms() { return WIDE ? 6 : 1; }
 // The planes of a term.
@@ -591,6 +597,7 @@ __device__ __forceinline__ bool clears(const Tile& o, int kb) {
 template <class TO, int MODE, bool WIDE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped_tc(const __grid_constant__ P p) {
   using namespace ccb;
+  constexpr int CHUNK = WIDE ? kChunkWide : MODE == kDw && sizeof(TO) == 4 ? kChunk : kWhole;
   extern __shared__ __align__(1024) unsigned char smem[];
   const unsigned raw = smem_u32(smem), pad = (1024u - (raw & 1023u)) & 1023u;
   const unsigned ring = raw + pad;
@@ -642,7 +649,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
         const unsigned box = MODE == kDw ? (p.b2 ? 16384u : 8192u) : (unsigned)p.box * 128u, bytes = kABytes + boxes * box;
         int a = o.b0;
         do {
-          const int z = chunk_end<WIDE>(a, o.b1);
+          const int z = chunk_end<CHUNK>(a, o.b1);
           for (int term = 0; term < terms<WIDE>(); ++term)
             for (int kb = a; kb < z; ++kb) {
               if (!wait(empty + st, phase)) return;
@@ -720,7 +727,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
         const unsigned idesc = base | ((unsigned)(o.nn >> 3) << 17);
         int from = o.b0;
         do {
-          const int to = chunk_end<WIDE>(from, o.b1);
+          const int to = chunk_end<CHUNK>(from, o.b1);
           const unsigned ab = it & 1u, d = tmem + ab * kTok;
           if (!wait(acce + 8 * ab, ((it >> 1) & 1u) ^ 1u)) return;
           tc::fence_after();
@@ -772,7 +779,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
         const int count = MODE == kDw ? min(p.k - o.c0, o.nn) : o.r1 - o.r0;
         TO* out = static_cast<TO*>(p.out) + o.split * p.split_stride + f + (MODE == kDw ? o.expert * p.oe + (i64)o.c0 * p.os : (i64)o.r0 * p.os);
         const unsigned acc0 = tmem + ((unsigned)(q * 32) << 16);
-        if constexpr (WIDE) {
+        if (CHUNK != kWhole && (WIDE || o.b1 - o.b0 > CHUNK)) {
           float sum[kTok / 64][32];
 #pragma unroll
           for (int g = 0; g < kTok / 64; ++g)
@@ -800,7 +807,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
             __syncwarp();
             if (lane == 0) arrive_relaxed(lead_acce + 8 * ab);
             ++it;
-            a = chunk_end<WIDE>(a, o.b1);
+            a = chunk_end<CHUNK>(a, o.b1);
           } while (a < o.b1);
           if (f < p.n) {
 #pragma unroll
@@ -809,24 +816,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
               if (c < count) store32(sum[g], out + c * p.os, p.os, count - c, p.n - f, lane);
             }
           }
-        } else {
-          const unsigned ab = it & 1u;
-          if (!wait(accf + 8 * ab, (it >> 1) & 1u)) return;
-          tc::fence_after();
-          if (f < p.n) {
-            for (int c = 32 * other; c < count; c += 32 * (kDrain / 4)) {
-              if constexpr (sizeof(TO) == 2)
-                drain16<TO>(acc0 + ab * kTok + c, o.b0 >= o.b1, smem_u32(s.out[warp - 2]), out + c * p.os, p.os, count - c, p.n - f, p.vec, lane);
-              else
-                drain32(acc0 + ab * kTok + c, o.b0 >= o.b1, out + c * p.os, p.os, count - c, p.n - f, lane);
-              __syncwarp();
-            }
-          }
-          tc::fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_relaxed(lead_acce + 8 * ab);
-          ++it;
+          continue;
         }
+        const unsigned ab = it & 1u;
+        if (!wait(accf + 8 * ab, (it >> 1) & 1u)) return;
+        tc::fence_after();
+        if (f < p.n) {
+          for (int c = 32 * other; c < count; c += 32 * (kDrain / 4)) {
+            if constexpr (sizeof(TO) == 2)
+              drain16<TO>(acc0 + ab * kTok + c, o.b0 >= o.b1, smem_u32(s.out[warp - 2]), out + c * p.os, p.os, count - c, p.n - f, p.vec, lane);
+            else
+              drain32(acc0 + ab * kTok + c, o.b0 >= o.b1, out + c * p.os, p.os, count - c, p.n - f, lane);
+            __syncwarp();
+          }
+        }
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_relaxed(lead_acce + 8 * ab);
+        ++it;
       }
     };
     drain();
@@ -838,7 +845,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
         const Tile o = tile_at<MODE>(p, s.g, t);
         int a = o.b0;
         do {
-          const int z = chunk_end<WIDE>(a, o.b1);
+          const int z = chunk_end<CHUNK>(a, o.b1);
           for (int term = 0; term < terms<WIDE>(); ++term)
             for (int kb = a; kb < z; ++kb) {
               if (clears<MODE>(o, kb)) {
@@ -889,7 +896,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
           const Tile o = tile_at<MODE>(p, s.g, t);
           int a = o.b0;
           do {
-            const int z = chunk_end<WIDE>(a, o.b1);
+            const int z = chunk_end<CHUNK>(a, o.b1);
             for (int term = 0; term < terms<WIDE>(); ++term)
               for (int kb = a; kb < z && j < last; ++kb, ++j) {
                 const unsigned bit = 1u << (j % kStages);

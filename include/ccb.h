@@ -324,7 +324,9 @@ int ccb_nn_block_norm_backward_workspace(long long rows, long long cols, size_t*
  * tensor cores, as exact as f32 arithmetic, but an infinite operand may give
  * NaN where f32 arithmetic gives an infinity. The gradient
  * of x is the same call on dy with transpose_w flipped. Sums are in 32 bits,
- * the same bits in every run. workspace: at least
+ * the same bits in every run; those of a 16-bit result are the tensor cores'
+ * accumulator's, which truncates: k terms of one sign come out low by up to
+ * some k * 6e-9 of their sum (1e-4 at 16384). workspace: at least
  * ccb_nn_grouped_matmul_workspace bytes, 16-byte aligned, uninitialised. */
 typedef struct {
   const void *x, *w;
@@ -341,7 +343,9 @@ int ccb_nn_grouped_matmul(const ccb_nn_grouped_matmul_t* a, void* stream);
 int ccb_nn_grouped_matmul_workspace(const ccb_nn_grouped_matmul_t* a, size_t* bytes);
 
 /* The gradient of w: matrix e of out (k x n) = (x rows of e)^T (dy rows of e),
- * 0 for an expert without rows. out has dtype or f32 (out_dtype). */
+ * 0 for an expert without rows. out has dtype or f32 (out_dtype); the sums of
+ * an f32 result are rounded to nearest every 512 rows and do not lose more the
+ * more rows there are. */
 typedef struct {
   const void *x, *dy;
   const int* offsets;
