@@ -48,9 +48,11 @@ def squared_error(shape) -> Graph:
     return Grad.grad(Graph("mse", [("loss", loss)]), "loss", ["out"])
 
 
-def descent(shape, rate: float) -> Graph:
+def descent(shape, rate=None) -> Graph:
+    """q = p - rate * g; the rate is the scalar parameter ``rate``, or a number built into the graph."""
     p, g = D.param("p", F32, shape), D.param("g", F32, shape)
-    return Graph("sgd", [("q", D.map2(lambda a, b: D.sub(a, D.mul(D.const(F32, rate), b)), p, g))])
+    r = D.broadcast(shape, D.scalar("rate", F32)) if rate is None else D.full(F32, shape, rate)
+    return Graph("sgd", [("q", D.map2(D.sub, p, D.map2(D.mul, r, g)))])
 
 
 class ExpertBlock:
@@ -66,7 +68,7 @@ class ExpertBlock:
             self.stream = R.Stream()
             self.buf = {n: R.Buffer(4 * numel(s)) for n, s in self.shapes.items()}
             self.buf.update({n + "'": R.Buffer(4 * numel(self.shapes[n])) for n in self.WEIGHTS})  # the update writes beside
-            self.buf["offsets"], self.buf["err"] = R.Buffer(4 * (experts + 1)), R.Buffer(4)
+            self.buf["offsets"], self.buf["err"], self.buf["rate"] = R.Buffer(4 * (experts + 1)), R.Buffer(4), R.Buffer(4)
             self.offsets = nn.Array(self.buf["offsets"].ptr, "i32", (experts + 1,))
             R.check(R.lib().ccb_memset_d8(self.buf["err"].ptr, 0, 4, self.stream.h))
             need = [nn.block_norm_backward_workspace(tokens, dim)]
@@ -77,6 +79,8 @@ class ExpertBlock:
             self.space = R.Buffer(max(need))
         self.graphs = {"act": cuda.compile_on(device, activation(wide)), "act_grad": cuda.compile_on(device, activation_grad(wide)),
                        "loss": cuda.compile_on(device, squared_error(act))}
+        self.graphs.update({s: cuda.compile_on(device, descent(s)) for s in {self.shapes[n] for n in self.WEIGHTS}})
+        self.rate = None  # the one on the device
 
     def __getitem__(self, name) -> nn.Array:
         return nn.Array(self.buf[name].ptr, "f32", self.shapes[name])
@@ -130,11 +134,11 @@ class ExpertBlock:
     def update(self, rate: float) -> None:
         """One step of gradient descent on every parameter, and the next step's masks."""
         with R.with_device(self.device):
+            if rate != self.rate:
+                self.buf["rate"].upload(np.array([rate], np.float32), self.stream.h)
+                self.rate = rate
             for n in self.WEIGHTS:
-                key = (n, rate)
-                if key not in self.graphs:
-                    self.graphs[key] = cuda.compile_on(self.device, descent(self.shapes[n], rate))
-                self._graph(key, {"p": n, "g": "d" + n}, {"q": n + "'"})
+                self._graph(self.shapes[n], {"p": n, "g": "d" + n, "rate": "rate"}, {"q": n + "'"})
                 self.buf[n], self.buf[n + "'"] = self.buf[n + "'"], self.buf[n]
         self.step_no += 1
 
