@@ -24,7 +24,7 @@ from . import examples as X
 from . import grad as Grad
 from . import nn
 from . import runtime as R
-from .ir import F32, Graph, numel
+from .ir import F32, I32, Graph, numel
 
 
 def activation(shape) -> Graph:
@@ -49,10 +49,12 @@ def squared_error(shape) -> Graph:
 
 
 def descent(shape, rate=None) -> Graph:
-    """q = p - rate * g; the rate is the scalar parameter ``rate``, or a number built into the graph."""
+    """q = p - rate * g, or p where the scalar parameter ``err`` is not 0 (whatever g
+    holds); the rate is the scalar parameter ``rate``, or a number built into the graph."""
     p, g = D.param("p", F32, shape), D.param("g", F32, shape)
     r = D.broadcast(shape, D.scalar("rate", F32)) if rate is None else D.full(F32, shape, rate)
-    return Graph("sgd", [("q", D.map2(D.sub, p, D.map2(D.mul, r, g)))])
+    step = D.map2(lambda e, s: D.select(D.eq(e, D.const(I32, 0)), s, D.const(F32, 0.0)), D.broadcast(shape, D.scalar("err", I32)), D.map2(D.mul, r, g))
+    return Graph("sgd", [("q", D.map2(D.sub, p, step))])
 
 
 class ExpertBlock:
@@ -132,22 +134,25 @@ class ExpertBlock:
                                    workspace=self.space, stream=s)
 
     def update(self, rate: float) -> None:
-        """One step of gradient descent on every parameter, and the next step's masks."""
+        """One step of gradient descent on every parameter, and the next step's masks. While a device check of the
+        products has failed and ``loss`` has not reported it, the parameters stay as they are."""
         with R.with_device(self.device):
             if rate != self.rate:
                 self.buf["rate"].upload(np.array([rate], np.float32), self.stream.h)
                 self.rate = rate
             for n in self.WEIGHTS:
-                self._graph(self.shapes[n], {"p": n, "g": "d" + n, "rate": "rate"}, {"q": n + "'"})
+                self._graph(self.shapes[n], {"p": n, "g": "d" + n, "rate": "rate", "err": "err"}, {"q": n + "'"})
                 self.buf[n], self.buf[n + "'"] = self.buf[n + "'"], self.buf[n]
         self.step_no += 1
 
     def loss(self) -> float:
-        """The last forward pass's loss; raises if a device check of the products failed."""
+        """The last forward pass's loss; raises if a device check of the products has failed since the last call, once."""
         err = np.empty(1, np.int32)
         with R.with_device(self.device):
             self.stream.synchronize()
             self.buf["err"].download(err)
+            if err[0]:
+                R.check(R.lib().ccb_memset_d8(self.buf["err"].ptr, 0, 4, self.stream.h))
         if err[0]:
             raise R.CcbError(6, f"ExpertBlock: error word {int(err[0])} (64: offsets out of order or range, 16: a wait ran out)")
         return float(self.get("loss")[0])

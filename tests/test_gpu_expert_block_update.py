@@ -1,8 +1,10 @@
-"""The expert block's update on a B200: rates that change from step to step."""
+"""The expert block's update on a B200: rates that change from step to step, and
+steps whose device checks failed."""
 import numpy as np
 import pytest
 
 from cudacaml_b200 import backend_cuda as cuda
+from cudacaml_b200 import runtime as R
 from cudacaml_b200.expert_block import ExpertBlock
 
 pytestmark = pytest.mark.gpu
@@ -38,5 +40,33 @@ def test_a_schedule_of_rates_compiles_nothing(monkeypatch):
                 moved = was - rate * block.get("d" + k).astype(np.float64)
                 assert np.all(np.abs(block.get(k) - moved) <= 2.0**-22 * (np.abs(moved) + np.abs(was)) + 1e-30), k
         assert len(block.graphs) == held
+    finally:
+        block.release()
+
+
+def test_a_failed_step_is_reported_once_and_moves_nothing():
+    block = filled(48, 32, 40, [0, 20, 48])
+    try:
+        step(block, 0.5)
+        block.loss()
+        before = {k: block.get(k) for k in ExpertBlock.WEIGHTS}
+        block.put("offsets", [0, 20, 99])
+        step(block, 0.5)
+        block.put("offsets", [0, 20, 48])
+        step(block, 0.5)  # not reported yet
+        for k, was in before.items():
+            assert np.array_equal(block.get(k), was), k
+        with pytest.raises(R.CcbError, match="error word 64"):
+            block.loss()
+        block.forward()
+        first = block.loss()
+        block.backward()
+        block.update(0.25)
+        for k, was in before.items():
+            assert not np.array_equal(block.get(k), was), k
+        for _ in range(20):
+            step(block, 0.25)
+        block.forward()
+        assert block.loss() < first
     finally:
         block.release()
