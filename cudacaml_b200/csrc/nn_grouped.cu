@@ -299,6 +299,13 @@ struct Tail {  // after the ring
 constexpr unsigned kSmem = kStages * kStageBytes + sizeof(Tail) + 1024;
 static_assert(kSmem <= 232448, "shared memory of a block");
 
+// Elements of f32 operands: expert e, step k of the contraction, feature f or
+// token (column of x, for dw) t, in units of elements.
+struct Plain {
+  const float *m, *n;
+  i64 me, mk, mf, nk, nt;
+};
+
 struct P {
   ccb::TmaDesc ta, tb;  // M side, N side
   const int* off;
@@ -311,6 +318,7 @@ struct P {
   int box;              // rows of a copy of tokens
   int vec;              // out takes 16-byte stores
   unsigned polls;       // of a wait, before it gives up
+  Plain plain;          // f32 operands as the caller gave them
 };
 
 // Barriers and tiles are addressed by 32-bit shared addresses throughout: one
@@ -491,6 +499,26 @@ __device__ __forceinline__ void store32(const float* v, TO* out, i64 os, int tok
     for (int i = 0; i < 32; ++i)
       if (i < tokens) dst[i * os] = v[i];
   }
+}
+// A result of f32 operands that came out as NaN, from the operands themselves:
+// an infinite operand times a plane of the other that is 0 is NaN, also where
+// that operand is not 0. In F32, eight steps at a time up to a NaN that is one:
+// a few loads where NaN is everywhere, some K / 10 us where a row of x holds one
+// infinity (the other roles' waits last some 40 s).
+__device__ __noinline__ float again(const Plain& q, int e, i64 k0, i64 k1, i64 f, i64 t) {
+  const float *m = q.m + e * q.me + f * q.mf, *n = q.n + t * q.nt;
+  float s = 0.0f;
+  for (i64 k = k0; k < k1 && s == s; k += 8) {
+    float a[8], b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] = k + i < k1 ? m[(k + i) * q.mk] : 0.0f;
+      b[i] = k + i < k1 ? n[(k + i) * q.nk] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = fmaf(a[i], b[i], s);
+  }
+  return s;
 }
 // The same in 32 bits: lanes are features, a store is one token's 128 bytes.
 __device__ __forceinline__ void drain32(unsigned taddr, bool zero, float* out, i64 os, int tokens, int feats, int lane) {
@@ -815,6 +843,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
               const int c = 32 * other + 64 * g;
               if (c < count) store32(sum[g], out + c * p.os, p.os, count - c, p.n - f, lane);
             }
+            if constexpr (WIDE) {
+              bool nan = false;
+#pragma unroll
+              for (int g = 0; g < kTok / 64; ++g)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) nan |= sum[g][i] != sum[g][i];
+              if (nan && f + lane < p.n) {  // columns past `count` may hold anything: the loop passes them over
+                const i64 k0 = (MODE == kDw ? o.r0 : 0) + (i64)o.b0 * kBK, k1 = min(k0 + (i64)(o.b1 - o.b0) * kBK, (i64)(MODE == kDw ? o.r1 : p.k));
+                for (int c = 32 * other; c < count; c += c % 32 == 31 ? 33 : 1) {
+                  TO* at = out + lane + c * p.os;
+                  if (*at != *at) *at = again(p.plain, MODE == kDw ? 0 : o.expert, k0, k1, f + lane, MODE == kDw ? o.c0 + c : o.r0 + c);
+                }
+              }
+            }
           }
           continue;
         }
@@ -1037,7 +1079,8 @@ std::string check_dw(const ccb_nn_grouped_matmul_dw_t* a) {
 // bf16 planes by truncation (8 significant bits each, so that hi + mid + lo is
 // the number itself and no plane rounds up past the largest), and 16-bit ones
 // whose rows are not aligned, copied. Rows of a plane are dense but for the
-// last 16 bytes. A number that is not finite is its first plane alone. Bound by
+// last 16 bytes. A number that is not finite is its first plane alone (`again` has
+// the products that this makes NaN). Bound by
 // memory, 10 bytes an f32 element; 4096 rows over 8 experts of 1024 x 4096 f32
 // take 231 us in all (CUDA-core tiles: 2029).
 struct PackP {
@@ -1262,6 +1305,9 @@ int tensor_forward(const ccb_nn_grouped_matmul_t* a, Plan plan, int sms, cudaStr
     ok = ok && encode_mn(&p.ta, p.format, plan.w.p, a->n, a->k, a->experts * plan.w.planes, plan.w.row_stride, plan.w.stride, &p.a2);
   }
   if (!ok) return fail(CCB_ERR_DRIVER, me, "cuTensorMapEncodeTiled refused x or w");
+  if (a->dtype == CCB_F32)
+    p.plain = {static_cast<const float*>(a->w), static_cast<const float*>(a->x), a->w_stride, a->transpose_w ? 1 : a->w_row_stride,
+               a->transpose_w ? a->w_row_stride : 1, 1, a->x_stride};
   p.out = a->out;
   p.os = a->out_stride;
   p.vec = aligned(a->out, 16) && a->out_stride % 8 == 0;
@@ -1315,6 +1361,7 @@ int tensor_dw(const ccb_nn_grouped_matmul_dw_t* a, Plan plan, int sms, cudaStrea
   if (!encode_mn(&p.tb, p.format, plan.x.p, a->k, a->rows, plan.x.planes, plan.x.row_stride, a->rows * plan.x.row_stride, &p.b2) ||
       !encode_mn(&p.ta, p.format, plan.w.p, a->n, a->rows, plan.w.planes, plan.w.row_stride, a->rows * plan.w.row_stride, &p.a2))
     return fail(CCB_ERR_DRIVER, me, "cuTensorMapEncodeTiled refused x or dy");
+  if (a->dtype == CCB_F32) p.plain = {static_cast<const float*>(a->dy), static_cast<const float*>(a->x), 0, a->dy_stride, 1, a->x_stride, 1};
   p.out = a->out;
   p.os = a->out_row_stride;
   p.oe = a->out_stride;
