@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
       }
       if (channel) {
         vec8(v, p.gate, p.gdt, 0.0f, w);
-        act8(p.act, v);
+        act8<true>(p.act, v);
         kept.put(k * slots + gate_at, v);
       }
     }
@@ -177,11 +177,13 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__
           if (channel) {
             kept.get(k * slots + gate_at, v);
           } else {
-            if (full)
+            if (full) {
               PT::get(v, here + og, row_at<T>(p.gate, r, p.gs), w0, k);
-            else
+              act8<sizeof(T) == 4>(p.act, v);
+            } else {
               vec8(v, gate_row(p.gate, p.gdt, p.gs, r), p.gdt, 0.0f, w);
-            act8(p.act, v);
+              act8<true>(p.act, v);
+            }
           }
           mul8(b, b, v);
         }

@@ -315,10 +315,24 @@ __device__ __forceinline__ void words8(unsigned* u, const Drop& d, u64 e0, const
   }
 }
 
-// act(g) from the hardware's exponential and reciprocal: a few units in the
-// last place, below the rounding of any 16-bit result and within 1e-6 in F32.
+// act(g) from the hardware's exponential and reciprocal. The sigmoid's 2^t, t =
+// -g log2(e), has the relative error of t's rounding, |t| 2^-24: below that of
+// any 16-bit gate, but 3e-6 of an F32 gate's at -80. FINE takes t's rounding and
+// log2(e)'s along and is within ten units of 2^-24 everywhere (its gates are cut
+// to +-88, where the sigmoid is 1 or below the least normal number).
+template <bool FINE>
 __device__ __forceinline__ void act8(int act, float* g) {
-  if (act == 1) {
+  if (act == 1 && FINE) {
+#pragma unroll
+    for (int i = 0; i < kE; ++i) {
+      float x = -g[i], e;
+      asm("max.NaN.f32 %0, %0, 0fC2B00000;\n\tmin.NaN.f32 %0, %0, 0f42B00000;" : "+f"(x));  // -88, 88
+      const float t = x * 1.44269502f, rest = fmaf(x, 1.44269502f, -t) + x * 1.92596303e-8f;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+      e = fmaf(e, rest * 0.693147181f, e);
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(g[i]) : "f"(1.0f + e));
+    }
+  } else if (act == 1) {
 #pragma unroll
     for (int i = 0; i < kE; i += 2) {
       float e[2];

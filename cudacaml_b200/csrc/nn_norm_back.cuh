@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
       }
       if (channel) {
         vec8(v, p.gate, p.gdt, 0.0f, w);
-        act8(p.act, v);
+        act8<true>(p.act, v);
         kept.put(k * slots + gate_at, v);
       }
     }
@@ -293,11 +293,13 @@ __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ Ba
         if (channel) {
           kept.get(k * slots + gate_at, a);
         } else {
-          if (full)
+          if (full) {
             PT::get(a, here + og, row_at<T>(p.gate, r, p.gs), w0, k);
-          else
+            act8<sizeof(T) == 4>(p.act, a);
+          } else {
             vec8(a, gate_row(p.gate, p.gdt, p.gs, r), p.gdt, 0.0f, w);
-          act8(p.act, a);
+            act8<true>(p.act, a);
+          }
         }
         float u[kE];
         if (c2) {
