@@ -321,8 +321,10 @@ int ccb_nn_block_norm_backward_workspace(long long rows, long long cols, size_t*
  * then ends, out is undefined, the device and the stream stay usable (err may
  * be NULL). Matrix e of w starts w_stride * e elements in, its rows w_row_stride apart. At most 1024
  * experts and 2^31 - 1025 rows. f32 products are sums of 16-bit products on the
- * tensor cores, as exact as f32 arithmetic; infinite and NaN operands give what
- * f32 arithmetic gives, at a lower speed. The gradient
+ * tensor cores, as exact as f32 arithmetic for operands of 2^-110 and more: an
+ * operand is taken to a multiple of 2^-133, so that smaller ones lose their last
+ * bits (each product is off by at most 2^-133 of the other operand). Infinite and
+ * NaN operands give what f32 arithmetic gives, at a lower speed. The gradient
  * of x is the same call on dy with transpose_w flipped. Sums are in 32 bits,
  * the same bits in every run; those of a 16-bit result are the tensor cores'
  * accumulator's, which truncates: k terms of one sign come out low by up to

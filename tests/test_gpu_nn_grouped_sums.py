@@ -16,7 +16,12 @@ less, a chunk's sums and those of the chunks as above but of either sign:
 Operands of which one pair of planes carries the result: products of 4 at most
 cancel, in one MMA, which may cut four of them and the sum below 2^-23 of the
 largest; the pairs of lower planes add a hundredth of that: 5 * 4 * 2^-23 * 1.1 =
-2.7e-6, of results of 1.5e-5 or more."""
+2.7e-6, of results of 1.5e-5 or more.
+
+Operands down to the least normal number: the lowest plane that there is ends at
+2^-133, so that either operand may be off by that: 2^-133 * (|a| + |b|) for each
+product beside the bound of test_gpu_nn_grouped.py, and a product below 2^-126
+may be lost whole in each of its six terms."""
 import numpy as np
 import pytest
 import torch
@@ -93,3 +98,21 @@ def test_f32_products_by_every_pair_of_planes(term, rows, k, n):
     for got in (forward(x, ws, offsets, False).reshape(want.shape), forward(x, ws.transpose(1, 2).contiguous(), offsets, True).reshape(want.shape),
                 gradient(xs.transpose(1, 2).reshape(3 * k, rows).contiguous(), ws.reshape(3 * k, n), steps, torch.float32)):
         assert float((got.double() - want).abs().max()) <= 2.7e-6
+
+
+@pytest.mark.parametrize("small", [-100, -110, -112, -118, -123])
+@pytest.mark.parametrize("large", [0, 60, 120])
+def test_f32_products_of_very_small_operands(small, large):
+    rows, k, n = 96, 200, 72
+    offsets = [0, rows // 3, rows]
+    x, w = rand((rows, k), torch.float32, 6) * 2.0**small, rand((2, k, n), torch.float32, 7) * 2.0**large
+    dy = rand((rows, n), torch.float32, 8) * 2.0**large
+
+    def check(got, want, mag, others, terms):
+        bound = 2.0**-24 * want.abs() + (terms + 16) * 2.0**-23 * mag + 2.0**-133 * others + 6 * terms * 2.0**-126
+        assert float((got.double() - want).abs().sub(bound).max()) <= 0
+
+    ones, onesw, onesd = torch.ones_like(x), torch.ones_like(w), torch.ones_like(dy)
+    check(forward(x, w, offsets, False), *grouped(x, w, offsets), grouped(x, onesw, offsets)[1] + grouped(ones, w, offsets)[1], k)
+    check(forward(x, w.transpose(1, 2).contiguous(), offsets, True), *grouped(x, w, offsets), grouped(x, onesw, offsets)[1] + grouped(ones, w, offsets)[1], k)
+    check(gradient(x, dy, offsets, torch.float32), *grouped_dw(x, dy, offsets), grouped_dw(x, onesd, offsets)[1] + grouped_dw(ones, dy, offsets)[1], rows)
