@@ -315,7 +315,6 @@ struct P {
   i64 split_stride;     // elements from one part's result to the next
   int rows, experts, n, k, splits, format;
   int a2, b2;           // whether one copy takes two 64-wide blocks of an MN-major operand
-  int box;              // rows of a copy of tokens
   int vec;              // out takes 16-byte stores
   unsigned polls;       // of a wait, before it gives up
   Plain plain;          // f32 operands as the caller gave them
@@ -673,8 +672,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
       for (unsigned t = pair; t < tiles; t += pairs) {
         const Tile o = tile_at<MODE>(p, s.g, t);
         const int half = o.nn >> 1, f = o.f0 + (int)rank * 128, c = o.c0 + (int)rank * half, tok = o.r0 + (int)rank * half;
-        const int boxes = MODE == kDw ? (p.b2 ? 1 : half / 64) : (half + p.box - 1) / p.box;
-        const unsigned box = MODE == kDw ? (p.b2 ? 16384u : 8192u) : (unsigned)p.box * 128u, bytes = kABytes + boxes * box;
+        // tokens come as one copy of 128 rows, those that are not the tile's in vain (boxes of 16 or 64: the same up to 200
+        // rows an expert of 4096 x 1024, 94 us against 89 at 270, 106-114 against 104 at 400)
+        const unsigned bytes = kABytes + (MODE == kDw && !p.b2 ? half * 128u : kBBytes);
         int a = o.b0;
         do {
           const int z = chunk_end<CHUNK>(a, o.b1);
@@ -693,7 +693,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
                   expect_relaxed(bar, bytes);
                 }
                 const int k0 = kb * kBK;
-                unsigned sb = at + kABytes;
+                const unsigned sb = at + kABytes;
                 if (MODE == kDw) {
                   const int r = o.r0 + k0;
                   if (p.a2) {
@@ -706,7 +706,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
                     load4(sb, &p.tb, 0, r, c >> 6, pn, bar);
                   } else {
                     load4(sb, &p.tb, c, r, pn, 0, bar);
-                    if (boxes > 1) load4(sb + 8192u, &p.tb, c + 64, r, pn, 0, bar);
+                    if (half > 64) load4(sb + 8192u, &p.tb, c + 64, r, pn, 0, bar);
                   }
                 } else {
                   const int e = pm * p.experts + o.expert;
@@ -719,10 +719,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) grouped
                     load4(at + 8192u, &p.ta, f + 64, k0, e, 0, bar);
                   }
                   load4(sb, &p.tb, k0, tok, pn, 0, bar);
-                  for (int i = 1; i < boxes; ++i) {
-                    sb += box;
-                    load4(sb, &p.tb, k0, tok + i * p.box, pn, 0, bar);
-                  }
                 }
               }
               __syncwarp();
@@ -1290,12 +1286,8 @@ int tensor_forward(const ccb_nn_grouped_matmul_t* a, Plan plan, int sms, cudaStr
   tcg::P p = tensor_params(plan, a->offsets, a->err, a->dtype, a->rows, a->experts, a->k, a->n);
   char* room = static_cast<char*>(a->workspace);
   if (const int rc = settle(&plan.w, &plan.x, a->dtype, &room, sms, st, me)) return rc;
-  // tokens come in boxes of about half of what an expert has on average: a
-  // box is one copy, and a larger one than needed is read in vain
-  const i64 mean = a->rows / (a->experts < a->rows ? a->experts : a->rows);
-  p.box = mean <= 16 ? 16 : mean <= 64 ? 64 : 128;
   const i64 xd[4] = {a->k, a->rows, plan.x.planes, 1}, xs[3] = {plan.x.row_stride, a->rows * plan.x.row_stride, 8};
-  const int xb[4] = {64, p.box, 1, 1};
+  const int xb[4] = {64, 128, 1, 1};
   bool ok = tcg::encode(&p.tb, p.format, plan.x.p, 4, xd, xs, xb);
   if (a->transpose_w) {
     const i64 wd[4] = {a->k, a->n, a->experts * plan.w.planes, 1}, ws[3] = {plan.w.row_stride, plan.w.stride, 8};
