@@ -62,10 +62,12 @@ __global__ void __launch_bounds__(256) dropout_any(const __grid_constant__ Dropo
 // 16 bytes, and rows of whole pieces of 8 (dense rows are one long row, whose
 // last elements the first threads take). The generator takes half as long as
 // the memory, so they have to overlap: a thread has 32 bytes (64 with a
-// residual) on their way whatever the type, two pieces of a 16-bit one (one
-// alone left 16384 x 4096 of them at 75 us without a residual, two 73).
-// 16384 x 4096 bf16 with a residual takes 78 us (5.1 TB/s; the generator's
-// products and the ALU bound it), 8192 x 4096 f32 61 us (6.6 TB/s, HBM).
+// residual) on their way whatever the type, two pieces of a 16-bit one (with one
+// alone 16384 x 4096 of them took 1 us more).
+// 16384 x 4096 bf16 with a residual takes 80 us (5.0 TB/s), without 74 (3.6
+// TB/s): no unit is saturated (the generator's products and the ALU at half their
+// rates); some 21 KB an SM on their way are too few for the memory's latency.
+// 8192 x 4096 f32 with a residual takes 62 us (6.5 TB/s, HBM).
 template <class T>
 __global__ void __launch_bounds__(256) dropout_wide(const __grid_constant__ DropoutP p, unsigned pieces, u64 total) {
   constexpr int kWords = sizeof(T) / 2, kOnce = 4 / (int)sizeof(T);  // 16-byte words of a piece, pieces at once

@@ -276,9 +276,9 @@ void few(const FewP& q, bool wt, int sms, cudaStream_t st) {
 // Every tile is dealt out round-robin; a segment's rows are cut evenly, so
 // that no tile is a short remainder. Why pairs and 256 x 256: a step of 64 moves
 // 32 KiB into each SM for 512 cycles of its tensor pipe, and L2 feeds some 10
-// TB/s. Measured on one B200: one group of 8192 x 8192 x 4096 bf16 349-370 us
-// (1490-1576 TFLOP/s; bound by power, the clock falls to 1.6 GHz), 16384 rows
-// over 16 experts of 4096 x 4096 415-443 us, one row for each of 64 experts of
+// TB/s. Measured on one B200: one group of 8192 x 8192 x 4096 bf16 334-366 us
+// (1500-1645 TFLOP/s; bound by power, the clock falls to 1.6 GHz), 16384 rows
+// over 16 experts of 4096 x 4096 375-405 us, one row for each of 64 experts of
 // 2048 x 2048 81 us (6.6 TB/s, bound by HBM), the gradient of 64 experts'
 // 4096 x 1024 from 32 rows 103-116 us (4.6-5.2 TB/s, bound by its writes).
 namespace tcg {
@@ -1078,7 +1078,7 @@ std::string check_dw(const ccb_nn_grouped_matmul_dw_t* a) {
 // last 16 bytes. A number that is not finite is its first plane alone (`again` has
 // the products that this makes NaN). Bound by
 // memory, 10 bytes an f32 element; 4096 rows over 8 experts of 1024 x 4096 f32
-// take 231 us in all (CUDA-core tiles: 2029).
+// take 220 us in all (CUDA-core tiles: 2029).
 struct PackP {
   const void* in;
   unsigned short* out;

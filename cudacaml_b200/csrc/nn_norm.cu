@@ -18,7 +18,8 @@ struct NormP {
 
 // Rows of any length, alignment and stride, for what norm_rows does not take: a
 // block walks a row once for each statistic and once for the results, reading
-// it again each time (8192 x 4096 bf16 with gate and mask: 565 us).
+// it again each time (8192 x 4096 bf16 with gate and mask: 565 us; 4096 rows of
+// 16384 columns 1118 us, where 12288 take 152 us by norm_rows).
 template <class T, class TX, int KIND>
 __global__ void __launch_bounds__(kBlock) norm_any(const __grid_constant__ NormP p) {
   __shared__ float s[kBlock / 32];
@@ -57,10 +58,12 @@ __global__ void __launch_bounds__(kBlock) norm_any(const __grid_constant__ NormP
 // The join of rows that a group holds. HAS: 0 any arguments; else a normed
 // branch without biases and both results, with (2) a gate as a matrix of T or
 // without one (1): what a training step of an rms norm asks for, whose loops
-// have no branches left to end the compiler's schedule. Bound by instruction
-// issue: at 8192 x 4096 bf16 with a sigmoid gate and a mask 72 us (4.7 TB/s; 78
-// by HAS = 0; the generator is 17 us of it), a mask alone 62 us (70), neither 53
-// us (52; 512 columns 15 against 16).
+// have no branches left to end the compiler's schedule. Bound by latency: three
+// rows of 4096 leave 24 of 64 warps resident, which wait between a row's sums
+// (57 % of the issue slots used, no unit near its rate). At 8192 x 4096 bf16 with a
+// sigmoid gate and a mask 73 us (4.6 TB/s; 78 by HAS = 0; the generator is 17 us
+// of it), a mask alone 62 us (70), neither 53 us (52; 512 columns 15 against 16);
+// an f32 stream 99 us (4.4 TB/s), f32 throughout 177 us (3.8 TB/s).
 template <class T, class TX, int KIND, bool VEC, int PIECES, int HAS>
 __global__ void __launch_bounds__(kRowThreads) norm_rows(const __grid_constant__ NormP p, const Hold hold) {
   __shared__ __align__(16) float s[kRowThreads / 32 * 8];
@@ -263,8 +266,9 @@ struct Forward {
     if ((p.d.base & 3) || !wide(p.cols, {p.x, p.b, p.gate, p.y, p.h}, {p.xs, p.bs, p.gs, p.ys, p.hs}))
       return p.cols <= kRowThreads * kE ? rows<false, 1, 0>(p, sms, st) : rows<false, 2, 0>(p, sms, st);
     // What a thread does once a row (its sums, addresses, copies) is some 300
-    // instructions: 16 elements share them, fewer where a warp holds the row (32
-    // would spill at the registers that three rows of 4096 leave). The shape goes
+    // instructions: 16 elements share them, fewer where a warp holds the row (65536
+    // rows of 256 columns: 35 us by 8 elements a thread, 57 by 16; of 320 71 and 63;
+    // 32 would spill at the registers that three rows of 4096 leave). The shape goes
     // by the columns alone: a row's result does not depend on the rows beside it.
     const bool one = p.cols <= 256;
     if (p.b && p.post && p.y && p.h && !p.c1 && !p.c2) {

@@ -22,7 +22,8 @@ __attribute__((visibility("hidden"))) void backward_f16(int x_dtype, int kind, c
 namespace {
 
 // The gradient for any length, alignment and stride, for what norm_back_rows
-// does not take (8192 x 4096 bf16: 1767 us). A block takes every grid-th row
+// does not take (8192 x 4096 bf16: 1767 us; 4096 rows of 12288 columns 3.5 ms, of
+// 16384 5.2 ms). A block takes every grid-th row
 // and keeps its own partial sums over rows in the workspace; a thread always
 // handles the same columns of it.
 template <class T, class TX, int KIND>
@@ -106,10 +107,11 @@ __global__ void __launch_bounds__(kBlock) norm_back_any(const __grid_constant__ 
 // the sums over rows: they stay in them for all of a thread's rows. HAS: 0 any
 // arguments; else all of rms norms without biases, with (2) a gate as a matrix of
 // T or without one (1), in loops without branches that end the compiler's
-// schedule. Bound by instruction issue and latency at two rows of 4096 an SM:
-// 8192 x 4096 bf16 with gate and mask 120 us (4.5 TB/s; 135 by HAS = 0), without
-// either 88 us (94), 246 us with the layer norm's biases and a channel gate, whose
-// five sums spill registers.
+// schedule. Bound by latency: two rows of 4096 leave 15 of 64 warps resident
+// (51 % of the issue slots used). 8192 x 4096 bf16 with gate and mask 124 us (4.3
+// TB/s; 135 by HAS = 0), without either 88 us (94); an f32 stream 210 us, f32
+// throughout 309 us; with MORE a channel gate 188 us, its biases too 215 us, those
+// of the layer norm 251 us: five sums, whichever are asked for, spill registers.
 template <class T, class TX, int KIND, bool VEC, int PIECES, bool MORE, int HAS>
 __global__ void __launch_bounds__(512) norm_back_rows(const __grid_constant__ BackP p, const Hold hold) {
   __shared__ __align__(16) float s[16 * 8];
@@ -435,7 +437,10 @@ struct Backward {
   }
   // Rows of 16 elements a thread, so that a block of 512 threads (128 registers
   // each) holds two of 4096 columns and one waits for its sums while the other
-  // computes; of 8 where there are few columns. The shape does not go by the
+  // computes; of 8 where there are few columns (65536 x 256 bf16: 63 us, by 16 98;
+  // 65536 x 320 127 and 106), of an f32 stream, whose ring holds fewer rows, up to
+  // 4096 (16.8 million elements f32 of 512 columns 142 us and 152, of 2048 147 and
+  // 153, of 4096 166 and 167). The shape does not go by the
   // rows or by which sums over them are asked for (all five spill some
   // registers), so that a row's results do not either.
   template <bool MORE>
