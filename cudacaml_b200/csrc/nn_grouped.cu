@@ -343,7 +343,7 @@ struct Waiter {
   unsigned* err;
   __device__ __forceinline__ bool operator()(unsigned bar, unsigned parity) const {
     if (__all_sync(0xffffffffu, try_wait(bar, parity))) return true;
-    for (unsigned it = 0; it < polls; ++it) {
+    for (unsigned it = 1; it < polls; ++it) {
       if (__all_sync(0xffffffffu, try_wait(bar, parity))) return true;
       unsigned flag;
       asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(flag) : "r"(stop) : "memory");
@@ -503,7 +503,7 @@ __device__ __forceinline__ void store32(const float* v, TO* out, i64 os, int tok
 // an infinite operand times a plane of the other that is 0 is NaN, also where
 // that operand is not 0. In F32, eight steps at a time up to a NaN that is one:
 // a few loads where NaN is everywhere, some K / 10 us where a row of x holds one
-// infinity (the other roles' waits last some 40 s).
+// infinity (the other roles' waits last 16 s).
 __device__ __noinline__ float again(const Plain& q, int e, i64 k0, i64 k1, i64 f, i64 t) {
   const float *m = q.m + e * q.me + f * q.mf, *n = q.n + t * q.nt;
   float s = 0.0f;

@@ -468,7 +468,7 @@ def grouped_matmul_dw(x, dy, offsets, out, *, workspace=None, err=None, stream=N
 def wait_polls(polls: int = 0) -> None:
     """How often a wait inside the grouped products polls before it gives up
     (bit 16 of ``err``, the output undefined, the stream usable), for the calls
-    that follow; 0 is the default, 2**22."""
+    that follow; 0 is the default, 2**22 (4 us each: 16 s)."""
     if not 0 <= polls < 1 << 32:
         raise ValueError(f"nn.wait_polls: {polls} is outside [0, 2^32)")
     R.check((R._LIB or R.lib()).ccb_nn_wait_polls(polls))

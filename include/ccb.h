@@ -361,7 +361,8 @@ int ccb_nn_grouped_matmul_dw(const ccb_nn_grouped_matmul_dw_t* a, void* stream);
 int ccb_nn_grouped_matmul_dw_workspace(const ccb_nn_grouped_matmul_dw_t* a, size_t* bytes);
 
 /* How often a wait inside the grouped products polls before it gives up, for
- * the calls that this process issues from here on; 0: the default, 2^22. */
+ * the calls that this process issues from here on; 0: the default, 2^22
+ * (4 us each: 16 s). */
 int ccb_nn_wait_polls(unsigned polls);
 
 /* ---------------------------------------------------------------- peer memory and the cross-rank sum

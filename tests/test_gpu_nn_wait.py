@@ -1,8 +1,9 @@
 """Grouped products whose waits run out on a B200: the call ends, says so in its
 error word, and leaves the device, the stream and the next call as they were.
 
-The bound of a wait is set to one poll, which a draining warp passes long before
-the 256 steps of its tile's contraction are multiplied."""
+The bound of a wait is set to a few polls, of 4 us each; a draining warp waits for
+a tile's contraction, at the two larger sizes 100 us and more, or a chunk of it,
+from 7 us on for F32."""
 import pytest
 import torch
 
@@ -46,7 +47,7 @@ def calls(t, rows, k, n):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("rows,k,n", [(512, 16384, 4096), (16384, 1024, 4096), (700, 264, 520)])
+@pytest.mark.parametrize("rows,k,n", [(512, 65536, 2048), (131072, 512, 2048), (700, 264, 520)])
 def test_a_wait_that_runs_out_ends_the_call_and_is_reported(dtype, rows, k, n):
     every = calls(TYPES[dtype], rows, k, n)
     err = torch.zeros(1, dtype=torch.int32, device=DEV)
@@ -54,7 +55,7 @@ def test_a_wait_that_runs_out_ends_the_call_and_is_reported(dtype, rows, k, n):
     assert int(err) == 0
     seen = 0
     try:
-        for polls in (1, 2, 8):
+        for polls in (1, 2, 3):
             nn.wait_polls(polls)
             for f, want in zip(every, clean):
                 for _ in range(5):
@@ -66,7 +67,7 @@ def test_a_wait_that_runs_out_ends_the_call_and_is_reported(dtype, rows, k, n):
                     seen |= got
     finally:
         nn.wait_polls()
-    assert seen == 16 or rows < 1000 and k < 1000
+    assert seen == 16 or rows == 700
     err.zero_()
     for f, want in zip(every, clean):
         assert torch.equal(f(err), want)
